@@ -148,7 +148,7 @@ def _pack_plain(x):
     e = torch.where(amax > 0, torch.clamp(ex - 9 + (m > 0.875).int(), -110, 120), -110)
     q = xb * _two_to(-e)[:, :, None]
     c = q.to(torch.float8_e4m3fn).view(torch.uint8)
-    c = torch.where((c & 127 == 0) & (q != 0), c | 1, c)
+    c = torch.where((c & 127 == 0) & (xb != 0), c | 1, c)
     c = torch.where(fin, c, c | 127)
     return c.view(M, nb * 32)[:, :N].contiguous(), (e + 127).to(torch.uint8)
 
