@@ -1,0 +1,426 @@
+// Grouped products: one layer of every expert over its own rows.  Rows are sorted by expert, expert
+// e has rows offs[e] .. offs[e + 1) (device memory: no host synchronization, ragged and empty groups
+// allowed); rows behind offs[E] are not touched.
+//
+//   group_nt     out[p, n] = epi(sum_k A[row(p), k] B[e, n, k])      A, B bf16, K-contiguous
+//                forward:  A = x (row(p) = p, or src[p] / top_k: the sorted slot's token), B = w,
+//                          epi = + bias[e, n], relu
+//                gradient: A = dz, B = w^T, epi = * scale, masked where the layer input is not > 0
+//                          (the input in bf16 or as 8-bit codes)
+//   group_wgrad  dw[e, n, k] = sum_p dz[p, n] x[row(p), k],  db[e, n] = sum_p dz[p, n]    (fp32)
+//                x in bf16, or 8-bit codes with one scale per 32 columns (act8.h)
+//
+// A workgroup finds its expert by a scan over the group sizes in its own registers.  Accumulation is
+// fp32 on MFMA; nothing is summed by atomics.
+#include "act8.h"
+
+struct GroupNtArgs {
+  const bf16* a;           // [rows, K], row stride lda
+  const bf16* b;           // [E, N, K], row stride ldb, expert stride es
+  const float* bias;       // [E, N] or null
+  const void* mask;        // null, bf16 [S, N] or codes [S, N], row stride ldm
+  void* out;               // [S, N], row stride ldo, bf16 or fp32
+  const int* offs;         // [E + 1]
+  const int* src;          // [S] or null
+  long lda, ldb, es, ldm, ldo;
+  int S, rows, K, N, E, top_k, relu, mask8, out_f32;
+  float scale;
+};
+
+struct GroupWgArgs {
+  const bf16* dz;          // [S, N], row stride ldz
+  const void* x;           // bf16 or codes [rows, K], row stride ldx
+  const uint8_t* xs;       // scales [rows, ceil(K / 32)] (codes), else null
+  const int* offs;
+  const int* src;
+  float* dw;               // [E, N, K]
+  float* db;               // [E, N] or null
+  float* ws;               // [ns, E, N, K] + [ns, E, N] (ns > 1)
+  long ldz, ldx;
+  int S, rows, K, N, E, top_k, ns;
+};
+
+// The offsets are the caller's device data: whatever they hold, no row outside [0, S) is touched.
+__device__ __forceinline__ void group_rows(const int* offs, int e, int S, int& lo, int& hi) {
+  lo = min(max(offs[e], 0), S);
+  hi = min(max(offs[e + 1], lo), S);
+}
+
+// Row tile `tm` (of BM rows) over all groups in order: its expert, first row and the group's end.
+template <int BM>
+__device__ __forceinline__ bool group_find(const int* offs, int E, int S, int tm, int& e, int& r0, int& r1) {
+  const int lane = threadIdx.x & 63;
+  int run = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    int lo = 0, hi = 0;
+    if (e0 + lane < E) group_rows(offs, e0 + lane, S, lo, hi);
+    const int n = (hi - lo + BM - 1) / BM;
+    int inc = n;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(inc, d);
+      if (lane >= d) inc += u;
+    }
+    const unsigned long long past = __ballot(run + inc > tm);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      e = e0 + l;
+      r0 = __shfl(lo, l) + (tm - run - __shfl(inc - n, l)) * BM;
+      r1 = __shfl(hi, l);
+      e = __builtin_amdgcn_readfirstlane(e);
+      r0 = __builtin_amdgcn_readfirstlane(r0);
+      r1 = __builtin_amdgcn_readfirstlane(r1);
+      return true;
+    }
+    run += __shfl(inc, 63);
+  }
+  return false;
+}
+
+// the row of x behind sorted place p, or -1 (a slot that is none of the rows reads as zeros)
+__device__ __forceinline__ int group_row(const int* src, int p, int rows, int top_k) {
+  if (!src) return p;
+  const int s = src[p];
+  const int r = s / top_k;
+  return s >= 0 && r < rows ? r : -1;
+}
+
+// 8 elements of a row from column c, zeros past n (VEC: 16-byte aligned, n a multiple of 8)
+template <bool VEC>
+__device__ __forceinline__ bf16x8 load8_bf(const bf16* row, int c, int n) {
+  bf16x8 v = {};
+  if (!row || c >= n) return v;
+  if (VEC) return *reinterpret_cast<const bf16x8*>(row + c);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j < n) v[j] = row[c + j];
+  return v;
+}
+template <bool VEC>
+__device__ __forceinline__ uint2 load8_code(const uint8_t* row, int c, int n) {
+  uint2 v = make_uint2(0, 0);
+  if (!row || c >= n) return v;
+  if (VEC) return *reinterpret_cast<const uint2*>(row + c);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j < n) {
+      const uint32_t b = row[c + j];
+      if (j < 4) v.x |= b << (8 * j);
+      else v.y |= b << (8 * (j - 4));
+    }
+  return v;
+}
+
+// ------------------------------------------------------------------ NT product, 128 x 128 tile
+// 256 threads = 4 waves of 64 x 64 outputs (4 x 4 MFMA 16x16x32), 64-deep steps through two LDS
+// buffers of 32 KB: the next step's 16-byte row chunks are in registers while this one multiplies.
+// LDS image: rows of 64 elements (128 B), 16-byte chunk c of row r at c ^ ((r >> 1) & 7).
+constexpr int GN_B = 128, GN_K = 64, GN_PANEL = GN_B * GN_K * 2;
+
+template <bool VEC>
+__global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_n) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * GN_PANEL];
+  int e, r0, r1;
+  if (!group_find<GN_B>(g.offs, g.E, g.S, blockIdx.x / tiles_n, e, r0, r1)) return;
+  const int n0 = (blockIdx.x % tiles_n) * GN_B;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  const int fr = lane & 15, fq = lane >> 4;
+  // staging: chunk tid & 7 of rows (tid >> 3) + 32 i
+  const int ch = tid & 7, sr = tid >> 3;
+  const bf16* pa[4];
+  const bf16* pb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = r0 + sr + 32 * i, n = n0 + sr + 32 * i;
+    const int row = p < r1 ? group_row(g.src, p, g.rows, g.top_k) : -1;
+    pa[i] = row >= 0 ? g.a + (size_t)row * g.lda : nullptr;
+    pb[i] = n < g.N ? g.b + (size_t)e * g.es + (size_t)n * g.ldb : nullptr;
+  }
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bf16x8 ra[4], rb[4];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ra[i] = load8_bf<VEC>(pa[i], k0 + ch * 8, g.K);
+      rb[i] = load8_bf<VEC>(pb[i], k0 + ch * 8, g.K);
+    }
+  };
+  auto stage = [&](int buf) {
+    char* s = smem + buf * 2 * GN_PANEL;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = sr + 32 * i, o = r * 128 + ((ch ^ ((r >> 1) & 7)) << 4);
+      *reinterpret_cast<bf16x8*>(s + o) = ra[i];
+      *reinterpret_cast<bf16x8*>(s + GN_PANEL + o) = rb[i];
+    }
+  };
+  const int nt = (g.K + GN_K - 1) / GN_K;
+  const int sw = (fr >> 1) & 7;
+  if (nt > 0) {
+    fetch(0);
+    stage(0);
+  }
+  for (int t = 0; t < nt; ++t) {
+    __syncthreads();
+    if (t + 1 < nt) fetch((t + 1) * GN_K);
+    const char* s = smem + (t & 1) * 2 * GN_PANEL;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8 fa[4], fb[4];
+      const int c = ((ks * 4 + fq) ^ sw) << 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        fa[i] = *reinterpret_cast<const bf16x8*>(s + (wr + i * 16 + fr) * 128 + c);
+        fb[i] = *reinterpret_cast<const bf16x8*>(s + GN_PANEL + (wc + i * 16 + fr) * 128 + c);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    }
+    if (t + 1 < nt) stage((t + 1) & 1);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + wc + j * 16 + fr;
+    if (n >= g.N) continue;
+    const float bias = g.bias ? g.bias[(size_t)e * g.N + n] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int p = r0 + wr + i * 16 + fq * 4 + q;
+        if (p >= r1) continue;
+        float v = acc[i][j][q] * g.scale + bias;
+        if (g.relu && v < 0.f) v = 0.f;        // (NaN stays)
+        if (g.mask) {
+          const size_t m = (size_t)p * g.ldm + n;
+          const bool on = g.mask8 ? a8_positive(reinterpret_cast<const uint8_t*>(g.mask)[m])
+                                  : bf2f(reinterpret_cast<const bf16*>(g.mask)[m]) > 0.f;
+          if (!on) v = 0.f;
+        }
+        const size_t o = (size_t)p * g.ldo + n;
+        if (g.out_f32) reinterpret_cast<float*>(g.out)[o] = v;
+        else reinterpret_cast<bf16*>(g.out)[o] = f2bf(v);
+      }
+  }
+}
+
+HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
+  const GroupNtArgs g = *gp;
+  if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
+  if (g.S == 0 || g.N == 0) return 0;
+  const bool vec = ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.K % 8 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0 &&
+                   g.es % 8 == 0;
+  const int tn = (g.N + GN_B - 1) / GN_B;
+  const long blocks = (long)(g.S / GN_B + g.E) * tn;      // (each group adds less than one tile)
+  if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
+  if (vec) hipLaunchKernelGGL(group_nt_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
+  else hipLaunchKernelGGL(group_nt_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
+  HFM_LAUNCH_CHECK();
+}
+
+// ------------------------------------------------------------------ weight gradient, 128 x 128 tile
+// The reduction runs over rows, both operands are row-major: a thread takes an 8 x 8 block (8 rows
+// p, 8 columns) into registers, transposes it (bf16 pairs, one byte permute per output word) and
+// writes 8 chunks of 8 p-contiguous elements into the LDS image [column][64 p], which the MFMA
+// fragments read like the NT kernel's.  256 threads = 128 blocks of dz + 128 of x per 64-row step.
+// Image swizzle: 16-byte chunk m of row n at m ^ s(n), s(n) = ((n >> 1) ^ (n >> 3)) & 7: the 8 rows a
+// thread writes and the 16 rows a fragment reads both spread over the banks.
+__device__ __forceinline__ int wg_swz(int n) { return ((n >> 1) ^ (n >> 3)) & 7; }
+
+// in[m] = 8 columns of row m  ->  out[c] = 8 rows of column c
+__device__ __forceinline__ void transpose8(const uint4 (&in)[8], uint4 (&out)[8]) {
+#pragma unroll
+  for (int c2 = 0; c2 < 4; ++c2) {
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int m2 = 0; m2 < 4; ++m2) {
+      const uint32_t a = reinterpret_cast<const uint32_t*>(&in[2 * m2])[c2];
+      const uint32_t b = reinterpret_cast<const uint32_t*>(&in[2 * m2 + 1])[c2];
+      lo[m2] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+      hi[m2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+    out[2 * c2] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    out[2 * c2 + 1] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  }
+}
+
+template <bool VEC, bool X8>
+__global__ void __launch_bounds__(256) group_wgrad_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * GN_PANEL];
+  int bid = blockIdx.x;
+  const int kt = bid % tiles_k;
+  bid /= tiles_k;
+  const int ntile = bid % tiles_n;
+  bid /= tiles_n;
+  const int e = bid % g.E, sp = bid / g.E;
+  int lo, hi;
+  group_rows(g.offs, e, g.S, lo, hi);
+  // this split's rows: whole 64-row steps
+  const int steps = (hi - lo + 63) / 64, per = (steps + g.ns - 1) / g.ns;
+  const int p0 = lo + min(steps, sp * per) * 64, p1 = min(hi, lo + min(steps, (sp + 1) * per) * 64);
+  const int n0 = ntile * GN_B, k0 = kt * GN_B;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
+  const int fr = lane & 15, fq = lane >> 4;
+  // staging block: waves 0, 1 take dz, waves 2, 3 take x; 16 column blocks x 8 row blocks
+  const bool isx = wave >= 2;
+  const int cb = lane & 15, mb = (wave & 1) * 4 + (lane >> 4);
+  const int col = (isx ? k0 : n0) + cb * 8;
+  const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
+  uint4 in[8];
+  auto fetch = [&](int pbase) {
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const int p = pbase + mb * 8 + m;
+      bf16x8 v = {};
+      if (p < p1) {
+        if (!isx) {
+          v = load8_bf<VEC>(g.dz + (size_t)p * g.ldz, col, g.N);
+        } else {
+          const int row = group_row(g.src, p, g.rows, g.top_k);
+          if (row >= 0) {
+            if (X8) {
+              const uint2 w = load8_code<VEC>(reinterpret_cast<const uint8_t*>(g.x) + (size_t)row * g.ldx, col, g.K);
+              const float s = col < g.K ? a8_scale(g.xs[(size_t)row * sblk + col / A8_BLOCK]) : 0.f;
+              float f[8];
+              a8_unpack8(w, s, f);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = f2bf(f[j]);
+            } else {
+              v = load8_bf<VEC>(reinterpret_cast<const bf16*>(g.x) + (size_t)row * g.ldx, col, g.K);
+            }
+          }
+        }
+      }
+      in[m] = *reinterpret_cast<const uint4*>(&v);
+    }
+  };
+  auto stage = [&](int buf) {
+    char* s = smem + buf * 2 * GN_PANEL + (isx ? GN_PANEL : 0);
+    uint4 o[8];
+    transpose8(in, o);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int n = cb * 8 + c;
+      *reinterpret_cast<uint4*>(s + n * 128 + ((mb ^ wg_swz(n)) << 4)) = o[c];
+    }
+  };
+  f32x4 acc[4][4], accb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    accb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // db: one more product, with a column of ones (first k tile, waves of its first columns)
+  const bool sum = g.db != nullptr && kt == 0 && wc == 0;
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.f);
+  const int nt = p1 > p0 ? (p1 - p0 + 63) / 64 : 0;
+  if (nt > 0) {
+    fetch(p0);
+    stage(0);
+  }
+  for (int t = 0; t < nt; ++t) {
+    __syncthreads();
+    if (t + 1 < nt) fetch(p0 + (t + 1) * 64);
+    const char* s = smem + (t & 1) * 2 * GN_PANEL;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8 fa[4], fb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = wr + i * 16 + fr, b = wc + i * 16 + fr;
+        fa[i] = *reinterpret_cast<const bf16x8*>(s + a * 128 + (((ks * 4 + fq) ^ wg_swz(a)) << 4));
+        fb[i] = *reinterpret_cast<const bf16x8*>(s + GN_PANEL + b * 128 + (((ks * 4 + fq) ^ wg_swz(b)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+      if (sum) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], ones, accb[i], 0, 0, 0);
+      }
+    }
+    if (t + 1 < nt) stage((t + 1) & 1);
+  }
+  const size_t en = (size_t)g.E * g.N;
+  float* dw = g.ns > 1 ? g.ws + (size_t)sp * en * g.K : g.dw;
+  float* db = g.ns > 1 ? g.ws + (size_t)g.ns * en * g.K + sp * en : g.db;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = n0 + wr + i * 16 + fq * 4 + q;
+      if (n >= g.N) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + wc + j * 16 + fr;
+        if (k < g.K) dw[((size_t)e * g.N + n) * g.K + k] = acc[i][j][q];
+      }
+      if (sum && fr == 0) db[(size_t)e * g.N + n] = accb[i][q];
+    }
+}
+
+// dw = sum of the ns partial products in order (and db)
+__global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
+  const size_t nw = (size_t)g.E * g.N * g.K, nb = g.db ? (size_t)g.E * g.N : 0;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= nw + nb) return;
+  const float* s = i < nw ? g.ws + i : g.ws + (size_t)g.ns * nw + (i - nw);
+  const size_t step = i < nw ? nw : (size_t)g.E * g.N;
+  float v = s[0];
+  for (int q = 1; q < g.ns; ++q) v += s[q * step];
+  (i < nw ? g.dw[i] : g.db[i - nw]) = v;
+}
+
+// Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
+// 64 rows on average.
+HFM_API int hfm_group_wgrad_splits(int S, int N, int K, int E) {
+  const long tiles = (long)E * ((N + GN_B - 1) / GN_B) * ((K + GN_B - 1) / GN_B);
+  if (tiles <= 0) return 1;
+  long ns = 512 / tiles;
+  const long most = (long)S / E / 512;
+  if (ns > most) ns = most;
+  if (ns > 32) ns = 32;
+  return ns < 1 ? 1 : (int)ns;
+}
+
+HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
+  GroupWgArgs g = *gp;
+  if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
+  if (g.N == 0) return 0;
+  g.ns = hfm_group_wgrad_splits(g.S, g.N, g.K, g.E);
+  if (g.ns > 1 && !g.ws) return (int)hipErrorInvalidValue;
+  const bool x8 = g.xs != nullptr;
+  const bool vec = (uintptr_t)g.dz % 16 == 0 && g.N % 8 == 0 && g.ldz % 8 == 0 && (uintptr_t)g.x % (x8 ? 8 : 16) == 0 &&
+                   g.K % 8 == 0 && g.ldx % 8 == 0;
+  const int tn = (g.N + GN_B - 1) / GN_B, tk = g.K > 0 ? (g.K + GN_B - 1) / GN_B : 1;
+  const long blocks = (long)tn * tk * g.E * g.ns;
+  if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks), blk(256);
+  if (x8) {
+    if (vec) hipLaunchKernelGGL((group_wgrad_kernel<true, true>), grid, blk, 0, st, g, tn, tk);
+    else hipLaunchKernelGGL((group_wgrad_kernel<false, true>), grid, blk, 0, st, g, tn, tk);
+  } else {
+    if (vec) hipLaunchKernelGGL((group_wgrad_kernel<true, false>), grid, blk, 0, st, g, tn, tk);
+    else hipLaunchKernelGGL((group_wgrad_kernel<false, false>), grid, blk, 0, st, g, tn, tk);
+  }
+  if (g.ns > 1) {
+    const size_t n = (size_t)g.E * g.N * g.K + (g.db ? (size_t)g.E * g.N : 0);
+    const size_t nb = (n + 255) / 256;
+    if (nb > 0x7FFFFFFFull) return (int)hipErrorInvalidValue;
+    hipLaunchKernelGGL(group_wgrad_sum_kernel, dim3((unsigned)nb), dim3(256), 0, st, g);
+  }
+  HFM_LAUNCH_CHECK();
+}
+HFM_API int hfm_group_nt_args_bytes() { return (int)sizeof(GroupNtArgs); }
+HFM_API int hfm_group_wg_args_bytes() { return (int)sizeof(GroupWgArgs); }

@@ -203,7 +203,62 @@ class WgJob(C.Structure):
                 ("splitk", c_int), ("kchunk", c_int), ("task0", c_int), ("pad", c_int)]
 
 
+class RouteArgs(C.Structure):
+    _fields_ = [("logits", c_void_p), ("valid", c_void_p), ("expert", c_void_p), ("weight", c_void_p),
+                ("pos", c_void_p), ("src", c_void_p), ("offs", c_void_p), ("bh", c_void_p), ("wpre", c_void_p),
+                ("ld", c_long), ("T", c_int), ("E", c_int), ("k", c_int), ("renorm", c_int), ("bf", c_int),
+                ("nblk", c_int), ("tpb", c_int)]
+
+
+class RouteBwdArgs(C.Structure):
+    _fields_ = [("logits", c_void_p), ("expert", c_void_p), ("weight", c_void_p), ("dweight", c_void_p),
+                ("dlogits", c_void_p), ("ld", c_long), ("ldo", c_long), ("T", c_int), ("E", c_int), ("k", c_int),
+                ("renorm", c_int), ("bf", c_int)]
+
+
+class ExchArgs(C.Structure):
+    _fields_ = [("a", c_void_p), ("b", c_void_p), ("out", c_void_p), ("pos", c_void_p), ("weight", c_void_p),
+                ("dweight", c_void_p), ("lda", c_long), ("ldb", c_long), ("ldo", c_long), ("T", c_int),
+                ("k", c_int), ("D", c_int), ("S", c_int), ("bf", c_int), ("vec", c_int)]
+
+
+class Act8Args(C.Structure):
+    _fields_ = [("x", c_void_p), ("codes", c_void_p), ("scales", c_void_p), ("out", c_void_p), ("ld", c_long),
+                ("ldc", c_long), ("M", c_int), ("N", c_int), ("bf", c_int)]
+
+
+class GroupNtArgs(C.Structure):
+    _fields_ = [("a", c_void_p), ("b", c_void_p), ("bias", c_void_p), ("mask", c_void_p), ("out", c_void_p),
+                ("offs", c_void_p), ("src", c_void_p), ("lda", c_long), ("ldb", c_long), ("es", c_long),
+                ("ldm", c_long), ("ldo", c_long), ("S", c_int), ("rows", c_int), ("K", c_int), ("N", c_int),
+                ("E", c_int), ("top_k", c_int), ("relu", c_int), ("mask8", c_int), ("out_f32", c_int),
+                ("scale", c_float)]
+
+
+class GroupWgArgs(C.Structure):
+    _fields_ = [("dz", c_void_p), ("x", c_void_p), ("xs", c_void_p), ("offs", c_void_p), ("src", c_void_p),
+                ("dw", c_void_p), ("db", c_void_p), ("ws", c_void_p), ("ldz", c_long), ("ldx", c_long),
+                ("S", c_int), ("rows", c_int), ("K", c_int), ("N", c_int), ("E", c_int), ("top_k", c_int),
+                ("ns", c_int)]
+
+
 _SIGS = {
+    "hfm_route_blocks": [c_int, c_int],
+    "hfm_route_ws_ints": [c_int, c_int],
+    "hfm_route": [C.POINTER(RouteArgs), c_void_p],
+    "hfm_route_bwd": [C.POINTER(RouteBwdArgs), c_void_p],
+    "hfm_route_args_bytes": [],
+    "hfm_route_bwd_args_bytes": [],
+    "hfm_exchange": [c_int, C.POINTER(ExchArgs), c_void_p],
+    "hfm_exch_args_bytes": [],
+    "hfm_act8_pack": [C.POINTER(Act8Args), c_void_p],
+    "hfm_act8_unpack": [C.POINTER(Act8Args), c_void_p],
+    "hfm_act8_args_bytes": [],
+    "hfm_group_nt": [C.POINTER(GroupNtArgs), c_void_p],
+    "hfm_group_nt_args_bytes": [],
+    "hfm_group_wgrad_splits": [c_int, c_int, c_int, c_int],
+    "hfm_group_wgrad": [C.POINTER(GroupWgArgs), c_void_p],
+    "hfm_group_wg_args_bytes": [],
     "hfm_fm_fwd": [c_void_p] * 5 + [c_int] * 4 + [c_void_p] * 6 + [c_long, c_long, c_void_p, c_int,
                                                                       c_void_p],
     "hfm_fm_bwd_sorted": [c_void_p] * 7 + [c_int] * 4 + [c_void_p, c_void_p],
@@ -357,7 +412,10 @@ def get_lib():
                            ("hfm_sparse_fused_args_bytes", SfArgs),
                            ("hfm_sh_apply_args_bytes", ShApplyArgs),
                            ("hfm_sh_dense_args_bytes", ShDenseArgs), ("hfm_fs_job_bytes", FsJob),
-                           ("hfm_sh_route_batch_bytes", ShRouteBatch)):
+                           ("hfm_sh_route_batch_bytes", ShRouteBatch),
+                           ("hfm_route_args_bytes", RouteArgs), ("hfm_route_bwd_args_bytes", RouteBwdArgs),
+                           ("hfm_exch_args_bytes", ExchArgs), ("hfm_act8_args_bytes", Act8Args),
+                           ("hfm_group_nt_args_bytes", GroupNtArgs), ("hfm_group_wg_args_bytes", GroupWgArgs)):
             n = getattr(lib, cname)()
             if n != C.sizeof(pys):
                 raise RuntimeError(f"ABI mismatch {pys.__name__}: C {n} vs ctypes {C.sizeof(pys)}")

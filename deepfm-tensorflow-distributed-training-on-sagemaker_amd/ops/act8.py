@@ -1,0 +1,83 @@
+"""Activations kept in 8 bits for the backward pass (csrc/kernels/act8.hip).
+
+``pack`` turns [M, N] activations into OCP e4m3 codes and one power-of-two scale per row and 32
+columns: 1.03 bytes a value instead of 2 or 4.  A block's scale is the smallest 2^e (e in [-110,
+120]) that keeps its largest finite magnitude within 448; a code is the e4m3 value nearest to
+x / 2^e (ties to even).  Two rules serve the backward pass: a value that is not zero never becomes
+a zero (it takes the smallest code of its sign instead), so a relu or dropout mask read from the
+codes is the mask of the activations themselves; and infinities and NaN become NaN, in their own
+place only.
+
+The codes go into the gradient products as they are: ``experts.group_wgrad`` takes an ``Act8`` for
+its input, ``experts.group_dgrad`` for its mask.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from ._lib import Act8Args, check, ptr
+from .checks import contiguous, launch, need, out_or_new, row_stride, rows2d
+
+BLOCK = 32            # columns per scale
+
+
+class Act8(NamedTuple):
+    """8-bit activations: ``codes`` uint8 [M, N] (e4m3; rows may be strided), ``scales`` uint8
+    [M, ceil(N / 32)], a scale's exponent + 127."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def scale_cols(N: int) -> int:
+    return -(-N // BLOCK)
+
+
+def empty(M: int, N: int, device) -> Act8:
+    """Uninitialised storage for [M, N] activations."""
+    return Act8(torch.empty(M, N, dtype=torch.uint8, device=device),
+                torch.empty(M, scale_cols(N), dtype=torch.uint8, device=device))
+
+
+def check_act8(a: Act8, M: int, N: int, what: str) -> None:
+    need(isinstance(a, Act8), f"{what} must be an Act8")
+    rows2d(a.codes, f"{what}.codes", (torch.uint8,), M, N)
+    need(a.scales.dtype == torch.uint8 and tuple(a.scales.shape) == (M, scale_cols(N)) and contiguous(a.scales),
+         f"{what}.scales must be a contiguous uint8 [{M}, {scale_cols(N)}]")
+
+
+_VALUES = (torch.float32, torch.bfloat16)
+
+
+def pack(x: torch.Tensor, out: Optional[Act8] = None) -> Act8:
+    """x [M, N] (fp32 or bf16, rows may be strided) -> ``Act8``."""
+    rows2d(x, "x", _VALUES)
+    M, N = x.shape
+    if out is None:
+        out = empty(M, N, x.device)
+    else:
+        check_act8(out, M, N, "out")
+    a = Act8Args(ptr(x), ptr(out.codes), ptr(out.scales), 0, row_stride(x), row_stride(out.codes), M, N,
+                 1 if x.dtype == torch.bfloat16 else 0)
+    with launch("act8.pack", x, *out) as st:
+        check(_lib.get_lib().hfm_act8_pack(C.byref(a), st), "act8_pack")
+    return out
+
+
+def unpack(a: Act8, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values that ``a`` stands for, in fp32 or bf16 (exact in both, but where a value of a
+    block with the smallest scales lies below the type's normal range)."""
+    need(isinstance(a, Act8), "a must be an Act8")
+    need(a.codes.dim() == 2, "a.codes must be 2-D")
+    M, N = a.codes.shape
+    check_act8(a, M, N, "a")
+    need(dtype in _VALUES, f"unpack to fp32 or bf16, not {dtype}")
+    out = out_or_new(out, (M, N), dtype, a.codes.device)
+    args = Act8Args(0, ptr(a.codes), ptr(a.scales), ptr(out), row_stride(out), row_stride(a.codes), M, N,
+                    1 if dtype == torch.bfloat16 else 0)
+    with launch("act8.unpack", *a, out) as st:
+        check(_lib.get_lib().hfm_act8_unpack(C.byref(args), st), "act8_unpack")
+    return out

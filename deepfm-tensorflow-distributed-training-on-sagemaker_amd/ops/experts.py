@@ -1,0 +1,301 @@
+"""Mixture-of-experts operators (csrc/kernels/experts.hip, group.hip): routing, the exchange of rows
+between token order and expert order, and the experts' products, each with its gradient.
+
+One training step of a layer of E experts, of which every token takes ``top_k``::
+
+    r  = route(logits, top_k)                       # choices, weights, expert order
+    h  = group_linear(x, w1, b1, r.offs, relu=True, src=r.src, top_k=top_k)
+    ys = group_linear(h, w2, b2, r.offs)
+    y  = combine(ys, r)
+    ...
+    dys, dweight = combine_bwd(dy, ys, r)
+    dw2, db2 = group_wgrad(dys, h, r.offs)
+    dh  = group_dgrad(dys, w2t, r.offs, mask=h)
+    dw1, db1 = group_wgrad(dh, x, r.offs, src=r.src, top_k=top_k)
+    dx  = dispatch_bwd(group_dgrad(dh, w1t, r.offs), r)
+    dlogits = route_bwd(logits, r, dweight)
+
+``x`` goes into the first product through ``src`` (no copy in expert order); ``dispatch`` makes that
+copy where one is wanted.  ``h`` (or ``x``) can be kept in 8 bits between the passes: ``act8.pack``
+after the forward, and the ``Act8`` in place of ``h`` in ``group_wgrad`` and ``group_dgrad``.
+
+Expert order.  Slot s = t * top_k + j is choice j of token t.  ``src`` lists the live slots by expert,
+in slot order within an expert; ``offs[e]`` is the first place of expert e and ``offs[E]`` the number
+of live slots; ``pos`` is the place of each slot.  Group sizes stay on the GPU: a call takes ``S``
+rows at most and no result depends on rows from ``offs[E]`` on, which keep what they held (a result
+that the call allocated holds nothing there).
+
+Results are allocated by the call unless ``out`` is given; workspaces come from torch's allocator on
+the current stream, so calls on several streams and in several graphs share nothing.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from ._lib import ExchArgs, GroupNtArgs, GroupWgArgs, RouteArgs, RouteBwdArgs, check, ptr
+from .act8 import Act8, check_act8
+from .checks import flat, launch, need, out_or_new, row_stride, rows2d
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 16
+_MAX_SLOTS = 1 << 30
+_VALUES = (torch.float32, torch.bfloat16)
+_BF = (torch.bfloat16,)
+_EX_DISPATCH, _EX_DISPATCH_BWD, _EX_COMBINE, _EX_COMBINE_BWD = 0, 1, 2, 3
+
+
+class Routes(NamedTuple):
+    """Choices and expert order of T tokens (see the module's text): ``expert`` int32 [T, top_k]
+    (-1: none), ``weight`` fp32 [T, top_k], ``pos`` int32 [T, top_k] (-1: none), ``src`` int32
+    [T * top_k] (-1 behind the last live slot), ``offs`` int32 [E + 1]."""
+    expert: torch.Tensor
+    weight: torch.Tensor
+    pos: torch.Tensor
+    src: torch.Tensor
+    offs: torch.Tensor
+
+
+def _bf(t) -> int:
+    return 1 if t.dtype == torch.bfloat16 else 0
+
+
+def _check_gate(logits, top_k):
+    rows2d(logits, "logits", _VALUES)
+    T, E = logits.shape
+    need(1 <= E <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts, got {E}")
+    need(isinstance(top_k, int) and 1 <= top_k <= min(E, MAX_TOP_K),
+         f"top_k must be 1 to {min(E, MAX_TOP_K)}, got {top_k}")
+    need(T * top_k <= _MAX_SLOTS, f"{T} x {top_k} slots are more than {_MAX_SLOTS}")
+    return T, E
+
+
+def _check_routes(r: Routes, T: Optional[int] = None) -> Tuple[int, int]:
+    need(isinstance(r, Routes), "routes must be a Routes")
+    need(r.expert.dim() == 2 and 1 <= r.expert.shape[1] <= MAX_TOP_K, f"routes.expert must be [T, 1 to {MAX_TOP_K}]")
+    n, k = r.expert.shape
+    need(T is None or n == T, f"routes are of {n} tokens, the rows of {T}")
+    need(n * k <= _MAX_SLOTS, "too many slots")
+    flat(r.expert, "routes.expert", torch.int32, (n, k))
+    flat(r.weight, "routes.weight", torch.float32, (n, k))
+    flat(r.pos, "routes.pos", torch.int32, (n, k))
+    flat(r.src, "routes.src", torch.int32, (n * k,))
+    return n, k
+
+
+def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, valid: Optional[torch.Tensor] = None,
+          out: Optional[Routes] = None) -> Routes:
+    """The ``top_k`` experts of every row of ``logits`` [T, E] (fp32 or bf16), the largest first and the
+    lowest index first among equals; weights are the softmax over the chosen (``renormalize``) or
+    over all experts.  A logit of -inf or NaN closes its expert, +inf counts as the largest finite
+    number; rows where ``valid`` (bool [T]) is False choose nothing."""
+    T, E = _check_gate(logits, top_k)
+    if valid is not None:
+        flat(valid, "valid", torch.bool, (T,))
+    dev = logits.device
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=dev)
+        out = Routes(torch.empty(T, top_k, **i32), torch.empty(T, top_k, dtype=torch.float32, device=dev),
+                     torch.empty(T, top_k, **i32), torch.empty(T * top_k, **i32), torch.empty(E + 1, **i32))
+    else:
+        need(_check_routes(out, T)[1] == top_k, "out has another top_k")
+        flat(out.offs, "out.offs", torch.int32, (E + 1,))
+    with launch("route", logits, valid, *out) as st:
+        lib = _lib.get_lib()
+        ws = torch.empty(lib.hfm_route_ws_ints(T, E), dtype=torch.int32, device=dev)
+        a = RouteArgs(ptr(logits), ptr(valid), *(ptr(t) for t in out), ptr(ws), 0, row_stride(logits), T, E, top_k,
+                      1 if renormalize else 0, _bf(logits), 0, 0)
+        check(lib.hfm_route(C.byref(a), st), "route")
+    return out
+
+
+def route_bwd(logits: torch.Tensor, routes: Routes, dweight: torch.Tensor, renormalize: bool = True,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dL/dlogits (the logits' type) from dL/dweight (fp32 [T, top_k]); ``logits``, ``routes`` and
+    ``renormalize`` as in ``route``.  Closed experts, empty slots and rows that are not valid get zeros."""
+    rows2d(logits, "logits", _VALUES)
+    T, k = _check_routes(routes, logits.shape[0])
+    _, E = _check_gate(logits, k)
+    flat(dweight, "dweight", torch.float32, (T, k))
+    out = out_or_new(out, (T, E), logits.dtype, logits.device)
+    a = RouteBwdArgs(ptr(logits), ptr(routes.expert), ptr(routes.weight), ptr(dweight), ptr(out),
+                     row_stride(logits), row_stride(out), T, E, k, 1 if renormalize else 0, _bf(logits))
+    with launch("route_bwd", logits, *routes, dweight, out) as st:
+        check(_lib.get_lib().hfm_route_bwd(C.byref(a), st), "route_bwd")
+    return out
+
+
+def _exchange(mode, what, a, b, out, r: Routes, weight, dweight, T, k, D, S):
+    args = ExchArgs(ptr(a), ptr(b), ptr(out), ptr(r.pos), ptr(weight), ptr(dweight), row_stride(a),
+                    row_stride(b) if b is not None else 0, row_stride(out), T, k, D, S, _bf(a), 0)
+    with launch(what, a, b, out, r.pos, weight, dweight) as st:
+        check(_lib.get_lib().hfm_exchange(mode, C.byref(args), st), what)
+
+
+def dispatch(x: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [T, D] (fp32 or bf16) -> its rows in expert order, [T * top_k, D]."""
+    rows2d(x, "x", _VALUES)
+    T, k = _check_routes(routes, x.shape[0])
+    D = x.shape[1]
+    out = out_or_new(out, (T * k, D), x.dtype, x.device)
+    _exchange(_EX_DISPATCH, "dispatch", x, None, out, routes, None, None, T, k, D, T * k)
+    return out
+
+
+def dispatch_bwd(dxs: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``dispatch``: dx[t] = the sum of token t's rows of dxs (fp32 sum, in slot order)."""
+    rows2d(dxs, "dxs", _VALUES)
+    T, k = _check_routes(routes)
+    D = dxs.shape[1]
+    need(dxs.shape[0] == T * k, f"dxs must have {T * k} rows, got {dxs.shape[0]}")
+    out = out_or_new(out, (T, D), dxs.dtype, dxs.device)
+    _exchange(_EX_DISPATCH_BWD, "dispatch_bwd", dxs, None, out, routes, None, None, T, k, D, T * k)
+    return out
+
+
+def combine(ys: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """ys [T * top_k, D] in expert order -> y[t] = sum_j weight[t, j] ys[pos[t, j]] (fp32 sum, in slot
+    order); a token without live slots gets zeros."""
+    rows2d(ys, "ys", _VALUES)
+    T, k = _check_routes(routes)
+    D = ys.shape[1]
+    need(ys.shape[0] == T * k, f"ys must have {T * k} rows, got {ys.shape[0]}")
+    out = out_or_new(out, (T, D), ys.dtype, ys.device)
+    _exchange(_EX_COMBINE, "combine", ys, None, out, routes, routes.weight, None, T, k, D, T * k)
+    return out
+
+
+def combine_bwd(dy: torch.Tensor, ys: torch.Tensor, routes: Routes,
+                out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of ``combine``: (dys [T * top_k, D], dweight fp32 [T, top_k]) from dy [T, D]."""
+    rows2d(dy, "dy", _VALUES)
+    T, k = _check_routes(routes, dy.shape[0])
+    D = dy.shape[1]
+    rows2d(ys, "ys", (dy.dtype,), T * k, D)
+    out = out_or_new(out, (T * k, D), dy.dtype, dy.device)
+    dweight = torch.empty(T, k, dtype=torch.float32, device=dy.device)
+    _exchange(_EX_COMBINE_BWD, "combine_bwd", dy, ys, out, routes, routes.weight, dweight, T, k, D, T * k)
+    return out, dweight
+
+
+# ------------------------------------------------------------------ grouped products
+def _check_groups(offs, E):
+    flat(offs, "offs", torch.int32, (E + 1,))
+
+
+def _check_gather(src, top_k, S):
+    need(isinstance(top_k, int) and top_k >= 1, f"top_k must be a positive int, got {top_k}")
+    if src is not None:
+        flat(src, "src", torch.int32, (S,))
+    else:
+        need(top_k == 1, "top_k without src")
+
+
+def _check_weight(w, what, E=None, N=None, K=None):
+    need(isinstance(w, torch.Tensor) and w.dim() == 3 and w.dtype == torch.bfloat16, f"{what} must be a 3-D bf16 tensor")
+    need((E is None or w.shape[0] == E) and (N is None or w.shape[1] == N) and (K is None or w.shape[2] == K),
+         f"{what} must be [{E or 'E'}, {N or 'N'}, {K or 'K'}], got {tuple(w.shape)}")
+    need(w.shape[0] >= 1, f"{what} has no experts")
+    if w.numel():
+        need(w.shape[2] == 1 or w.stride(2) == 1, f"{what}'s last axis must be adjacent")
+        need(w.stride(1) >= 0 and w.stride(0) >= 0, f"{what} has negative strides")
+
+
+def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], offs: torch.Tensor,
+                 relu: bool = False, src: Optional[torch.Tensor] = None, top_k: int = 1,
+                 out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """out[p] = [relu](x[row(p)] w[e(p)]^T + bias[e(p)]) for every place p below offs[E]; x bf16 [rows, K],
+    w bf16 [E, N, K], bias fp32 [E, N] or None, out bf16 or fp32 [S, N].  row(p) = p, or with ``src`` (int32
+    [S]) row(p) = src[p] // top_k, the token of the slot; an entry of ``src`` that is no slot of a row
+    of x reads as a row of zeros.  Without ``src``, S is x's rows."""
+    rows2d(x, "x", _BF)
+    _check_weight(w, "w", K=x.shape[1])
+    E, N, K = w.shape
+    _check_groups(offs, E)
+    S = x.shape[0] if src is None else src.shape[0]
+    _check_gather(src, top_k, S)
+    if bias is not None:
+        flat(bias, "bias", torch.float32, (E, N))
+    if out is not None:
+        out_dtype = out.dtype
+    need(out_dtype in _VALUES, f"out must be bf16 or fp32, not {out_dtype}")
+    out = out_or_new(out, (S, N), out_dtype, x.device)
+    a = GroupNtArgs(ptr(x), ptr(w), ptr(bias), 0, ptr(out), ptr(offs), ptr(src), row_stride(x), w.stride(1),
+                    w.stride(0), 0, row_stride(out), S, x.shape[0], K, N, E, top_k, 1 if relu else 0, 0,
+                    0 if _bf(out) else 1, 1.0)
+    with launch("group_linear", x, w, bias, offs, src, out) as st:
+        check(_lib.get_lib().hfm_group_nt(C.byref(a), st), "group_linear")
+    return out
+
+
+def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
+                mask: Union[None, torch.Tensor, Act8] = None, scale: float = 1.0,
+                out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Gradient towards the layer's input in expert order: out[p] = scale * dz[p] w[e(p)], zero where
+    ``mask`` [S, K] (the input itself, bf16 or ``Act8``: what its relu and dropout left) is not above
+    zero.  dz bf16 [S, N]; ``wt`` bf16 [E, K, N] is the transposed copy of w."""
+    rows2d(dz, "dz", _BF)
+    S = dz.shape[0]
+    _check_weight(wt, "wt", K=dz.shape[1])
+    E, K, N = wt.shape
+    _check_groups(offs, E)
+    m, ldm, m8 = None, 0, 0
+    if isinstance(mask, Act8):
+        check_act8(mask, S, K, "mask")
+        m, ldm, m8 = mask.codes, row_stride(mask.codes), 1
+    elif mask is not None:
+        rows2d(mask, "mask", _BF, S, K)
+        m, ldm = mask, row_stride(mask)
+    if out is not None:
+        out_dtype = out.dtype
+    need(out_dtype in _VALUES, f"out must be bf16 or fp32, not {out_dtype}")
+    out = out_or_new(out, (S, K), out_dtype, dz.device)
+    a = GroupNtArgs(ptr(dz), ptr(wt), 0, ptr(m), ptr(out), ptr(offs), 0, row_stride(dz), wt.stride(1), wt.stride(0),
+                    ldm, row_stride(out), S, S, N, K, E, 1, 0, m8, 0 if _bf(out) else 1, float(scale))
+    with launch("group_dgrad", dz, wt, offs, m, out) as st:
+        check(_lib.get_lib().hfm_group_nt(C.byref(a), st), "group_dgrad")
+    return out
+
+
+def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tensor,
+                src: Optional[torch.Tensor] = None, top_k: int = 1, bias: bool = True,
+                out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None
+                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradients of w and bias, fp32: dw[e] = sum over the rows p of expert e of dz[p]^T x[row(p)]
+    ([E, N, K]) and db[e] = sum dz[p] ([E, N], None without ``bias``); an expert without rows gets zeros.
+    dz bf16 [S, N]; x bf16 [rows, K] or ``Act8``; ``src`` and ``top_k`` as in ``group_linear``.
+    ``out``: the pair to write into, contiguous."""
+    rows2d(dz, "dz", _BF)
+    S, N = dz.shape
+    x8 = isinstance(x, Act8)
+    if x8:
+        need(x.codes.dim() == 2, "x.codes must be 2-D")
+        check_act8(x, x.codes.shape[0], x.codes.shape[1], "x")
+    else:
+        rows2d(x, "x", _BF)
+    xv = x.codes if x8 else x
+    K = xv.shape[1]
+    need(isinstance(offs, torch.Tensor) and offs.dim() == 1 and offs.shape[0] >= 2, "offs must be int32 [E + 1]")
+    E = offs.shape[0] - 1
+    _check_groups(offs, E)
+    _check_gather(src, top_k, S)
+    need(src is not None or xv.shape[0] == S, f"x must have {S} rows, got {xv.shape[0]}")
+    if out is None:
+        dw = torch.empty(E, N, K, dtype=torch.float32, device=dz.device)
+        db = torch.empty(E, N, dtype=torch.float32, device=dz.device) if bias else None
+    else:
+        dw, db = out
+        flat(dw, "dw", torch.float32, (E, N, K))
+        if db is not None:
+            flat(db, "db", torch.float32, (E, N))
+    with launch("group_wgrad", dz, xv, x.scales if x8 else None, offs, src, dw, db) as st:
+        lib = _lib.get_lib()
+        ns = lib.hfm_group_wgrad_splits(S, N, K, E)
+        ws = torch.empty(ns * E * N * (K + 1), dtype=torch.float32, device=dz.device) if ns > 1 else None
+        a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), ptr(ws),
+                        row_stride(dz), row_stride(xv), S, xv.shape[0], K, N, E, top_k, ns)
+        check(lib.hfm_group_wgrad(C.byref(a), st), "group_wgrad")
+    return dw, db
