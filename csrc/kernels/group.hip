@@ -210,12 +210,279 @@ __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_
   }
 }
 
+// 8 neighbouring outputs of row p from column n: mask, rounding, store (vec: 16-byte aligned rows of
+// the output and the mask, N a multiple of 8)
+__device__ __forceinline__ void group_store8(const GroupNtArgs& g, int p, int n, const float (&v)[8], int vec) {
+  const size_t o = (size_t)p * g.ldo + n, m = (size_t)p * g.ldm + n;
+  if (vec) {
+    float w[8];
+    if (g.mask && g.mask8) {
+      const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(g.mask) + m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = a8_positive(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFFu) ? v[j] : 0.f;
+    } else if (g.mask) {
+      const bf16x8 h = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const bf16*>(g.mask) + m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = bf2f(h[j]) > 0.f ? v[j] : 0.f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = v[j];
+    }
+    if (g.out_f32) {
+      float* d = reinterpret_cast<float*>(g.out) + o;
+      *reinterpret_cast<f32x4*>(d) = f32x4{w[0], w[1], w[2], w[3]};
+      *reinterpret_cast<f32x4*>(d + 4) = f32x4{w[4], w[5], w[6], w[7]};
+    } else {
+      bf16x8 d;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = f2bf(w[j]);
+      *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(g.out) + o) = d;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (n + j >= g.N) break;
+    float w = v[j];
+    if (g.mask) {
+      const bool on = g.mask8 ? a8_positive(reinterpret_cast<const uint8_t*>(g.mask)[m + j])
+                              : bf2f(reinterpret_cast<const bf16*>(g.mask)[m + j]) > 0.f;
+      if (!on) w = 0.f;
+    }
+    if (g.out_f32) reinterpret_cast<float*>(g.out)[o + j] = w;
+    else reinterpret_cast<bf16*>(g.out)[o + j] = f2bf(w);
+  }
+}
+
+// ------------------------------------------------------------------ 256 x 256 ping-pong products
+// 512 threads = 8 waves in two groups of 4 (group g owns rows g * 128 .., wave c of a group columns
+// c * 64 ..: 8 x 4 MFMA 16x16x32 tiles, 128 accumulators).  Every SIMD hosts one wave of each group and
+// the groups run one barrier apart: between two barriers one group reads the fragments of its next
+// phase from LDS and stages the next step by LDS-DMA while the other group's 16 MFMAs run.  A 64-deep
+// step is 4 phases of one 64 x 32 output quadrant, in the order (A0,B0) (A0,B1) (A1,B1) (A1,B0), so a
+// phase reads only the half that changes.  Staging of step t + 1 goes into the other buffer: group 1 in
+// its load slots 0-2, group 0 in 1-3 (the buffer's last reads retire in group 1's last compute slot of
+// step t - 1, which is group 0's load slot 0); each wave waits for its own DMA once per step, before
+// the barrier that publishes the step.
+// LDS: 2 buffers x (A 32 KB + B 32 KB).
+constexpr int GP_B = 256, GP_K = 64, GP_THREADS = 512;
+constexpr int GP_PANEL = GP_B * GP_K * 2, GP_BUF = 2 * GP_PANEL;
+
+constexpr int GP_MIN_TILES = 128;
+__device__ __attribute__((aligned(16))) uint32_t g_zero16[4];      // the source of padding chunks
+
+__device__ __forceinline__ void dma16(const void* src, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// One step's 4 phases on buffers `pa` / `pb`.  load_a(half), load_b(half) read fragments, stage(slot)
+// is called in this group's three staging slots (0 .. 2) of the step, wait() once before it ends.
+template <typename LA, typename LB, typename ST, typename MM>
+__device__ __forceinline__ void pp_step(int grp, LA load_a, LB load_b, ST stage, MM mma) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int qa = (q == 0 || q == 1) ? 0 : 1, qb = (q == 0 || q == 3) ? 0 : 1;
+    if (q == 3 && grp == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (q == 0 || q == 2) load_a(qa);
+    load_b(qb);
+    stage(q - (grp == 0 ? 1 : 0));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    mma(q, qa, qb);
+    __builtin_amdgcn_s_setprio(0);
+    if (q == 3 && grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// block b of n -> position in an order where each XCD (blocks go round the 8 of them) has a run of
+// neighbouring tiles, which share operand panels in its L2
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int xcd = b & 7, q8 = n >> 3, rr = n & 7;
+  return (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (b >> 3);
+}
+
+// A wave's 128 x 64 outputs leave through its 16 KB of LDS, 64 rows a pass, so that a lane holds 8
+// neighbouring columns of a row: emit(row in the block, first column in the block, 8 values).
+template <typename F>
+__device__ __forceinline__ void pp_emit(const f32x4 (&acc)[8][4], char* img, int lane, F emit) {
+  const int fr = lane & 15, fq = lane >> 4;
+  auto wsync = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // rows of 64 floats; 16-byte chunk c of row r at chunk c ^ (r & 15)
+  auto off = [](int r, int c) { return r * 256 + ((((c >> 2) ^ (r & 15))) << 4) + (c & 3) * 4; };
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<float*>(img + off(i * 16 + fq * 4 + k, j * 16 + fr)) = acc[p * 4 + i][j][k];
+    wsync();
+#pragma unroll 2
+    for (int it = 0; it < 8; ++it) {
+      const int r = it * 8 + (lane >> 3), c = (lane & 7) * 8;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(img + off(r, c));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(img + off(r, c + 4));
+      const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      emit(p * 64 + r, c, v);
+    }
+    wsync();
+  }
+}
+
+// ---- NT: rows of A and B are K-contiguous, LDS image as in the 128 x 128 kernel.  K a multiple of 8;
+// the last step's chunks past K come from the zero source.
+__global__ void __launch_bounds__(GP_THREADS, 1) group_nt_pp_kernel(GroupNtArgs g, int tiles_n, int ovec) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * GP_BUF];
+  const int tile = xcd_order(blockIdx.x, gridDim.x);
+  int e, r0, r1;
+  if (!group_find<GP_B>(g.offs, g.E, g.S, tile / tiles_n, e, r0, r1)) return;
+  const int n0 = (tile % tiles_n) * GP_B;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int grp = wave >> 2, wc = wave & 3;
+  const int fr = lane & 15, fq = lane >> 4, swz = (fr >> 1) & 7;
+  const int la[2] = {(grp * 128 + fr) * 128 + ((fq ^ swz) << 4), (grp * 128 + fr) * 128 + (((4 + fq) ^ swz) << 4)};
+  const int lb[2] = {(wc * 64 + fr) * 128 + ((fq ^ swz) << 4), (wc * 64 + fr) * 128 + (((4 + fq) ^ swz) << 4)};
+  // staging pieces of 8 rows x 128 B: 4 of A and 4 of B per wave.  Rows past the group's end and
+  // columns past N read the last one (their outputs are not stored).
+  const bf16* src[8];
+  int ck[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int r = (wave * 4 + (p & 3)) * 8 + (lane >> 3);
+    ck[p] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    if (p < 4) {
+      const int row = max(group_row(g.src, min(r0 + r, r1 - 1), g.rows, g.top_k), 0);
+      src[p] = g.a + (size_t)row * g.lda + ck[p];
+    } else {
+      src[p] = g.b + (size_t)e * g.es + (size_t)min(n0 + r, g.N - 1) * g.ldb + ck[p];
+    }
+  }
+  const int nt = (g.K + GP_K - 1) / GP_K;
+  const bool ragged = (g.K & (GP_K - 1)) != 0;
+  auto piece = [&](int p, char* buf, int t) {
+    const void* s = src[p] + t * GP_K;
+    if (ragged && t == nt - 1 && t * GP_K + ck[p] >= g.K) s = g_zero16;
+    dma16(s, buf + (p >= 4 ? GP_PANEL : 0) + (wave * 4 + (p & 3)) * 1024);
+  };
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int p = 0; p < 8; ++p) piece(p, smem, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  if (grp == 1) {                         // the stagger: group 1 runs one slot behind
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  bf16x8 fa[4][2], fb[2][2];
+  for (int t = 0; t < nt; ++t) {
+    const char* pa = smem + (t & 1) * GP_BUF;
+    const char* pb = pa + GP_PANEL;
+    char* nxt = smem + ((t + 1) & 1) * GP_BUF;
+    pp_step(
+        grp,
+        [&](int h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+              fa[i][ks] = *reinterpret_cast<const bf16x8*>(pa + la[ks] + (h * 64 + i * 16) * 128);
+        },
+        [&](int h) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+              fb[j][ks] = *reinterpret_cast<const bf16x8*>(pb + lb[ks] + (h * 32 + j * 16) * 128);
+        },
+        [&](int s) {
+          if (t + 1 >= nt) return;
+          if (s == 0)
+            for (int p = 0; p < 3; ++p) piece(p, nxt, t + 1);
+          if (s == 1)
+            for (int p = 3; p < 6; ++p) piece(p, nxt, t + 1);
+          if (s == 2)
+            for (int p = 6; p < 8; ++p) piece(p, nxt, t + 1);
+        },
+        [&](int, int qa, int qb) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                acc[qa * 4 + i][qb * 2 + j] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][ks], fb[j][ks], acc[qa * 4 + i][qb * 2 + j], 0, 0, 0);
+        });
+  }
+  if (grp == 0) __builtin_amdgcn_s_barrier();   // (every wave passes the same number of barriers)
+  __syncthreads();
+  // a source that is no slot: a row of zeros
+  if (g.src) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int p = r0 + grp * 128 + i * 16 + fq * 4 + q;
+        if (p < r1 && group_row(g.src, p, g.rows, g.top_k) < 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j][q] = 0.f;
+        }
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = n0 + wc * 64 + j * 16 + fr;
+    const float bias = g.bias && n < g.N ? g.bias[(size_t)e * g.N + n] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v = acc[i][j][q] * g.scale + bias;
+        if (g.relu && v < 0.f) v = 0.f;
+        acc[i][j][q] = v;
+      }
+  }
+  pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
+    const int p = r0 + grp * 128 + r, n = n0 + wc * 64 + c;
+    if (p < r1 && n < g.N) group_store8(g, p, n, v, ovec);
+  });
+}
+
 HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   const GroupNtArgs g = *gp;
   if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
   if (g.S == 0 || g.N == 0) return 0;
   const bool vec = ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.K % 8 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0 &&
                    g.es % 8 == 0;
+  const bool ovec = g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0 &&
+                    (!g.mask || (g.ldm % 8 == 0 && (uintptr_t)g.mask % (g.mask8 ? 8 : 16) == 0));
+  if (vec && g.K >= GP_K) {
+    const int tn = (g.N + GP_B - 1) / GP_B;
+    const long blocks = (long)(g.S / GP_B + g.E) * tn;
+    if (blocks >= GP_MIN_TILES && blocks <= 0x7FFFFFFFl) {
+      hipLaunchKernelGGL(group_nt_pp_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn, ovec ? 1 : 0);
+      HFM_LAUNCH_CHECK();
+    }
+  }
   const int tn = (g.N + GN_B - 1) / GN_B;
   const long blocks = (long)(g.S / GN_B + g.E) * tn;      // (each group adds less than one tile)
   if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;

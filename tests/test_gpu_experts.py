@@ -349,6 +349,77 @@ def test_group_wgrad(sizes, K, N, x8):
         close(db[i], a.sum(0), (n + 4) * 2.0 ** -23 * a.abs().sum(0), "db")
 
 
+LARGE = [([9000, 0, 257, 1, 5000, 256], 200, 1032), ([20000], 64, 777), ([3] * 150, 72, 40), ([700, 4000, 1300], 1248, 2048),
+         ([1, 0, 30000], 136, 264), ([5000, 6000], 512, 1000)]
+
+
+@pytest.mark.parametrize("sizes,K,N", LARGE)
+def test_group_products_many_tiles(sizes, K, N):
+    """The same three products where the output has many tiles (the large-tile kernels)."""
+    EX, A8 = ops()
+    E = len(sizes)
+    g = torch.Generator(device=DEV).manual_seed(K + N)
+    offs, S = groups(sizes, tail=5)
+    e = R.group_ids(offs, S)
+    o = offs.to(DEV)
+
+    def rn(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device=DEV, generator=g).to(dtype)
+
+    x, w, b, dz = rn(S, K), rn(E, N, K), rn(E, N, dtype=torch.float32), rn(S, N)
+    x[S - 5:], dz[S - 5:] = math.nan, math.nan
+    live = S - 5
+
+    def spans():
+        return [(i, int(offs[i]), int(offs[i + 1])) for i in range(E) if offs[i + 1] > offs[i]]
+
+    def check(got, want, bound, what):
+        d = (got.double() - want).abs()
+        assert bool((d <= bound).all()), (what, float((d - bound).max()))
+
+    half = HALF[torch.bfloat16]
+    out = torch.full((S, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    y = EX.group_linear(x, w, b, o, relu=True, out=out)
+    assert bool((y[live:] == 7).all())
+    k3 = torch.randint(0, 3, (S,), device=DEV, generator=g)
+    perm = torch.randperm(S, device=DEV, generator=g)
+    src = (torch.argsort(perm) * 3 + k3).int()
+    assert torch.equal(EX.group_linear(x[perm], w, b, o, relu=True, src=src, top_k=3)[:live], y[:live])
+    gone = src.clone()
+    gone[::7] = -1
+    z = EX.group_linear(x[perm], w, b, o, src=gone, top_k=3, out_dtype=torch.float32)
+    zero = torch.arange(S, device=DEV) % 7 == 0
+    h = torch.relu(rn(S, K, dtype=torch.float32)).to(torch.bfloat16)
+    a8 = A8.pack(h)
+    wt = w.transpose(1, 2).contiguous()
+    dx = EX.group_dgrad(dz, wt, o, mask=h, scale=0.5)
+    assert torch.equal(dx[:live], EX.group_dgrad(dz, wt, o, mask=a8, scale=0.5)[:live])
+    dw, db = EX.group_wgrad(dz, x, o)
+    dwp, dbp = EX.group_wgrad(dz, x[perm], o, src=src, top_k=3)
+    assert torch.equal(dw, dwp) and torch.equal(db, dbp)
+    dw8, db8 = EX.group_wgrad(dz, a8, o)
+    ap = A8.Act8(a8.codes[perm], a8.scales[perm])
+    dw8p, db8p = EX.group_wgrad(dz, ap, o, src=src, top_k=3)
+    assert torch.equal(dw8, dw8p) and torch.equal(db8, db8p) and torch.equal(db8, db)
+    h8 = A8.unpack(a8, torch.float32).double()
+    for i, lo, hi in spans():
+        xd, wd, zd = x[lo:hi].double(), w[i].double(), dz[lo:hi].double()
+        c = 2.0 ** -23 * 1.01
+        p, mag = xd @ wd.T, xd.abs() @ wd.abs().T
+        want = p + b[i].double()
+        check(y[lo:hi], want.clamp(min=0), half * want.abs() + c * ((K + 4) * mag + want.abs()), "y")
+        want = torch.where(zero[lo:hi, None], 0.0, p) + b[i].double()
+        check(z[lo:hi], want, 2.0 ** -24 * want.abs() + c * ((K + 4) * mag + want.abs()), "z")
+        want = 0.5 * (zd @ wd) * (h[lo:hi] > 0)
+        check(dx[lo:hi], want, half * want.abs() + c * ((N + 4) * 0.5 * (zd.abs() @ wd.abs()) + want.abs()), "dx")
+        check(dw[i], zd.T @ xd, c * (hi - lo + 4) * (zd.abs().T @ xd.abs()), "dw")
+        check(dw8[i], zd.T @ h8[lo:hi], c * (hi - lo + 4) * (zd.abs().T @ h8[lo:hi]), "dw8")
+        check(db[i], zd.sum(0), c * (hi - lo + 4) * zd.abs().sum(0), "db")
+    for i in range(E):
+        if sizes[i] == 0:
+            assert not dw[i].any() and not db[i].any() and not dw8[i].any()
+
+
 def test_group_bad_device_data_stays_in_bounds():
     """Offsets that are not in order and sources that are no slots: rows read as documented, no more."""
     EX, _ = ops()
