@@ -45,5 +45,13 @@ __device__ __forceinline__ void a8_unpack8(uint2 w, float s, float (&f)[8]) {
   f[4] = p2[0] * s; f[5] = p2[1] * s; f[6] = p3[0] * s; f[7] = p3[1] * s;
 }
 
+// 2 codes (the low or high half of a word) -> 2 bf16 values times the scale, exact: one conversion
+template <bool HI>
+__device__ __forceinline__ uint32_t a8_pair_bf16(uint32_t w, float s) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, HI);
+  return __builtin_bit_cast(uint32_t, v);
+}
+
 // whether a code stands for a value above zero (0x7F is NaN)
 __device__ __forceinline__ bool a8_positive(uint32_t code) { return code - 1u < 0x7Eu; }

@@ -288,6 +288,7 @@ __device__ __forceinline__ void pp_step(int grp, LA load_a, LB load_b, ST stage,
     load_b(qb);
     stage(q - (grp == 0 ? 1 : 0));
     __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");          // (no access moves over a barrier)
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -298,6 +299,7 @@ __device__ __forceinline__ void pp_step(int grp, LA load_a, LB load_b, ST stage,
     if (q == 3 && grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -313,6 +315,9 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
 // neighbouring columns of a row: emit(row in the block, first column in the block, 8 values).
 template <typename F>
 __device__ __forceinline__ void pp_emit(const f32x4 (&acc)[8][4], char* img, int lane, F emit) {
+  // (the lane hidden from the optimizer: in a loop over tiles it would otherwise keep the image's
+  // addresses in registers through the product, which has none left)
+  asm volatile("" : "+v"(lane));
   const int fr = lane & 15, fq = lane >> 4;
   auto wsync = [] {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -649,9 +654,414 @@ __global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
   (i < nw ? g.dw[i] : g.db[i - nw]) = v;
 }
 
+// ---- TN: the weight gradient on the ping-pong tile.  Both panels keep their global layout, [64 rows][256
+// columns]; the fragments (8 rows of one column per lane) come from transposing LDS reads
+// (ds_read_b64_tr_b16: a 16-lane group reads 4 rows x 16 columns, lane l gets column l's 4 rows).
+// A panel row is 512 B, so a fragment's 16 rows would meet in the same banks: 32-byte granule c of row r
+// lies at c ^ f(r), f(r) = (r & 3) | (r >> 1 & 4), which spreads them over all 8 granules of 256 B.
+// 8-bit x: 16 codes a thread are loaded one step ahead, turned into bf16 times the block's scale
+// (one conversion per pair, exact) and written into the same image.
+//
+// The work is cut evenly, not by tiles: `units` = 64-row steps of all tiles (a group without rows counts
+// one per tile, which writes its zeros), tiles in expert order, and workgroup w takes the units from
+// w U / W to (w + 1) U / W.  A tile within one workgroup goes straight to dw; a workgroup's first and last tile
+// may be parts, which go to its two workspace tiles and are summed in row order by a second launch.
+// Groups of any sizes thus load the CUs evenly (by whole tiles the fullest of 16 groups set the
+// time), for at most 512 tiles of 256 KB.
+constexpr int GW_SLAB = GP_B * GP_B + GP_B;      // floats of a workspace tile: dw part, db part
+
+struct WgCut {
+  long u0, u1;             // the workgroup's units
+};
+__device__ __forceinline__ WgCut wg_cut(long U, int W, int w) { return {U * w / W, U * (w + 1) / W}; }
+__device__ __forceinline__ int wg_owner(long U, int W, long u) {        // the workgroup of unit u
+  int w = (int)((u * W) / U);
+  while (U * (w + 1) / W <= u) ++w;
+  while (w > 0 && U * w / W > u) --w;
+  return w;
+}
+__device__ __forceinline__ int wg_steps(const int* offs, int e, int S) {
+  int lo, hi;
+  group_rows(offs, e, S, lo, hi);
+  return max(1, (hi - lo + GP_K - 1) / GP_K);
+}
+// a value that is the same in all lanes, into scalar registers
+__device__ __forceinline__ long uni64(long v) {
+  return (long)(((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+// units of all groups, by every wave for itself
+__device__ __forceinline__ long wg_units(const int* offs, int E, int S, int tiles) {
+  const int lane = threadIdx.x & 63;
+  long n = 0;
+  for (int e = lane; e < E; e += 64) n += wg_steps(offs, e, S);
+  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+  return uni64(n) * tiles;
+}
+// the expert of unit u, and its first unit
+__device__ __forceinline__ void wg_find(const int* offs, int E, int S, int tiles, long u, int& e, long& first) {
+  const int lane = threadIdx.x & 63;
+  long run = 0;
+  e = 0;
+  first = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const long n = e0 + lane < E ? (long)wg_steps(offs, e0 + lane, S) * tiles : 0;
+    long inc = n;
+    for (int d = 1; d < 64; d <<= 1) {
+      const long v = __shfl_up(inc, d);
+      if (lane >= d) inc += v;
+    }
+    const unsigned long long past = __ballot(run + inc > u);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      e = e0 + l;
+      first = run + __shfl(inc - n, l);
+      break;
+    }
+    run += __shfl(inc, 63);
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  first = uni64(first);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8 tr_read(const char* p0, const char* p1) {
+  typedef __attribute__((address_space(3))) s16x4* lp;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p0);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p1);
+  const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+template <bool X8, bool GATHER>
+__global__ void __launch_bounds__(GP_THREADS, 1) group_wgrad_pp_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int ovec) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * GP_BUF];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int grp = wave >> 2, wc = wave & 3;
+  const int fr = lane & 15, fq = lane >> 4;
+  const int tiles = tiles_n * tiles_k;
+  const int w = xcd_order(blockIdx.x, gridDim.x);
+  const WgCut cut = wg_cut(wg_units(g.offs, g.E, g.S, tiles), gridDim.x, w);
+  int e;
+  long first;
+  wg_find(g.offs, g.E, g.S, tiles, cut.u0, e, first);
+  // fragment addresses: granule (base + i) ^ f(row) = f-and-base part ^ i, rows of fq and fr >> 2
+  const int fsw = (fr >> 2) | ((fq & 1) << 2);
+  const int rowoff = (fq * 8 + (fr >> 2)) * 512 + (fr & 3) * 8;
+  int la = rowoff + ((grp * 8 ^ fsw) << 5), lb = rowoff + ((wc * 4 ^ fsw) << 5);
+  // staging pieces: 2 rows of 512 B, 4 of each operand per wave.  Row 2 i + hi of the wave's 8 has
+  // f = ((2 i + hi) & 3) | 4 (wave & 1), so the lane's 16-byte chunk is one column for even i and
+  // that column ^ 32 for odd i.
+  const int hi = lane >> 5, c16 = lane & 31;
+  const int ce = (((c16 >> 1) ^ (hi | ((wave & 1) << 2))) * 2 + (c16 & 1)) * 8;
+  const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
+  // 8-bit x: 16 codes at column xc of rows xr, xr + 32
+  const int xr = threadIdx.x >> 4, xc = (threadIdx.x & 15) * 16;
+  const int xo = GP_PANEL + xr * 512 + (((xc >> 4) ^ ((xr & 3) | ((xr >> 1) & 4))) << 5);
+  bf16x8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.f);
+
+  long u = cut.u0;
+  while (u < cut.u1) {
+    int steps = wg_steps(g.offs, e, g.S);
+    while (u >= first + (long)steps * tiles) {      // the next group
+      first += (long)steps * tiles;
+      ++e;
+      steps = wg_steps(g.offs, e, g.S);
+    }
+    int lo, hi_row;
+    group_rows(g.offs, e, g.S, lo, hi_row);
+    const int ti = (int)((u - first) / steps), s0 = (int)((u - first) % steps);
+    const int s1 = (int)min((long)steps, s0 + (cut.u1 - u));
+    const int n0 = (ti / tiles_k) * GP_B, k0 = (ti % tiles_k) * GP_B;
+    const int p0 = lo + s0 * GP_K, p1 = min(hi_row, lo + s1 * GP_K);
+    const int nt = p1 > p0 ? (p1 - p0 + GP_K - 1) / GP_K : 0;
+    const bool ragged = ((p1 - p0) & (GP_K - 1)) != 0;
+    const bool sum = g.db != nullptr && k0 == 0;
+    f32x4 acc[8][4], accb[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    accb[0] = accb[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // columns past N or K read column 0 (their outputs are not stored), rows past p1 the zero source
+    // (the last step only).  Scalar row base + the lane's 32-bit byte offset.
+    const uint32_t ao0 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + ce < g.N ? n0 + ce : 0));
+    const uint32_t ao1 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + (ce ^ 32) < g.N ? n0 + (ce ^ 32) : 0));
+    const int bc0 = k0 + ce < g.K ? k0 + ce : 0, bc1 = k0 + (ce ^ 32) < g.K ? k0 + (ce ^ 32) : 0;
+    const bool xin = k0 + xc < g.K;
+    int xrow[4];                                       // GATHER: x rows of the next step's pieces (-1: zeros)
+    uint4 cd[2];
+    uint32_t cs[2];
+    auto piece_a = [&](int i, char* buf, int t) {
+      const int p = p0 + t * GP_K + wave * 8 + 2 * i;
+      const void* s = reinterpret_cast<const char*>(g.dz + (size_t)p * g.ldz) + ((i & 1) ? ao1 : ao0);
+      if (ragged && t == nt - 1 && p + hi >= p1) s = g_zero16;
+      dma16(s, buf + (wave * 4 + i) * 1024);
+    };
+    auto rows_of = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + t * GP_K + wave * 8 + 2 * i + hi;
+        xrow[i] = p < p1 ? group_row(g.src, p, g.rows, g.top_k) : -1;
+      }
+    };
+    auto piece_b = [&](int i, char* buf, int t) {
+      const bf16* xb = reinterpret_cast<const bf16*>(g.x);
+      const void* s;
+      if (GATHER) {
+        s = xrow[i] >= 0 ? (const void*)(xb + (size_t)(uint32_t)xrow[i] * g.ldx + ((i & 1) ? bc1 : bc0)) : (const void*)g_zero16;
+      } else {
+        const int p = p0 + t * GP_K + wave * 8 + 2 * i;
+        s = reinterpret_cast<const char*>(xb + (size_t)p * g.ldx) + 2u * (uint32_t)(hi * (int)g.ldx + ((i & 1) ? bc1 : bc0));
+        if (ragged && t == nt - 1 && p + hi >= p1) s = g_zero16;
+      }
+      dma16(s, buf + GP_PANEL + (wave * 4 + i) * 1024);
+    };
+    auto codes_of = [&](int t) {                       // X8: the codes of step t into registers
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int pb = p0 + t * GP_K + 32 * h, p = pb + xr;
+        cd[h] = make_uint4(0, 0, 0, 0);
+        cs[h] = 127;
+        if (p < p1 && xin) {
+          const uint8_t* x8 = reinterpret_cast<const uint8_t*>(g.x) + k0;
+          if (GATHER) {
+            const int row = group_row(g.src, p, g.rows, g.top_k);
+            if (row >= 0) {
+              cd[h] = *reinterpret_cast<const uint4*>(x8 + (size_t)row * g.ldx + xc);
+              cs[h] = g.xs[(size_t)row * sblk + (k0 + xc) / A8_BLOCK];
+            }
+          } else {
+            cd[h] = *reinterpret_cast<const uint4*>(x8 + (size_t)pb * g.ldx + (uint32_t)(xr * (int)g.ldx + xc));
+            cs[h] = g.xs[(size_t)pb * sblk + (uint32_t)(xr * sblk + (k0 + xc) / A8_BLOCK)];
+          }
+        }
+      }
+    };
+    auto codes_to = [&](char* buf) {                   // X8: registers -> bf16 image
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                    // (row + 32: the same f)
+        const float s = a8_scale(cs[h]);
+        char* d = buf + xo + h * 32 * 512;
+        *reinterpret_cast<uint4*>(d) = make_uint4(a8_pair_bf16<false>(cd[h].x, s), a8_pair_bf16<true>(cd[h].x, s),
+                                                  a8_pair_bf16<false>(cd[h].y, s), a8_pair_bf16<true>(cd[h].y, s));
+        *reinterpret_cast<uint4*>(d + 16) = make_uint4(a8_pair_bf16<false>(cd[h].z, s), a8_pair_bf16<true>(cd[h].z, s),
+                                                       a8_pair_bf16<false>(cd[h].w, s), a8_pair_bf16<true>(cd[h].w, s));
+      }
+    };
+    if (nt > 0) {
+      if (X8) codes_of(0);
+      else if (GATHER) rows_of(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        piece_a(i, smem, 0);
+        if (!X8) piece_b(i, smem, 0);
+      }
+      if (X8) {
+        codes_to(smem);
+        if (nt > 1) codes_of(1);
+      } else if (GATHER && nt > 1) {
+        rows_of(1);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (grp == 1) {
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bf16x8 fa[4][2], fb[2][2];
+    for (int t = 0; t < nt; ++t) {
+      const char* pa = smem + (t & 1) * GP_BUF;
+      const char* pb = pa + GP_PANEL;
+      char* nxt = smem + ((t + 1) & 1) * GP_BUF;
+      asm volatile("" : "+v"(la), "+v"(lb));           // (12 addresses made by one xor each, not kept)
+      pp_step(
+          grp,
+          [&](int h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) {
+                const char* a = pa + (la ^ ((h * 4 + i) << 5)) + ks * 32 * 512;
+                fa[i][ks] = tr_read(a, a + 4 * 512);
+              }
+          },
+          [&](int h) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) {
+                const char* b = pb + (lb ^ ((h * 2 + j) << 5)) + ks * 32 * 512;
+                fb[j][ks] = tr_read(b, b + 4 * 512);
+              }
+          },
+          [&](int s) {
+            if (t + 1 >= nt) return;
+            if (X8) {
+              if (s == 0) codes_to(nxt);
+              if (s == 1) {
+                piece_a(0, nxt, t + 1);
+                piece_a(1, nxt, t + 1);
+                if (t + 2 < nt) codes_of(t + 2);
+              }
+              if (s == 2) {
+                piece_a(2, nxt, t + 1);
+                piece_a(3, nxt, t + 1);
+              }
+            } else {
+              if (s == 0) {
+                piece_a(0, nxt, t + 1);
+                piece_a(1, nxt, t + 1);
+                piece_a(2, nxt, t + 1);
+              }
+              if (s == 1) {
+                piece_a(3, nxt, t + 1);
+                piece_b(0, nxt, t + 1);
+                piece_b(1, nxt, t + 1);
+              }
+              if (s == 2) {
+                piece_b(2, nxt, t + 1);
+                piece_b(3, nxt, t + 1);
+                if (GATHER && t + 2 < nt) rows_of(t + 2);
+              }
+            }
+          },
+          [&](int q, int qa, int qb) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  acc[qa * 4 + i][qb * 2 + j] =
+                      __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][ks], fb[j][ks], acc[qa * 4 + i][qb * 2 + j], 0, 0, 0);
+            // db: dz against a column of ones; wave c of a group takes row tiles 2 c, 2 c + 1
+            if (sum && (q & 1) == 0 && (wc >> 1) == qa) {
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) {
+                if (wc & 1) {
+                  accb[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2][ks], ones, accb[0], 0, 0, 0);
+                  accb[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[3][ks], ones, accb[1], 0, 0, 0);
+                } else {
+                  accb[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[0][ks], ones, accb[0], 0, 0, 0);
+                  accb[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[1][ks], ones, accb[1], 0, 0, 0);
+                }
+              }
+            }
+          });
+    }
+    if (grp == 0) __builtin_amdgcn_s_barrier();
+    __syncthreads();
+    // a whole tile goes to dw, a part to the workspace: slot 2 w if it is the workgroup's first, 2 w + 1
+    // if it goes on in the next one
+    const bool whole = s0 == 0 && s1 == steps;
+    if (whole) {
+      float* dw = g.dw + (size_t)e * g.N * g.K;
+      pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
+        const int n = n0 + grp * 128 + r, k = k0 + wc * 64 + c;
+        if (n >= g.N || k >= g.K) return;
+        float* d = dw + (size_t)n * g.K + k;
+        if (ovec) {
+          *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (k + j < g.K) d[j] = v[j];
+        }
+      });
+    } else {
+      float* slab = g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB;
+      pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
+        float* d = slab + (grp * 128 + r) * GP_B + wc * 64 + c;
+        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      });
+    }
+    if (sum && fr == 0) {
+      float* db = whole ? g.db + (size_t)e * g.N : g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB + GP_B * GP_B;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = grp * 128 + (wc * 2 + i) * 16 + fq * 4 + q;
+          if (!whole) db[r] = accb[i][q];
+          else if (n0 + r < g.N) db[n0 + r] = accb[i][q];
+        }
+    }
+    u += s1 - s0;
+    __syncthreads();                      // (the next tile's staging reuses the images)
+  }
+}
+
+// Tiles that two or more workgroups made: their parts in row order.  grid (tiles of an expert, E, 4
+// quarters); the same cut as the product's.
+__global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int W, int ovec) {
+  const int tiles = tiles_n * tiles_k, ti = blockIdx.x, e = blockIdx.y;
+  const int lane = threadIdx.x & 63;
+  long before = 0, n = 0;
+  for (int i = lane; i < g.E; i += 64) {
+    const int s = wg_steps(g.offs, i, g.S);
+    n += s;
+    if (i < e) before += s;
+  }
+  for (int d = 32; d; d >>= 1) {
+    n += __shfl_xor(n, d);
+    before += __shfl_xor(before, d);
+  }
+  const long U = n * tiles;
+  const int steps = wg_steps(g.offs, e, g.S);
+  const long a = before * tiles + (long)ti * steps, b = a + steps - 1;
+  const int w0 = wg_owner(U, W, a), w1 = wg_owner(U, W, b);
+  if (w0 == w1) return;
+  const int n0 = (ti / tiles_k) * GP_B, k0 = (ti % tiles_k) * GP_B;
+  // the part that starts the tile is the last of w0 (slot 1), the others are the first of theirs
+  auto slab = [&](int w) { return g.ws + (size_t)(2 * w + (w == w0 ? 1 : 0)) * GW_SLAB; };
+  const int row0 = blockIdx.z * 64;
+  for (int i = threadIdx.x; i < 64 * (GP_B / 4); i += 256) {
+    const int r = row0 + i / (GP_B / 4), c = (i % (GP_B / 4)) * 4;
+    if (n0 + r >= g.N || k0 + c >= g.K) continue;
+    f32x4 v = *reinterpret_cast<const f32x4*>(slab(w0) + r * GP_B + c);
+    for (int q = w0 + 1; q <= w1; ++q) v += *reinterpret_cast<const f32x4*>(slab(q) + r * GP_B + c);
+    float* d = g.dw + ((size_t)e * g.N + n0 + r) * g.K + k0 + c;
+    if (ovec) {
+      *reinterpret_cast<f32x4*>(d) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k0 + c + j < g.K) d[j] = v[j];
+    }
+  }
+  if (g.db && k0 == 0 && threadIdx.x < 64 && n0 + row0 + threadIdx.x < g.N) {
+    const int r = row0 + threadIdx.x;
+    float v = slab(w0)[GP_B * GP_B + r];
+    for (int q = w0 + 1; q <= w1; ++q) v += slab(q)[GP_B * GP_B + r];
+    g.db[(size_t)e * g.N + n0 + r] = v;
+  }
+}
+
+// Where the large tile is taken, and its workgroups (one per CU: 128 KB of LDS each): operands with 16-byte
+// rows, and enough work for every CU (GP_MIN_UNITS steps each; below that the 128 x 128 tile's smaller
+// pieces fill the chip better).
+constexpr int GW_WGS = 256, GP_MIN_UNITS = 2;
+static bool wgrad_big(const GroupWgArgs& g) {
+  const bool x8 = g.xs != nullptr;
+  if ((uintptr_t)g.dz % 16 || (uintptr_t)g.x % 16 || g.N % 8 || g.ldz % 8) return false;
+  if (g.K % (x8 ? 16 : 8) || g.ldx % (x8 ? 16 : 8)) return false;
+  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25) return false;      // (32-bit offsets within 64 rows)
+  const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
+  return tiles * (g.S / GP_K) >= (long)GW_WGS * GP_MIN_UNITS;
+}
+
 // Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
 // 64 rows on average.
-HFM_API int hfm_group_wgrad_splits(int S, int N, int K, int E) {
+static int wgrad_splits(int S, int N, int K, int E) {
   const long tiles = (long)E * ((N + GN_B - 1) / GN_B) * ((K + GN_B - 1) / GN_B);
   if (tiles <= 0) return 1;
   long ns = 512 / tiles;
@@ -661,11 +1071,29 @@ HFM_API int hfm_group_wgrad_splits(int S, int N, int K, int E) {
   return ns < 1 ? 1 : (int)ns;
 }
 
+HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
+  if (wgrad_big(*gp)) return 2l * GW_WGS * GW_SLAB;
+  const int ns = wgrad_splits(gp->S, gp->N, gp->K, gp->E);
+  return ns > 1 ? (long)ns * gp->E * gp->N * (gp->K + 1) : 0;
+}
+
 HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   GroupWgArgs g = *gp;
   if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
   if (g.N == 0) return 0;
-  g.ns = hfm_group_wgrad_splits(g.S, g.N, g.K, g.E);
+  if (wgrad_big(g)) {
+    const int tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
+    if (!g.ws || (uintptr_t)g.ws % 16 || g.E > 65535) return (int)hipErrorInvalidValue;
+    const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
+    const dim3 grid(GW_WGS), blk(GP_THREADS);
+    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_pp_kernel<true, true>), grid, blk, 0, st, g, tn, tk, ovec);
+    else if (g.xs) hipLaunchKernelGGL((group_wgrad_pp_kernel<true, false>), grid, blk, 0, st, g, tn, tk, ovec);
+    else if (g.src) hipLaunchKernelGGL((group_wgrad_pp_kernel<false, true>), grid, blk, 0, st, g, tn, tk, ovec);
+    else hipLaunchKernelGGL((group_wgrad_pp_kernel<false, false>), grid, blk, 0, st, g, tn, tk, ovec);
+    hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 4), dim3(256), 0, st, g, tn, tk, GW_WGS, ovec);
+    HFM_LAUNCH_CHECK();
+  }
+  g.ns = wgrad_splits(g.S, g.N, g.K, g.E);
   if (g.ns > 1 && !g.ws) return (int)hipErrorInvalidValue;
   const bool x8 = g.xs != nullptr;
   const bool vec = (uintptr_t)g.dz % 16 == 0 && g.N % 8 == 0 && g.ldz % 8 == 0 && (uintptr_t)g.x % (x8 ? 8 : 16) == 0 &&

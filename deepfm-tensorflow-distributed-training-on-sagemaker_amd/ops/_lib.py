@@ -256,7 +256,7 @@ _SIGS = {
     "hfm_act8_args_bytes": [],
     "hfm_group_nt": [C.POINTER(GroupNtArgs), c_void_p],
     "hfm_group_nt_args_bytes": [],
-    "hfm_group_wgrad_splits": [c_int, c_int, c_int, c_int],
+    "hfm_group_wgrad_ws_floats": [C.POINTER(GroupWgArgs)],
     "hfm_group_wgrad": [C.POINTER(GroupWgArgs), c_void_p],
     "hfm_group_wg_args_bytes": [],
     "hfm_fm_fwd": [c_void_p] * 5 + [c_int] * 4 + [c_void_p] * 6 + [c_long, c_long, c_void_p, c_int,
@@ -400,7 +400,7 @@ def get_lib():
         for name, args in _SIGS.items():
             fn = getattr(lib, name)
             fn.argtypes = args
-            fn.restype = c_int
+            fn.restype = c_long if name == "hfm_group_wgrad_ws_floats" else c_int
         # ABI checks: ctypes struct layouts must match the C structs
         for cname, pys in (("hfm_epi_args_bytes", EpiArgs), ("hfm_head_args_bytes", HeadArgs),
                            ("hfm_slab_job_bytes", SlabJob), ("hfm_rowsum_job_bytes", RowSumJob),

@@ -293,9 +293,10 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
             flat(db, "db", torch.float32, (E, N))
     with launch("group_wgrad", dz, xv, x.scales if x8 else None, offs, src, dw, db) as st:
         lib = _lib.get_lib()
-        ns = lib.hfm_group_wgrad_splits(S, N, K, E)
-        ws = torch.empty(ns * E * N * (K + 1), dtype=torch.float32, device=dz.device) if ns > 1 else None
-        a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), ptr(ws),
-                        row_stride(dz), row_stride(xv), S, xv.shape[0], K, N, E, top_k, ns)
+        a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), 0,
+                        row_stride(dz), row_stride(xv), S, xv.shape[0], K, N, E, top_k, 1)
+        n = lib.hfm_group_wgrad_ws_floats(C.byref(a))
+        ws = torch.empty(n, dtype=torch.float32, device=dz.device) if n else None
+        a.ws = ptr(ws)
         check(lib.hfm_group_wgrad(C.byref(a), st), "group_wgrad")
     return dw, db

@@ -400,7 +400,7 @@ def test_group_products_many_tiles(sizes, K, N):
     dw8, db8 = EX.group_wgrad(dz, a8, o)
     ap = A8.Act8(a8.codes[perm], a8.scales[perm])
     dw8p, db8p = EX.group_wgrad(dz, ap, o, src=src, top_k=3)
-    assert torch.equal(dw8, dw8p) and torch.equal(db8, db8p) and torch.equal(db8, db)
+    assert torch.equal(dw8, dw8p) and torch.equal(db8, db8p)
     h8 = A8.unpack(a8, torch.float32).double()
     for i, lo, hi in spans():
         xd, wd, zd = x[lo:hi].double(), w[i].double(), dz[lo:hi].double()
@@ -414,7 +414,8 @@ def test_group_products_many_tiles(sizes, K, N):
         check(dx[lo:hi], want, half * want.abs() + c * ((N + 4) * 0.5 * (zd.abs() @ wd.abs()) + want.abs()), "dx")
         check(dw[i], zd.T @ xd, c * (hi - lo + 4) * (zd.abs().T @ xd.abs()), "dw")
         check(dw8[i], zd.T @ h8[lo:hi], c * (hi - lo + 4) * (zd.abs().T @ h8[lo:hi]), "dw8")
-        check(db[i], zd.sum(0), c * (hi - lo + 4) * zd.abs().sum(0), "db")
+        for d in (db, db8):                    # (of two kernels where the width suits one of the types only)
+            check(d[i], zd.sum(0), c * (hi - lo + 4) * zd.abs().sum(0), "db")
     for i in range(E):
         if sizes[i] == 0:
             assert not dw[i].any() and not db[i].any() and not dw8[i].any()
