@@ -12,6 +12,8 @@
 //
 // A workgroup finds its expert by a scan over the group sizes in its own registers.  Accumulation is
 // fp32 on MFMA; nothing is summed by atomics.
+#include <type_traits>
+
 #include "act8.h"
 
 struct GroupNtArgs {
@@ -74,6 +76,19 @@ __device__ __forceinline__ bool group_find(const int* offs, int E, int S, int tm
     run += __shfl(inc, 63);
   }
   return false;
+}
+
+// row tiles of all groups
+template <int BM>
+__device__ __forceinline__ int group_tiles(const int* offs, int E, int S) {
+  const int lane = threadIdx.x & 63;
+  int n = 0, lo, hi;
+  for (int e = lane; e < E; e += 64) {
+    group_rows(offs, e, S, lo, hi);
+    n += (hi - lo + BM - 1) / BM;
+  }
+  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+  return __builtin_amdgcn_readfirstlane(n);
 }
 
 // the row of x behind sorted place p, or -1 (a slot that is none of the rows reads as zeros)
@@ -254,21 +269,22 @@ __device__ __forceinline__ void group_store8(const GroupNtArgs& g, int p, int n,
   }
 }
 
-// ------------------------------------------------------------------ 256 x 256 ping-pong products
-// 512 threads = 8 waves in two groups of 4 (group g owns rows g * 128 .., wave c of a group columns
-// c * 64 ..: 8 x 4 MFMA 16x16x32 tiles, 128 accumulators).  Every SIMD hosts one wave of each group and
-// the groups run one barrier apart: between two barriers one group reads the fragments of its next
-// phase from LDS and stages the next step by LDS-DMA while the other group's 16 MFMAs run.  A 64-deep
-// step is 4 phases of one 64 x 32 output quadrant, in the order (A0,B0) (A0,B1) (A1,B1) (A1,B0), so a
-// phase reads only the half that changes.  Staging of step t + 1 goes into the other buffer: group 1 in
-// its load slots 0-2, group 0 in 1-3 (the buffer's last reads retire in group 1's last compute slot of
-// step t - 1, which is group 0's load slot 0); each wave waits for its own DMA once per step, before
-// the barrier that publishes the step.
-// LDS: 2 buffers x (A 32 KB + B 32 KB).
-constexpr int GP_B = 256, GP_K = 64, GP_THREADS = 512;
-constexpr int GP_PANEL = GP_B * GP_K * 2, GP_BUF = 2 * GP_PANEL;
-
+// ------------------------------------------------------------------ 256 x 256 products
+// 256 threads = 4 waves, one per SIMD, of 128 x 128 outputs (4 x 4 MFMA 32x32x16 tiles: 256
+// accumulators; 32 cycles an MFMA leave room for the other instructions of the one wave).  The reduction runs in 32-deep steps through a ring of 4 LDS buffers (A 16 KB + B 16 KB
+// each).  In step s a wave multiplies fragments that it read during step s - 1, reads those of step s + 1
+// and starts the LDS-DMA of step s + 3, spread between the MFMAs, so that no load is waited for:
+// a fragment has 4 rounds of 128 cycles of MFMA or more to arrive, DMA two steps.  Row fragment i
+// is replaced after its round; the 8 column fragments serve all rounds and are held twice.
+//   Top of step s: the wave's own DMA of step s + 1 has landed; the barrier makes that true for all waves,
+//   and buffer (s + 3) % 4 = (s - 1) % 4 free: its fragments were multiplied in step s - 1.
+// A 128 x 128 block per wave reads 64 KB of fragments a step and CU and writes 32 KB: 768 cycles of LDS
+// against 1024 of MFMA; 128 x 64 blocks (8 waves) need 1024 + 256.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int GP_B = 256, GP_K = 32, GP_THREADS = 256;
+constexpr int GP_PANEL = GP_B * GP_K * 2, GP_BUF = 2 * GP_PANEL, GP_RING = 4;
 constexpr int GP_MIN_TILES = 128;
+
 __device__ __attribute__((aligned(16))) uint32_t g_zero16[4];      // the source of padding chunks
 
 __device__ __forceinline__ void dma16(const void* src, char* lds) {
@@ -276,32 +292,56 @@ __device__ __forceinline__ void dma16(const void* src, char* lds) {
                                    (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// One step's 4 phases on buffers `pa` / `pb`.  load_a(half), load_b(half) read fragments, stage(slot)
-// is called in this group's three staging slots (0 .. 2) of the step, wait() once before it ends.
-template <typename LA, typename LB, typename ST, typename MM>
-__device__ __forceinline__ void pp_step(int grp, LA load_a, LB load_b, ST stage, MM mma) {
+// 16 bytes a lane from `base` + soff + voff, zeros where that lies at or past `bytes` (the buffer's own check)
+__device__ __forceinline__ void dma16_buf(const void* base, uint32_t bytes, uint32_t voff, uint32_t soff, char* lds) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)voff, (int)soff, 0, 0);
+}
+
+// D: DMA pieces of a wave per step.  stage(i, step): piece i (0 .. D - 1) of a step, zeros from the step `ns`
+// on (the loop runs on a pair of steps at a time and three steps ahead, without a branch);
+// load_a(i, buf), load_b(j, buf): fragments; extra(parity, step): what else a step brings (8-bit inputs).
+template <int D, typename ST, typename LA, typename LB, typename EX>
+__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[4][4], ST stage, LA load_a, LB load_b, EX extra) {
+  bf16x8 fa[8], fb[2][8];
+  auto step = [&](auto PAR, int s) {
+    constexpr int c = decltype(PAR)::value, n = c ^ 1;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");        // (the DMA of step s + 2 stays in flight)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");          // (no access moves over the barrier)
+    __builtin_amdgcn_sched_barrier(0);
+    extra(PAR, s);
+    const char* nb = smem + ((s + 1) & (GP_RING - 1)) * GP_BUF;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int qa = (q == 0 || q == 1) ? 0 : 1, qb = (q == 0 || q == 3) ? 0 : 1;
-    if (q == 3 && grp == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (q == 0 || q == 2) load_a(qa);
-    load_b(qb);
-    stage(q - (grp == 0 ? 1 : 0));
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");          // (no access moves over a barrier)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(1);
-    mma(q, qa, qb);
-    __builtin_amdgcn_s_setprio(0);
-    if (q == 3 && grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
+    for (int k = 0; k < 32; ++k) {
+      const int r = k >> 2, j = k & 3;      // round r: row fragment r (16-deep half r >> 2, rows 32 (r & 3) ..)
+      acc[r & 3][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[c][(r >> 2) * 4 + j], acc[r & 3][j], 0, 0, 0);
+      // at most one load between two MFMAs: a wave issues an instruction every 4 cycles, an MFMA runs 32
+      if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1, nb);
+      if (j == 1 && r < 4) fb[n][2 * r] = load_b(2 * r, nb);
+      if (j == 2 && r < 4) fb[n][2 * r + 1] = load_b(2 * r + 1, nb);
+      if (j == 3 && r < D) stage(r, s + GP_RING - 1);
+      if (k == 31) fa[7] = load_a(7, nb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < GP_RING - 1; ++s)
+#pragma unroll
+    for (int i = 0; i < D; ++i) stage(i, s);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * D) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    fb[0][i] = load_b(i, smem);
+    fa[i] = load_a(i, smem);
   }
+  for (int s = 0; s < ns; s += 2) {
+    step(std::integral_constant<int, 0>{}, s);
+    step(std::integral_constant<int, 1>{}, s + 1);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");     // (nothing in flight into LDS)
 }
 
 // block b of n -> position in an order where each XCD (blocks go round the 8 of them) has a run of
@@ -311,34 +351,45 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
   return (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (b >> 3);
 }
 
-// A wave's 128 x 64 outputs leave through its 16 KB of LDS, 64 rows a pass, so that a lane holds 8
+// Tile t of a rows x cols grid, in bands of GP_BAND rows walked column by column: the 32 CUs of an XCD then
+// work on about 8 x 4 tiles, which share 12 panels (row by row, at 16 columns: 18, and the panels' way
+// from the other side of the L2 sets the time).
+constexpr int GP_BAND = 8;
+__device__ __forceinline__ void band_tile(int t, int rows, int cols, int& r, int& c) {
+  const int band = t / (GP_BAND * cols), r0 = band * GP_BAND, h = min(GP_BAND, rows - r0);
+  const int i = t - r0 * cols;
+  r = r0 + i % h;
+  c = i / h;
+}
+
+// A wave's 128 x 128 outputs leave through its 32 KB of LDS, 64 rows a pass, so that a lane holds 8
 // neighbouring columns of a row: emit(row in the block, first column in the block, 8 values).
 template <typename F>
-__device__ __forceinline__ void pp_emit(const f32x4 (&acc)[8][4], char* img, int lane, F emit) {
+__device__ __forceinline__ void mm_emit(const f32x16 (&acc)[4][4], char* img, int lane, F emit) {
   // (the lane hidden from the optimizer: in a loop over tiles it would otherwise keep the image's
   // addresses in registers through the product, which has none left)
   asm volatile("" : "+v"(lane));
-  const int fr = lane & 15, fq = lane >> 4;
+  const int fr = lane & 31, fq = lane >> 5;
   auto wsync = [] {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  // rows of 64 floats; 16-byte chunk c of row r at chunk c ^ (r & 15)
-  auto off = [](int r, int c) { return r * 256 + ((((c >> 2) ^ (r & 15))) << 4) + (c & 3) * 4; };
+  // rows of 128 floats; 16-byte chunk c of row r at chunk c ^ (r & 15)
+  auto off = [](int r, int c) { return r * 512 + ((((c >> 2) ^ (r & 15))) << 4) + (c & 3) * 4; };
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<float*>(img + off(i * 16 + fq * 4 + k, j * 16 + fr)) = acc[p * 4 + i][j][k];
+        for (int q = 0; q < 16; ++q)
+          *reinterpret_cast<float*>(img + off(i * 32 + (q >> 2) * 8 + fq * 4 + (q & 3), j * 32 + fr)) = acc[p * 2 + i][j][q];
     wsync();
 #pragma unroll 2
-    for (int it = 0; it < 8; ++it) {
-      const int r = it * 8 + (lane >> 3), c = (lane & 7) * 8;
+    for (int it = 0; it < 16; ++it) {
+      const int r = it * 4 + (lane >> 4), c = (lane & 15) * 8;
       const f32x4 a = *reinterpret_cast<const f32x4*>(img + off(r, c));
       const f32x4 b = *reinterpret_cast<const f32x4*>(img + off(r, c + 4));
       const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -348,126 +399,70 @@ __device__ __forceinline__ void pp_emit(const f32x4 (&acc)[8][4], char* img, int
   }
 }
 
-// ---- NT: rows of A and B are K-contiguous, LDS image as in the 128 x 128 kernel.  K a multiple of 8;
-// the last step's chunks past K come from the zero source.
-__global__ void __launch_bounds__(GP_THREADS, 1) group_nt_pp_kernel(GroupNtArgs g, int tiles_n, int ovec) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * GP_BUF];
-  const int tile = xcd_order(blockIdx.x, gridDim.x);
+// ---- NT: rows of A and B are K-contiguous.  A panel's step is 256 rows x 64 B; 16-byte chunk c of row r
+// lies at c ^ ((r >> 2) & 3): the 16 rows of a fragment read meet in 16 different chunks of 256 B.  K a
+// multiple of 8; the last step's chunks past K come from the zero source.
+__global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
+group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int ovec) {
+  __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
+  // (the grid has room for one more row tile per group: the tiles that there are go round the XCDs)
+  const int tiles_m = group_tiles<GP_B>(g.offs, g.E, g.S);
+  if ((int)blockIdx.x >= tiles_m * tiles_n) return;
+  int tm, tn;
+  band_tile(xcd_order(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   int e, r0, r1;
-  if (!group_find<GP_B>(g.offs, g.E, g.S, tile / tiles_n, e, r0, r1)) return;
-  const int n0 = (tile % tiles_n) * GP_B;
+  if (!group_find<GP_B>(g.offs, g.E, g.S, tm, e, r0, r1)) return;
+  const int n0 = tn * GP_B;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int grp = wave >> 2, wc = wave & 3;
-  const int fr = lane & 15, fq = lane >> 4, swz = (fr >> 1) & 7;
-  const int la[2] = {(grp * 128 + fr) * 128 + ((fq ^ swz) << 4), (grp * 128 + fr) * 128 + (((4 + fq) ^ swz) << 4)};
-  const int lb[2] = {(wc * 64 + fr) * 128 + ((fq ^ swz) << 4), (wc * 64 + fr) * 128 + (((4 + fq) ^ swz) << 4)};
-  // staging pieces of 8 rows x 128 B: 4 of A and 4 of B per wave.  Rows past the group's end and
+  const int wr = wave >> 1, wc = wave & 1;
+  const int fr = lane & 31, fq = lane >> 5;
+  // fragment (half h, rows 32 i ..): row fr, chunk 2 h + fq
+  const int f0 = fr * 64 + ((fq ^ ((fr >> 2) & 3)) << 4), f1 = f0 ^ 32;
+  const int la = wr * 128 * 64, lb = GP_PANEL + wc * 128 * 64;
+  // staging pieces of 16 rows x 64 B: 4 of A and 4 of B per wave.  Rows past the group's end and
   // columns past N read the last one (their outputs are not stored).
   const bf16* src[8];
-  int ck[8];
+  bool none[4];                                              // (a source that is no slot: zeros)
+  const int ck = ((lane & 3) ^ ((lane >> 4) & 3)) * 8;       // (row of the piece: lane >> 2)
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
-    const int r = (wave * 4 + (p & 3)) * 8 + (lane >> 3);
-    ck[p] = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    const int r = (wave * 4 + (p & 3)) * 16 + (lane >> 2);
     if (p < 4) {
-      const int row = max(group_row(g.src, min(r0 + r, r1 - 1), g.rows, g.top_k), 0);
-      src[p] = g.a + (size_t)row * g.lda + ck[p];
+      const int row = group_row(g.src, min(r0 + r, r1 - 1), g.rows, g.top_k);
+      src[p] = g.a + (size_t)max(row, 0) * g.lda + ck;
+      none[p] = row < 0;
     } else {
-      src[p] = g.b + (size_t)e * g.es + (size_t)min(n0 + r, g.N - 1) * g.ldb + ck[p];
+      src[p] = g.b + (size_t)e * g.es + (size_t)min(n0 + r, g.N - 1) * g.ldb + ck;
     }
   }
-  const int nt = (g.K + GP_K - 1) / GP_K;
-  const bool ragged = (g.K & (GP_K - 1)) != 0;
-  auto piece = [&](int p, char* buf, int t) {
-    const void* s = src[p] + t * GP_K;
-    if (ragged && t == nt - 1 && t * GP_K + ck[p] >= g.K) s = g_zero16;
-    dma16(s, buf + (p >= 4 ? GP_PANEL : 0) + (wave * 4 + (p & 3)) * 1024);
-  };
-  f32x4 acc[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int p = 0; p < 8; ++p) piece(p, smem, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  if (grp == 1) {                         // the stagger: group 1 runs one slot behind
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  bf16x8 fa[4][2], fb[2][2];
-  for (int t = 0; t < nt; ++t) {
-    const char* pa = smem + (t & 1) * GP_BUF;
-    const char* pb = pa + GP_PANEL;
-    char* nxt = smem + ((t + 1) & 1) * GP_BUF;
-    pp_step(
-        grp,
-        [&](int h) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-              fa[i][ks] = *reinterpret_cast<const bf16x8*>(pa + la[ks] + (h * 64 + i * 16) * 128);
-        },
-        [&](int h) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-              fb[j][ks] = *reinterpret_cast<const bf16x8*>(pb + lb[ks] + (h * 32 + j * 16) * 128);
-        },
-        [&](int s) {
-          if (t + 1 >= nt) return;
-          if (s == 0)
-            for (int p = 0; p < 3; ++p) piece(p, nxt, t + 1);
-          if (s == 1)
-            for (int p = 3; p < 6; ++p) piece(p, nxt, t + 1);
-          if (s == 2)
-            for (int p = 6; p < 8; ++p) piece(p, nxt, t + 1);
-        },
-        [&](int, int qa, int qb) {
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                acc[qa * 4 + i][qb * 2 + j] =
-                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][ks], fb[j][ks], acc[qa * 4 + i][qb * 2 + j], 0, 0, 0);
-        });
-  }
-  if (grp == 0) __builtin_amdgcn_s_barrier();   // (every wave passes the same number of barriers)
+  f32x16 acc[4][4] = {};
+  mm_loop<8>(
+      smem, (g.K + GP_K - 1) / GP_K, acc,
+      [&](int p, int s) {
+        const void* q = src[p] + s * GP_K;
+        const bool zero = (s * GP_K + ck >= g.K) | (p < 4 ? none[p & 3] : false);
+        q = zero ? (const void*)g_zero16 : q;
+        dma16(q, smem + (s & (GP_RING - 1)) * GP_BUF + (p >= 4 ? GP_PANEL : 0) + (wave * 4 + (p & 3)) * 1024);
+      },
+      [&](int i, const char* b) { return *reinterpret_cast<const bf16x8*>(b + la + (i < 4 ? f0 : f1) + (i & 3) * 32 * 64); },
+      [&](int j, const char* b) { return *reinterpret_cast<const bf16x8*>(b + lb + (j < 4 ? f0 : f1) + (j & 3) * 32 * 64); },
+      [](auto, int) {});
   __syncthreads();
-  // a source that is no slot: a row of zeros
-  if (g.src) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int p = r0 + grp * 128 + i * 16 + fq * 4 + q;
-        if (p < r1 && group_row(g.src, p, g.rows, g.top_k) < 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j][q] = 0.f;
-        }
-      }
-  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int n = n0 + wc * 64 + j * 16 + fr;
+    const int n = n0 + wc * 128 + j * 32 + fr;
     const float bias = g.bias && n < g.N ? g.bias[(size_t)e * g.N + n] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 16; ++q) {
         float v = acc[i][j][q] * g.scale + bias;
         if (g.relu && v < 0.f) v = 0.f;
         acc[i][j][q] = v;
       }
   }
-  pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
-    const int p = r0 + grp * 128 + r, n = n0 + wc * 64 + c;
+  mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
+    const int p = r0 + wr * 128 + r, n = n0 + wc * 128 + c;
     if (p < r1 && n < g.N) group_store8(g, p, n, v, ovec);
   });
 }
@@ -480,11 +475,11 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
                    g.es % 8 == 0;
   const bool ovec = g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0 &&
                     (!g.mask || (g.ldm % 8 == 0 && (uintptr_t)g.mask % (g.mask8 ? 8 : 16) == 0));
-  if (vec && g.K >= GP_K) {
+  if (vec && g.K >= 64) {
     const int tn = (g.N + GP_B - 1) / GP_B;
     const long blocks = (long)(g.S / GP_B + g.E) * tn;
     if (blocks >= GP_MIN_TILES && blocks <= 0x7FFFFFFFl) {
-      hipLaunchKernelGGL(group_nt_pp_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn, ovec ? 1 : 0);
+      hipLaunchKernelGGL(group_nt_mm_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn, ovec ? 1 : 0);
       HFM_LAUNCH_CHECK();
     }
   }
@@ -654,21 +649,22 @@ __global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
   (i < nw ? g.dw[i] : g.db[i - nw]) = v;
 }
 
-// ---- TN: the weight gradient on the ping-pong tile.  Both panels keep their global layout, [64 rows][256
+// ---- TN: the weight gradient on the large tile.  Both panels keep their global layout, [32 rows][256
 // columns]; the fragments (8 rows of one column per lane) come from transposing LDS reads
 // (ds_read_b64_tr_b16: a 16-lane group reads 4 rows x 16 columns, lane l gets column l's 4 rows).
 // A panel row is 512 B, so a fragment's 16 rows would meet in the same banks: 32-byte granule c of row r
 // lies at c ^ f(r), f(r) = (r & 3) | (r >> 1 & 4), which spreads them over all 8 granules of 256 B.
-// 8-bit x: 16 codes a thread are loaded one step ahead, turned into bf16 times the block's scale
-// (one conversion per pair, exact) and written into the same image.
+// 8-bit x: 32 codes a thread (one scale) are loaded two steps ahead, turned into bf16 times the
+// scale (one conversion per pair, exact) and written into the same image.
 //
-// The work is cut evenly, not by tiles: `units` = 64-row steps of all tiles (a group without rows counts
+// The work is cut evenly, not by tiles: `units` = 64-row blocks of all tiles (a group without rows counts
 // one per tile, which writes its zeros), tiles in expert order, and workgroup w takes the units from
 // w U / W to (w + 1) U / W.  A tile within one workgroup goes straight to dw; a workgroup's first and last tile
 // may be parts, which go to its two workspace tiles and are summed in row order by a second launch.
 // Groups of any sizes thus load the CUs evenly (by whole tiles the fullest of 16 groups set the
 // time), for at most 512 tiles of 256 KB.
-constexpr int GW_SLAB = GP_B * GP_B + GP_B;      // floats of a workspace tile: dw part, db part
+constexpr int GW_UNIT = 64;                      // rows of a unit
+constexpr int GW_SLAB = GP_B * GP_B;             // floats of a workspace tile
 
 struct WgCut {
   long u0, u1;             // the workgroup's units
@@ -683,7 +679,7 @@ __device__ __forceinline__ int wg_owner(long U, int W, long u) {        // the w
 __device__ __forceinline__ int wg_steps(const int* offs, int e, int S) {
   int lo, hi;
   group_rows(offs, e, S, lo, hi);
-  return max(1, (hi - lo + GP_K - 1) / GP_K);
+  return max(1, (hi - lo + GW_UNIT - 1) / GW_UNIT);
 }
 // a value that is the same in all lanes, into scalar registers
 __device__ __forceinline__ long uni64(long v) {
@@ -725,44 +721,47 @@ __device__ __forceinline__ void wg_find(const int* offs, int E, int S, int tiles
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ bf16x8 tr_read(const char* p0, const char* p1) {
+// (restrict: a transposing read carries no type that would tell it from the LDS-DMA in flight, and without
+// an aliasing fact the compiler waits for all DMA before each; mm_loop has the waits that are needed)
+__device__ __forceinline__ bf16x8 tr_read(const char* __restrict__ p0, const char* __restrict__ p1) {
   typedef __attribute__((address_space(3))) s16x4* lp;
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p0);
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p1);
-  const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  return __builtin_bit_cast(bf16x8, v);
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// 16 bytes into LDS (restrict: as for tr_read)
+__device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(a, b, c, d);
 }
 
 template <bool X8, bool GATHER>
-__global__ void __launch_bounds__(GP_THREADS, 1) group_wgrad_pp_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int ovec) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * GP_BUF];
+__global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
+group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int ovec) {
+  __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int grp = wave >> 2, wc = wave & 3;
-  const int fr = lane & 15, fq = lane >> 4;
+  const int wr = wave >> 1, wc = wave & 1;
   const int tiles = tiles_n * tiles_k;
   const int w = xcd_order(blockIdx.x, gridDim.x);
   const WgCut cut = wg_cut(wg_units(g.offs, g.E, g.S, tiles), gridDim.x, w);
   int e;
   long first;
   wg_find(g.offs, g.E, g.S, tiles, cut.u0, e, first);
-  // fragment addresses: granule (base + i) ^ f(row) = f-and-base part ^ i, rows of fq and fr >> 2
-  const int fsw = (fr >> 2) | ((fq & 1) << 2);
-  const int rowoff = (fq * 8 + (fr >> 2)) * 512 + (fr & 3) * 8;
-  int la = rowoff + ((grp * 8 ^ fsw) << 5), lb = rowoff + ((wc * 4 ^ fsw) << 5);
+  // fragment (half h, columns 32 i ..): the lane's 16-lane group takes rows 16 h + 8 (lane >> 5) .. and
+  // columns 32 i + (lane & 16) ..: granule (2 i + (lane >> 4 & 1)) ^ f(row), which is an xor with 2 i
+  const int l4 = (lane >> 2) & 3, h5 = lane >> 5;
+  const int rowoff = (h5 * 8 + l4) * 512 + (lane & 3) * 8 + ((((lane >> 4) & 1) ^ l4 ^ (h5 << 2)) << 5);
+  int la = rowoff + wr * 256, lb = GP_PANEL + rowoff + wc * 256;
   // staging pieces: 2 rows of 512 B, 4 of each operand per wave.  Row 2 i + hi of the wave's 8 has
   // f = ((2 i + hi) & 3) | 4 (wave & 1), so the lane's 16-byte chunk is one column for even i and
   // that column ^ 32 for odd i.
   const int hi = lane >> 5, c16 = lane & 31;
   const int ce = (((c16 >> 1) ^ (hi | ((wave & 1) << 2))) * 2 + (c16 & 1)) * 8;
   const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
-  // 8-bit x: 16 codes at column xc of rows xr, xr + 32
-  const int xr = threadIdx.x >> 4, xc = (threadIdx.x & 15) * 16;
-  const int xo = GP_PANEL + xr * 512 + (((xc >> 4) ^ ((xr & 3) | ((xr >> 1) & 4))) << 5);
-  bf16x8 ones;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) ones[j] = f2bf(1.f);
-
+  // 8-bit x: 32 codes (granules 2 q, 2 q + 1) of row xr
+  const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32;
+  const int xf = (xr & 3) | ((xr >> 1) & 4);
+  const int xo = GP_PANEL + xr * 512 + (((2 * xq) ^ xf) << 5);        // (granule 2 q + 1: ^ 32)
   long u = cut.u0;
   while (u < cut.u1) {
     int steps = wg_steps(g.offs, e, g.S);
@@ -775,196 +774,144 @@ __global__ void __launch_bounds__(GP_THREADS, 1) group_wgrad_pp_kernel(GroupWgAr
     group_rows(g.offs, e, g.S, lo, hi_row);
     const int ti = (int)((u - first) / steps), s0 = (int)((u - first) % steps);
     const int s1 = (int)min((long)steps, s0 + (cut.u1 - u));
-    const int n0 = (ti / tiles_k) * GP_B, k0 = (ti % tiles_k) * GP_B;
-    const int p0 = lo + s0 * GP_K, p1 = min(hi_row, lo + s1 * GP_K);
-    const int nt = p1 > p0 ? (p1 - p0 + GP_K - 1) / GP_K : 0;
-    const bool ragged = ((p1 - p0) & (GP_K - 1)) != 0;
-    const bool sum = g.db != nullptr && k0 == 0;
-    f32x4 acc[8][4], accb[2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    accb[0] = accb[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    // columns past N or K read column 0 (their outputs are not stored), rows past p1 the zero source
-    // (the last step only).  Scalar row base + the lane's 32-bit byte offset.
+    int tn, tk;
+    band_tile(ti, tiles_n, tiles_k, tn, tk);
+    const int n0 = tn * GP_B, k0 = tk * GP_B;
+    // (scalar for certain: the buffers below are made of them)
+    const int p0 = __builtin_amdgcn_readfirstlane(lo + s0 * GW_UNIT);
+    const int p1 = __builtin_amdgcn_readfirstlane(min(hi_row, lo + s1 * GW_UNIT));
+    const int ns = p1 > p0 ? (p1 - p0 + GP_K - 1) / GP_K : 0;
+    f32x16 acc[4][4] = {};
+    // columns past N or K read column 0 (their outputs are not stored)
     const uint32_t ao0 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + ce < g.N ? n0 + ce : 0));
     const uint32_t ao1 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + (ce ^ 32) < g.N ? n0 + (ce ^ 32) : 0));
     const int bc0 = k0 + ce < g.K ? k0 + ce : 0, bc1 = k0 + (ce ^ 32) < g.K ? k0 + (ce ^ 32) : 0;
-    const bool xin = k0 + xc < g.K;
-    int xrow[4];                                       // GATHER: x rows of the next step's pieces (-1: zeros)
-    uint4 cd[2];
-    uint32_t cs[2];
-    auto piece_a = [&](int i, char* buf, int t) {
-      const int p = p0 + t * GP_K + wave * 8 + 2 * i;
-      const void* s = reinterpret_cast<const char*>(g.dz + (size_t)p * g.ldz) + ((i & 1) ? ao1 : ao0);
-      if (ragged && t == nt - 1 && p + hi >= p1) s = g_zero16;
-      dma16(s, buf + (wave * 4 + i) * 1024);
+    const uint32_t bo0 = GATHER ? 0u : 2u * (uint32_t)(hi * (int)g.ldx + bc0);
+    const uint32_t bo1 = GATHER ? 0u : 2u * (uint32_t)(hi * (int)g.ldx + bc1);
+    // GATHER: rows of x of a step's pieces (or of its codes), read two steps before they are used;
+    // -1: a row of zeros (past p1, or a source that is no slot)
+    int xrow[2][4];
+    auto row_at = [&](int p) {
+      const int s = g.src[min(p, g.S - 1)], r = s / g.top_k;
+      return p < p1 && s >= 0 && r < g.rows ? r : -1;
     };
-    auto rows_of = [&](int t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int p = p0 + t * GP_K + wave * 8 + 2 * i + hi;
-        xrow[i] = p < p1 ? group_row(g.src, p, g.rows, g.top_k) : -1;
-      }
-    };
-    auto piece_b = [&](int i, char* buf, int t) {
-      const bf16* xb = reinterpret_cast<const bf16*>(g.x);
-      const void* s;
-      if (GATHER) {
-        s = xrow[i] >= 0 ? (const void*)(xb + (size_t)(uint32_t)xrow[i] * g.ldx + ((i & 1) ? bc1 : bc0)) : (const void*)g_zero16;
+    auto rows_of = [&](int set, int s) {
+      if (!GATHER) return;
+      if (X8) {
+        xrow[set][0] = row_at(p0 + s * GP_K + xr);
       } else {
-        const int p = p0 + t * GP_K + wave * 8 + 2 * i;
-        s = reinterpret_cast<const char*>(xb + (size_t)p * g.ldx) + 2u * (uint32_t)(hi * (int)g.ldx + ((i & 1) ? bc1 : bc0));
-        if (ragged && t == nt - 1 && p + hi >= p1) s = g_zero16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xrow[set][i] = row_at(p0 + s * GP_K + wave * 8 + 2 * i + hi);
       }
-      dma16(s, buf + GP_PANEL + (wave * 4 + i) * 1024);
     };
-    auto codes_of = [&](int t) {                       // X8: the codes of step t into registers
+    // A step's rows of the wave as a buffer that ends with the last row of the part: past it read zeros
+    auto bytes_left = [&](int s, uint32_t row) {
+      const int n = p1 - (p0 + s * GP_K + wave * 8);
+      return (uint32_t)__builtin_amdgcn_readfirstlane((n < 0 ? 0 : n > 8 ? 8 : n) * (int)row);
+    };
+    auto piece_a = [&](int i, int s) {
+      const bf16* base = g.dz + (size_t)(p0 + s * GP_K + wave * 8) * g.ldz;
+      const uint32_t row = 2u * (uint32_t)g.ldz;
+      dma16_buf(base, bytes_left(s, row), (i & 1) ? ao1 : ao0, 2u * i * row,
+                smem + (s & (GP_RING - 1)) * GP_BUF + (wave * 4 + i) * 1024);
+    };
+    auto piece_b = [&](int i, int s, int row) {
+      char* to = smem + (s & (GP_RING - 1)) * GP_BUF + GP_PANEL + (wave * 4 + i) * 1024;
+      const bf16* xb = reinterpret_cast<const bf16*>(g.x);
+      if (GATHER) {
+        const void* q = row >= 0 ? (const void*)(xb + (size_t)(uint32_t)row * g.ldx + ((i & 1) ? bc1 : bc0)) : (const void*)g_zero16;
+        dma16(q, to);
+      } else {
+        const uint32_t rb = 2u * (uint32_t)g.ldx;
+        dma16_buf(xb + (size_t)(p0 + s * GP_K + wave * 8) * g.ldx, bytes_left(s, rb), (i & 1) ? bo1 : bo0,
+                  2u * i * rb, to);
+      }
+    };
+    // X8: a step's codes and scale into registers (set), and from there into the image
+    // (as loaded: a row that is none is cleared on the way to the image, where the loads have arrived)
+    uint4 cd[2][2];
+    uint32_t cs[2], con[2];
+    const bool x0 = k0 + xc < g.K, x1 = k0 + xc + 16 < g.K;     // (columns past K: any values)
+    auto codes_of = [&](int set, int s) {
+      const int p = p0 + s * GP_K + xr;
+      const int row = GATHER ? xrow[set][0] : (p < p1 ? p : -1);
+      con[set] = row >= 0 ? 0xFFFFFFFFu : 0u;
+      const size_t at = row >= 0 ? (size_t)row : 0;     // (row 0 is there: the part has rows)
+      const uint8_t* q = reinterpret_cast<const uint8_t*>(g.x) + at * g.ldx + (x0 ? k0 + xc : 0);
+      cd[set][0] = *reinterpret_cast<const uint4*>(q);
+      cd[set][1] = *reinterpret_cast<const uint4*>(x1 ? q + 16 : q);
+      cs[set] = g.xs[at * sblk + (x0 ? (k0 + xc) / A8_BLOCK : 0)];
+    };
+    auto codes_to = [&](int set, int s) {
+      char* d = smem + (s & (GP_RING - 1)) * GP_BUF;
+      const float f = a8_scale(cs[set]);
+      const uint32_t m = con[set];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int pb = p0 + t * GP_K + 32 * h, p = pb + xr;
-        cd[h] = make_uint4(0, 0, 0, 0);
-        cs[h] = 127;
-        if (p < p1 && xin) {
-          const uint8_t* x8 = reinterpret_cast<const uint8_t*>(g.x) + k0;
-          if (GATHER) {
-            const int row = group_row(g.src, p, g.rows, g.top_k);
-            if (row >= 0) {
-              cd[h] = *reinterpret_cast<const uint4*>(x8 + (size_t)row * g.ldx + xc);
-              cs[h] = g.xs[(size_t)row * sblk + (k0 + xc) / A8_BLOCK];
-            }
-          } else {
-            cd[h] = *reinterpret_cast<const uint4*>(x8 + (size_t)pb * g.ldx + (uint32_t)(xr * (int)g.ldx + xc));
-            cs[h] = g.xs[(size_t)pb * sblk + (uint32_t)(xr * sblk + (k0 + xc) / A8_BLOCK)];
-          }
-        }
+        const uint4 c = make_uint4(cd[set][h].x & m, cd[set][h].y & m, cd[set][h].z & m, cd[set][h].w & m);
+        char* o = d + (xo ^ (h << 5));
+        lds_put(o, a8_pair_bf16<false>(c.x, f), a8_pair_bf16<true>(c.x, f), a8_pair_bf16<false>(c.y, f),
+                a8_pair_bf16<true>(c.y, f));
+        lds_put(o + 16, a8_pair_bf16<false>(c.z, f), a8_pair_bf16<true>(c.z, f), a8_pair_bf16<false>(c.w, f),
+                a8_pair_bf16<true>(c.w, f));
       }
     };
-    auto codes_to = [&](char* buf) {                   // X8: registers -> bf16 image
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {                    // (row + 32: the same f)
-        const float s = a8_scale(cs[h]);
-        char* d = buf + xo + h * 32 * 512;
-        *reinterpret_cast<uint4*>(d) = make_uint4(a8_pair_bf16<false>(cd[h].x, s), a8_pair_bf16<true>(cd[h].x, s),
-                                                  a8_pair_bf16<false>(cd[h].y, s), a8_pair_bf16<true>(cd[h].y, s));
-        *reinterpret_cast<uint4*>(d + 16) = make_uint4(a8_pair_bf16<false>(cd[h].z, s), a8_pair_bf16<true>(cd[h].z, s),
-                                                       a8_pair_bf16<false>(cd[h].w, s), a8_pair_bf16<true>(cd[h].w, s));
-      }
+    // (la and lb are hidden from the optimizer in every step: 16 addresses made by one xor each, not kept)
+    auto hide = [&]() {
+      int a = la, b = lb;
+      asm volatile("" : "+v"(a), "+v"(b));
+      la = a;
+      lb = b;
     };
-    if (nt > 0) {
-      if (X8) codes_of(0);
-      else if (GATHER) rows_of(0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        piece_a(i, smem, 0);
-        if (!X8) piece_b(i, smem, 0);
+    auto frag = [](const char* p) { return tr_read(p, p + 4 * 512); };
+    auto load_a = [&](int i, const char* b) { return frag(b + (la ^ ((i & 3) << 6)) + (i >> 2) * 16 * 512); };
+    auto load_b = [&](int j, const char* b) { return frag(b + (lb ^ ((j & 3) << 6)) + (j >> 2) * 16 * 512); };
+    if (ns > 0) {
+      rows_of(0, 0);
+      rows_of(1, 1);
+      if constexpr (X8) {
+        // the codes of step s + 3 (read in step s - 2) go to the image in step s, those of s + 5 are read;
+        // they are in LDS before the fragments read at the end of step s, so before step s + 2 reads them
+        codes_of(0, 0);
+        codes_of(1, 1);
+        codes_to(0, 0);
+        codes_to(1, 1);
+        rows_of(0, 2);
+        rows_of(1, 3);
+        codes_of(0, 2);
+        codes_to(0, 2);
+        rows_of(0, 4);
+        codes_of(1, 3);
+        codes_of(0, 4);
+        rows_of(1, 5);
+        rows_of(0, 6);
+        mm_loop<4>(smem, ns, acc, piece_a, load_a, load_b, [&](auto PAR, int s) {
+          constexpr int set = decltype(PAR)::value ^ 1;
+          hide();
+          codes_to(set, s + 3);
+          codes_of(set, s + 5);
+          rows_of(set, s + 7);
+        });
+      } else {
+        // GATHER: a step's rows are read two steps before its DMA starts
+        mm_loop<8>(
+            smem, ns, acc,
+            [&](int i, int s) {
+              if (i < 4) piece_a(i, s);
+              else piece_b(i - 4, s, xrow[s & 1][i - 4]);
+              if (i == 7) rows_of(s & 1, s + 2);
+            },
+            load_a, load_b, [&](auto, int) { hide(); });
       }
-      if (X8) {
-        codes_to(smem);
-        if (nt > 1) codes_of(1);
-      } else if (GATHER && nt > 1) {
-        rows_of(1);
-      }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (grp == 1) {
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    bf16x8 fa[4][2], fb[2][2];
-    for (int t = 0; t < nt; ++t) {
-      const char* pa = smem + (t & 1) * GP_BUF;
-      const char* pb = pa + GP_PANEL;
-      char* nxt = smem + ((t + 1) & 1) * GP_BUF;
-      asm volatile("" : "+v"(la), "+v"(lb));           // (12 addresses made by one xor each, not kept)
-      pp_step(
-          grp,
-          [&](int h) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int ks = 0; ks < 2; ++ks) {
-                const char* a = pa + (la ^ ((h * 4 + i) << 5)) + ks * 32 * 512;
-                fa[i][ks] = tr_read(a, a + 4 * 512);
-              }
-          },
-          [&](int h) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int ks = 0; ks < 2; ++ks) {
-                const char* b = pb + (lb ^ ((h * 2 + j) << 5)) + ks * 32 * 512;
-                fb[j][ks] = tr_read(b, b + 4 * 512);
-              }
-          },
-          [&](int s) {
-            if (t + 1 >= nt) return;
-            if (X8) {
-              if (s == 0) codes_to(nxt);
-              if (s == 1) {
-                piece_a(0, nxt, t + 1);
-                piece_a(1, nxt, t + 1);
-                if (t + 2 < nt) codes_of(t + 2);
-              }
-              if (s == 2) {
-                piece_a(2, nxt, t + 1);
-                piece_a(3, nxt, t + 1);
-              }
-            } else {
-              if (s == 0) {
-                piece_a(0, nxt, t + 1);
-                piece_a(1, nxt, t + 1);
-                piece_a(2, nxt, t + 1);
-              }
-              if (s == 1) {
-                piece_a(3, nxt, t + 1);
-                piece_b(0, nxt, t + 1);
-                piece_b(1, nxt, t + 1);
-              }
-              if (s == 2) {
-                piece_b(2, nxt, t + 1);
-                piece_b(3, nxt, t + 1);
-                if (GATHER && t + 2 < nt) rows_of(t + 2);
-              }
-            }
-          },
-          [&](int q, int qa, int qb) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  acc[qa * 4 + i][qb * 2 + j] =
-                      __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i][ks], fb[j][ks], acc[qa * 4 + i][qb * 2 + j], 0, 0, 0);
-            // db: dz against a column of ones; wave c of a group takes row tiles 2 c, 2 c + 1
-            if (sum && (q & 1) == 0 && (wc >> 1) == qa) {
-#pragma unroll
-              for (int ks = 0; ks < 2; ++ks) {
-                if (wc & 1) {
-                  accb[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2][ks], ones, accb[0], 0, 0, 0);
-                  accb[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[3][ks], ones, accb[1], 0, 0, 0);
-                } else {
-                  accb[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[0][ks], ones, accb[0], 0, 0, 0);
-                  accb[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[1][ks], ones, accb[1], 0, 0, 0);
-                }
-              }
-            }
-          });
-    }
-    if (grp == 0) __builtin_amdgcn_s_barrier();
     __syncthreads();
     // a whole tile goes to dw, a part to the workspace: slot 2 w if it is the workgroup's first, 2 w + 1
     // if it goes on in the next one
     const bool whole = s0 == 0 && s1 == steps;
     if (whole) {
       float* dw = g.dw + (size_t)e * g.N * g.K;
-      pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
-        const int n = n0 + grp * 128 + r, k = k0 + wc * 64 + c;
+      mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
+        const int n = n0 + wr * 128 + r, k = k0 + wc * 128 + c;
         if (n >= g.N || k >= g.K) return;
         float* d = dw + (size_t)n * g.K + k;
         if (ovec) {
@@ -978,22 +925,11 @@ __global__ void __launch_bounds__(GP_THREADS, 1) group_wgrad_pp_kernel(GroupWgAr
       });
     } else {
       float* slab = g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB;
-      pp_emit(acc, smem + wave * 16384, lane, [&](int r, int c, const float (&v)[8]) {
-        float* d = slab + (grp * 128 + r) * GP_B + wc * 64 + c;
+      mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
+        float* d = slab + (wr * 128 + r) * GP_B + wc * 128 + c;
         *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
       });
-    }
-    if (sum && fr == 0) {
-      float* db = whole ? g.db + (size_t)e * g.N : g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB + GP_B * GP_B;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = grp * 128 + (wc * 2 + i) * 16 + fq * 4 + q;
-          if (!whole) db[r] = accb[i][q];
-          else if (n0 + r < g.N) db[n0 + r] = accb[i][q];
-        }
     }
     u += s1 - s0;
     __syncthreads();                      // (the next tile's staging reuses the images)
@@ -1020,7 +956,9 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
   const long a = before * tiles + (long)ti * steps, b = a + steps - 1;
   const int w0 = wg_owner(U, W, a), w1 = wg_owner(U, W, b);
   if (w0 == w1) return;
-  const int n0 = (ti / tiles_k) * GP_B, k0 = (ti % tiles_k) * GP_B;
+  int tn, tk;
+  band_tile(ti, tiles_n, tiles_k, tn, tk);
+  const int n0 = tn * GP_B, k0 = tk * GP_B;
   // the part that starts the tile is the last of w0 (slot 1), the others are the first of theirs
   auto slab = [&](int w) { return g.ws + (size_t)(2 * w + (w == w0 ? 1 : 0)) * GW_SLAB; };
   const int row0 = blockIdx.z * 64;
@@ -1038,12 +976,53 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
         if (k0 + c + j < g.K) d[j] = v[j];
     }
   }
-  if (g.db && k0 == 0 && threadIdx.x < 64 && n0 + row0 + threadIdx.x < g.N) {
-    const int r = row0 + threadIdx.x;
-    float v = slab(w0)[GP_B * GP_B + r];
-    for (int q = w0 + 1; q <= w1; ++q) v += slab(q)[GP_B * GP_B + r];
-    g.db[(size_t)e * g.N + n0 + r] = v;
+}
+
+// db of the large tile's path: column sums of dz, chunks of GW_DBROWS rows of a group (256 columns: 32
+// lanes of 8 columns, 8 rows at a time), then the group's chunks in order.  Beside the product rather
+// than in it: a ninth fragment column there costs its loop registers or a branch.
+constexpr int GW_DBROWS = 256;
+__global__ void __launch_bounds__(256) group_db_part_kernel(GroupWgArgs g, float* part) {
+  int e, r0, r1;
+  if (!group_find<GW_DBROWS>(g.offs, g.E, g.S, blockIdx.x, e, r0, r1)) return;
+  __shared__ float red[8][256];
+  const int c = threadIdx.x & 31, rl = threadIdx.x >> 5, n = blockIdx.y * 256 + c * 8;
+  const int end = min(r1, r0 + GW_DBROWS);
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  if (n < g.N) {
+#pragma unroll 4
+    for (int p = r0 + rl; p < end; p += 8) {
+      const bf16x8 v = *reinterpret_cast<const bf16x8*>(g.dz + (size_t)p * g.ldz + n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += bf2f(v[j]);
+    }
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[rl][c * 8 + j] = s[j];
+  __syncthreads();
+  const int col = blockIdx.y * 256 + threadIdx.x;
+  float t = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) t += red[q][threadIdx.x];
+  if (col < g.N) part[(size_t)blockIdx.x * g.N + col] = t;
+}
+
+__global__ void __launch_bounds__(256) group_db_sum_kernel(GroupWgArgs g, const float* part) {
+  const int e = blockIdx.y, col = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63;
+  int before = 0, lo, hi;
+  for (int i = lane; i < e; i += 64) {
+    group_rows(g.offs, i, g.S, lo, hi);
+    before += (hi - lo + GW_DBROWS - 1) / GW_DBROWS;
+  }
+  for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+  group_rows(g.offs, e, g.S, lo, hi);
+  const int n = (hi - lo + GW_DBROWS - 1) / GW_DBROWS;
+  if (col >= g.N) return;
+  float t = 0.f;
+  for (int q = 0; q < n; ++q) t += part[(size_t)(before + q) * g.N + col];
+  g.db[(size_t)e * g.N + col] = t;
 }
 
 // Where the large tile is taken, and its workgroups (one per CU: 128 KB of LDS each): operands with 16-byte
@@ -1056,7 +1035,7 @@ static bool wgrad_big(const GroupWgArgs& g) {
   if (g.K % (x8 ? 16 : 8) || g.ldx % (x8 ? 16 : 8)) return false;
   if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25) return false;      // (32-bit offsets within 64 rows)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
-  return tiles * (g.S / GP_K) >= (long)GW_WGS * GP_MIN_UNITS;
+  return tiles * (g.S / GW_UNIT) >= (long)GW_WGS * GP_MIN_UNITS;
 }
 
 // Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
@@ -1072,7 +1051,7 @@ static int wgrad_splits(int S, int N, int K, int E) {
 }
 
 HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
-  if (wgrad_big(*gp)) return 2l * GW_WGS * GW_SLAB;
+  if (wgrad_big(*gp)) return 2l * GW_WGS * GW_SLAB + (gp->db ? (long)(gp->S / GW_DBROWS + gp->E) * gp->N : 0);
   const int ns = wgrad_splits(gp->S, gp->N, gp->K, gp->E);
   return ns > 1 ? (long)ns * gp->E * gp->N * (gp->K + 1) : 0;
 }
@@ -1086,11 +1065,17 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
     if (!g.ws || (uintptr_t)g.ws % 16 || g.E > 65535) return (int)hipErrorInvalidValue;
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
     const dim3 grid(GW_WGS), blk(GP_THREADS);
-    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_pp_kernel<true, true>), grid, blk, 0, st, g, tn, tk, ovec);
-    else if (g.xs) hipLaunchKernelGGL((group_wgrad_pp_kernel<true, false>), grid, blk, 0, st, g, tn, tk, ovec);
-    else if (g.src) hipLaunchKernelGGL((group_wgrad_pp_kernel<false, true>), grid, blk, 0, st, g, tn, tk, ovec);
-    else hipLaunchKernelGGL((group_wgrad_pp_kernel<false, false>), grid, blk, 0, st, g, tn, tk, ovec);
+    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, ovec);
+    else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk, ovec);
+    else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk, ovec);
+    else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, ovec);
     hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 4), dim3(256), 0, st, g, tn, tk, GW_WGS, ovec);
+    if (g.db) {
+      float* part = g.ws + 2l * GW_WGS * GW_SLAB;
+      const int nc = (g.N + 255) / 256;
+      hipLaunchKernelGGL(group_db_part_kernel, dim3(g.S / GW_DBROWS + g.E, nc), dim3(256), 0, st, g, part);
+      hipLaunchKernelGGL(group_db_sum_kernel, dim3(nc, g.E), dim3(256), 0, st, g, part);
+    }
     HFM_LAUNCH_CHECK();
   }
   g.ns = wgrad_splits(g.S, g.N, g.K, g.E);
