@@ -225,50 +225,6 @@ __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_
   }
 }
 
-// 8 neighbouring outputs of row p from column n: mask, rounding, store (vec: 16-byte aligned rows of
-// the output and the mask, N a multiple of 8)
-__device__ __forceinline__ void group_store8(const GroupNtArgs& g, int p, int n, const float (&v)[8], int vec) {
-  const size_t o = (size_t)p * g.ldo + n, m = (size_t)p * g.ldm + n;
-  if (vec) {
-    float w[8];
-    if (g.mask && g.mask8) {
-      const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(g.mask) + m);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = a8_positive(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFFu) ? v[j] : 0.f;
-    } else if (g.mask) {
-      const bf16x8 h = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const bf16*>(g.mask) + m);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = bf2f(h[j]) > 0.f ? v[j] : 0.f;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[j];
-    }
-    if (g.out_f32) {
-      float* d = reinterpret_cast<float*>(g.out) + o;
-      *reinterpret_cast<f32x4*>(d) = f32x4{w[0], w[1], w[2], w[3]};
-      *reinterpret_cast<f32x4*>(d + 4) = f32x4{w[4], w[5], w[6], w[7]};
-    } else {
-      bf16x8 d;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = f2bf(w[j]);
-      *reinterpret_cast<bf16x8*>(reinterpret_cast<bf16*>(g.out) + o) = d;
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (n + j >= g.N) break;
-    float w = v[j];
-    if (g.mask) {
-      const bool on = g.mask8 ? a8_positive(reinterpret_cast<const uint8_t*>(g.mask)[m + j])
-                              : bf2f(reinterpret_cast<const bf16*>(g.mask)[m + j]) > 0.f;
-      if (!on) w = 0.f;
-    }
-    if (g.out_f32) reinterpret_cast<float*>(g.out)[o + j] = w;
-    else reinterpret_cast<bf16*>(g.out)[o + j] = f2bf(w);
-  }
-}
-
 // ------------------------------------------------------------------ 256 x 256 products
 // 256 threads = 4 waves, one per SIMD, of 128 x 128 outputs (4 x 4 MFMA 32x32x16 tiles: 256
 // accumulators; 32 cycles an MFMA leave room for the other instructions of the one wave).  The reduction runs in 32-deep steps through a ring of 4 LDS buffers (A 16 KB + B 16 KB
@@ -362,40 +318,89 @@ __device__ __forceinline__ void band_tile(int t, int rows, int cols, int& r, int
   c = i / h;
 }
 
-// A wave's 128 x 128 outputs leave through its 32 KB of LDS, 64 rows a pass, so that a lane holds 8
-// neighbouring columns of a row: emit(row in the block, first column in the block, 8 values).
-template <typename F>
-__device__ __forceinline__ void mm_emit(const f32x16 (&acc)[4][4], char* img, int lane, F emit) {
-  // (the lane hidden from the optimizer: in a loop over tiles it would otherwise keep the image's
-  // addresses in registers through the product, which has none left)
-  asm volatile("" : "+v"(lane));
-  const int fr = lane & 31, fq = lane >> 5;
-  auto wsync = [] {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-  // rows of 128 floats; 16-byte chunk c of row r at chunk c ^ (r & 15)
-  auto off = [](int r, int c) { return r * 512 + ((((c >> 2) ^ (r & 15))) << 4) + (c & 3) * 4; };
+// A wave's 128 x 128 fp32 outputs, straight from the accumulators (a lane holds rows 8 (q >> 2) + 4 (lane >> 5)
+// + (q & 3) of column lane & 31 of a 32 x 32 tile: a store is two rows' 128 B): rows past `rows` and columns
+// past `cols` are dropped by the buffer's end.  One wave per SIMD issues an instruction every 4 cycles,
+// so the way through LDS to 16-byte stores cost more (9 us a tile of 256 x 256) than it saved.
+constexpr uint32_t GP_FAR = 0x80000000u;                 // an offset past every buffer here
+constexpr long GP_MAXLD = 1l << 21;                      // (128 rows of fp32 within 2^30 bytes)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t out_rows(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+__device__ __forceinline__ void mm_out_f32(const f32x16 (&acc)[4][4], float* base, int rows, int cols, int ld, int lane) {
+  if (rows <= 0) return;
+  const __amdgpu_buffer_rsrc_t o = out_rows(base, (uint32_t)min(rows, 128) * ld * 4u);
+  const int fr = lane & 31, h = lane >> 5;
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int j = 0; j < 4; ++j) {
+    const int c = j * 32 + fr;
+    const uint32_t at = c < cols ? (uint32_t)(h * 4 * ld + c) * 4u : GP_FAR;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int q = 0; q < 16; ++q)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[i][j][q]), o, (int)at,
+                                              (i * 32 + (q >> 2) * 8 + (q & 3)) * ld * 4, 0);
+  }
+}
+
+// The NT kernel's outputs: max(acc * scale + bias, floor) (floor 0: relu, -inf: none; NaN stays), masked,
+// in fp32 as above, or in bf16 two columns a lane: the lanes of a column pair trade a row each
+// (pack two rows, one lane swap, one byte permute), so that a store is four rows' 64 B.
+// MASK 1: bf16 layer input, 2: its 8-bit codes; where that is not above zero the output is.
+template <int MASK, bool F32>
+__device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&acc)[4][4], int e, int row0, int rows, int n0,
+                                          int lane) {
+  if (rows <= 0) return;
+  constexpr int ES = F32 ? 4 : 2, MS = MASK == 1 ? 2 : 1;
+  const int fr = lane & 31, h = lane >> 5, odd = lane & 1;
+  const int ldo = (int)g.ldo, ldm = (int)g.ldm, left = min(rows, 128);
+  const __amdgpu_buffer_rsrc_t o = out_rows(reinterpret_cast<char*>(g.out) + (size_t)row0 * g.ldo * ES, (uint32_t)left * ldo * ES);
+  const __amdgpu_buffer_rsrc_t mr =
+      out_rows(reinterpret_cast<const char*>(g.mask) + (size_t)row0 * g.ldm * MS, (uint32_t)left * ldm * MS);
+  const float lo = g.relu ? 0.f : -INFINITY;
+  const uint32_t sel = odd ? 0x07060302u : 0x01000504u;
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          *reinterpret_cast<float*>(img + off(i * 32 + (q >> 2) * 8 + fq * 4 + (q & 3), j * 32 + fr)) = acc[p * 2 + i][j][q];
-    wsync();
-#pragma unroll 2
-    for (int it = 0; it < 16; ++it) {
-      const int r = it * 4 + (lane >> 4), c = (lane & 15) * 8;
-      const f32x4 a = *reinterpret_cast<const f32x4*>(img + off(r, c));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(img + off(r, c + 4));
-      const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      emit(p * 64 + r, c, v);
+  for (int j = 0; j < 4; ++j) {
+    const int c = n0 + j * 32 + fr;
+    const float bias = g.bias && c < g.N ? g.bias[(size_t)e * g.N + c] : 0.f;
+    const int cc = F32 ? c : c & ~1, rr = F32 ? h * 4 : h * 4 + odd;
+    const uint32_t at = cc < g.N ? (uint32_t)(rr * ldo + cc) * ES : GP_FAR;
+    const uint32_t mt = cc < g.N ? (uint32_t)(rr * ldm + cc) * MS : GP_FAR;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      constexpr int NQ = F32 ? 16 : 8;
+      uint32_t m[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int k = F32 ? q : 2 * q, row = i * 32 + (k >> 2) * 8 + (k & 3);
+        if (MASK == 1) m[q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, (int)mt, row * ldm * MS, 0)
+                                  : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(mr, (int)mt, row * ldm * MS, 0);
+        if (MASK == 2) m[q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(mr, (int)mt, row * ldm * MS, 0)
+                                  : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, (int)mt, row * ldm * MS, 0);
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int k = F32 ? q : 2 * q, row = i * 32 + (k >> 2) * 8 + (k & 3);
+        float v = __builtin_elementwise_maximum(fmaf(acc[i][j][k], g.scale, bias), lo);
+        uint32_t w;
+        if (F32) {
+          if (MASK == 1 && !(__uint_as_float(m[q] << 16) > 0.f)) v = 0.f;
+          if (MASK == 2 && !a8_positive(m[q])) v = 0.f;
+          w = __float_as_uint(v);
+        } else {
+          typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+          const float u = __builtin_elementwise_maximum(fmaf(acc[i][j][k + 1], g.scale, bias), lo);
+          const uint32_t p = __builtin_bit_cast(uint32_t, bf16x2{f2bf(v), f2bf(u)});
+          const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)p, 0xB1, 0xF, 0xF, true);     // lane ^ 1
+          w = __builtin_amdgcn_perm(p, t, sel);
+          if (MASK == 1) w = (__uint_as_float(m[q] << 16) > 0.f ? w & 0xFFFFu : 0u) |
+                             (__uint_as_float(m[q] & 0xFFFF0000u) > 0.f ? w & 0xFFFF0000u : 0u);
+          if (MASK == 2) w = (a8_positive(m[q] & 0xFFu) ? w & 0xFFFFu : 0u) | (a8_positive(m[q] >> 8) ? w & 0xFFFF0000u : 0u);
+        }
+        __builtin_amdgcn_raw_buffer_store_b32(w, o, (int)at, row * ldo * ES, 0);
+      }
     }
-    wsync();
   }
 }
 
@@ -403,7 +408,7 @@ __device__ __forceinline__ void mm_emit(const f32x16 (&acc)[4][4], char* img, in
 // lies at c ^ ((r >> 2) & 3): the 16 rows of a fragment read meet in 16 different chunks of 256 B.  K a
 // multiple of 8; the last step's chunks past K come from the zero source.
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
-group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int ovec) {
+group_nt_mm_kernel(GroupNtArgs g, int tiles_n) {
   __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
   // (the grid has room for one more row tile per group: the tiles that there are go round the XCDs)
   const int tiles_m = group_tiles<GP_B>(g.offs, g.E, g.S);
@@ -447,24 +452,17 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int ovec) {
       [&](int i, const char* b) { return *reinterpret_cast<const bf16x8*>(b + la + (i < 4 ? f0 : f1) + (i & 3) * 32 * 64); },
       [&](int j, const char* b) { return *reinterpret_cast<const bf16x8*>(b + lb + (j < 4 ? f0 : f1) + (j & 3) * 32 * 64); },
       [](auto, int) {});
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int n = n0 + wc * 128 + j * 32 + fr;
-    const float bias = g.bias && n < g.N ? g.bias[(size_t)e * g.N + n] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        float v = acc[i][j][q] * g.scale + bias;
-        if (g.relu && v < 0.f) v = 0.f;
-        acc[i][j][q] = v;
-      }
+  const int row0 = r0 + wr * 128, n1 = n0 + wc * 128;
+  if (!g.mask) {
+    if (g.out_f32) mm_out_nt<0, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<0, false>(g, acc, e, row0, r1 - row0, n1, lane);
+  } else if (!g.mask8) {
+    if (g.out_f32) mm_out_nt<1, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<1, false>(g, acc, e, row0, r1 - row0, n1, lane);
+  } else {
+    if (g.out_f32) mm_out_nt<2, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<2, false>(g, acc, e, row0, r1 - row0, n1, lane);
   }
-  mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
-    const int p = r0 + wr * 128 + r, n = n0 + wc * 128 + c;
-    if (p < r1 && n < g.N) group_store8(g, p, n, v, ovec);
-  });
 }
 
 HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
@@ -473,13 +471,14 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   if (g.S == 0 || g.N == 0) return 0;
   const bool vec = ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.K % 8 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0 &&
                    g.es % 8 == 0;
-  const bool ovec = g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0 &&
-                    (!g.mask || (g.ldm % 8 == 0 && (uintptr_t)g.mask % (g.mask8 ? 8 : 16) == 0));
-  if (vec && g.K >= 64) {
+  // the large tile stores (and reads the mask) in column pairs of bf16
+  const bool pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && g.ldm % 2 == 0 && (uintptr_t)g.out % 4 == 0 &&
+                     (uintptr_t)g.mask % (g.mask8 ? 2 : 4) == 0 && g.ldo < GP_MAXLD && g.ldm < GP_MAXLD;
+  if (vec && pairs && g.K >= 64) {
     const int tn = (g.N + GP_B - 1) / GP_B;
     const long blocks = (long)(g.S / GP_B + g.E) * tn;
     if (blocks >= GP_MIN_TILES && blocks <= 0x7FFFFFFFl) {
-      hipLaunchKernelGGL(group_nt_mm_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn, ovec ? 1 : 0);
+      hipLaunchKernelGGL(group_nt_mm_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
       HFM_LAUNCH_CHECK();
     }
   }
@@ -737,7 +736,7 @@ __device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32
 
 template <bool X8, bool GATHER>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
-group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int ovec) {
+group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
   __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave >> 1, wc = wave & 1;
@@ -904,35 +903,15 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int ovec) {
             load_a, load_b, [&](auto, int) { hide(); });
       }
     }
-    __syncthreads();
+    __syncthreads();                      // (the next part's staging overwrites what was read here)
     // a whole tile goes to dw, a part to the workspace: slot 2 w if it is the workgroup's first, 2 w + 1
     // if it goes on in the next one
-    const bool whole = s0 == 0 && s1 == steps;
-    if (whole) {
-      float* dw = g.dw + (size_t)e * g.N * g.K;
-      mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
-        const int n = n0 + wr * 128 + r, k = k0 + wc * 128 + c;
-        if (n >= g.N || k >= g.K) return;
-        float* d = dw + (size_t)n * g.K + k;
-        if (ovec) {
-          *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
-          *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (k + j < g.K) d[j] = v[j];
-        }
-      });
-    } else {
-      float* slab = g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB;
-      mm_emit(acc, smem + wave * 32768, lane, [&](int r, int c, const float (&v)[8]) {
-        float* d = slab + (wr * 128 + r) * GP_B + wc * 128 + c;
-        *reinterpret_cast<f32x4*>(d) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(d + 4) = f32x4{v[4], v[5], v[6], v[7]};
-      });
-    }
+    if (s0 == 0 && s1 == steps)
+      mm_out_f32(acc, g.dw + ((size_t)e * g.N + n0 + wr * 128) * g.K + k0 + wc * 128, g.N - n0 - wr * 128,
+                 g.K - k0 - wc * 128, g.K, lane);
+    else
+      mm_out_f32(acc, g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB + wr * 128 * GP_B + wc * 128, 128, 128, GP_B, lane);
     u += s1 - s0;
-    __syncthreads();                      // (the next tile's staging reuses the images)
   }
 }
 
@@ -1033,7 +1012,7 @@ static bool wgrad_big(const GroupWgArgs& g) {
   const bool x8 = g.xs != nullptr;
   if ((uintptr_t)g.dz % 16 || (uintptr_t)g.x % 16 || g.N % 8 || g.ldz % 8) return false;
   if (g.K % (x8 ? 16 : 8) || g.ldx % (x8 ? 16 : 8)) return false;
-  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25) return false;      // (32-bit offsets within 64 rows)
+  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD) return false;      // (32-bit offsets)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
   return tiles * (g.S / GW_UNIT) >= (long)GW_WGS * GP_MIN_UNITS;
 }
@@ -1065,10 +1044,10 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
     if (!g.ws || (uintptr_t)g.ws % 16 || g.E > 65535) return (int)hipErrorInvalidValue;
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
     const dim3 grid(GW_WGS), blk(GP_THREADS);
-    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, ovec);
-    else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk, ovec);
-    else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk, ovec);
-    else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, ovec);
+    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk);
+    else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk);
+    else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk);
+    else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk);
     hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 4), dim3(256), 0, st, g, tn, tk, GW_WGS, ovec);
     if (g.db) {
       float* part = g.ws + 2l * GW_WGS * GW_SLAB;
