@@ -656,54 +656,52 @@ __global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
 // 8-bit x: 32 codes a thread (one scale) are loaded two steps ahead, turned into bf16 times the
 // scale (one conversion per pair, exact) and written into the same image.
 //
-// The work is cut evenly, not by tiles: `units` = 64-row blocks of all tiles (a group without rows counts
-// one per tile, which writes its zeros), tiles in expert order, and workgroup w takes the units from
-// w U / W to (w + 1) U / W.  A tile within one workgroup goes straight to dw; a workgroup's first and last tile
-// may be parts, which go to its two workspace tiles and are summed in row order by a second launch.
-// Groups of any sizes thus load the CUs evenly (by whole tiles the fullest of 16 groups set the
-// time), for at most 512 tiles of 256 KB.
+// The rows are cut evenly, not by groups: all groups' rows in a line (in units of 64, and GW_SEG more for
+// each group, which is what its prologue and outputs cost) are cut into `lanes` equal parts, and
+// workgroup (lane, tile) sums its tile over its lane, group after group.  The tiles of a lane are
+// neighbours: they run side by side on an XCD and read the same rows at the same time (cut tile by
+// tile, every workgroup at its own rows, the panels came from beyond the L2: 150 us for 16 groups of
+// 2048 rows x 1024 x 1024 against 71 us for one of as many steps).  A group within one lane goes straight
+// to dw; what a lane boundary cuts goes to the workspace, two tiles per workgroup at most, and is
+// summed in row order by a second launch.
 constexpr int GW_UNIT = 64;                      // rows of a unit
 constexpr int GW_SLAB = GP_B * GP_B;             // floats of a workspace tile
 
-struct WgCut {
-  long u0, u1;             // the workgroup's units
-};
-__device__ __forceinline__ WgCut wg_cut(long U, int W, int w) { return {U * w / W, U * (w + 1) / W}; }
-__device__ __forceinline__ int wg_owner(long U, int W, long u) {        // the workgroup of unit u
-  int w = (int)((u * W) / U);
-  while (U * (w + 1) / W <= u) ++w;
-  while (w > 0 && U * w / W > u) --w;
-  return w;
+constexpr int GW_SEG = 6;                        // a group's own units (10 us against 1.7 us a unit)
+
+// Unit u of the line belongs to lane l with U l / L <= u < U (l + 1) / L.
+__device__ __forceinline__ int wg_cut(int U, int L, int l) { return (int)((long)U * l / L); }
+__device__ __forceinline__ int wg_owner(int U, int L, int u) {
+  int l = (int)((long)u * L / U);
+  while (wg_cut(U, L, l + 1) <= u) ++l;
+  while (l > 0 && wg_cut(U, L, l) > u) --l;
+  return l;
 }
+// 64-row steps of a group (one for an empty group: the lane that has it writes the zeros)
 __device__ __forceinline__ int wg_steps(const int* offs, int e, int S) {
   int lo, hi;
   group_rows(offs, e, S, lo, hi);
   return max(1, (hi - lo + GW_UNIT - 1) / GW_UNIT);
 }
-// a value that is the same in all lanes, into scalar registers
-__device__ __forceinline__ long uni64(long v) {
-  return (long)(((unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-                (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
-// units of all groups, by every wave for itself
-__device__ __forceinline__ long wg_units(const int* offs, int E, int S, int tiles) {
+// units of the groups below `upto`, by every wave for itself
+__device__ __forceinline__ int wg_units(const int* offs, int upto, int S) {
   const int lane = threadIdx.x & 63;
-  long n = 0;
-  for (int e = lane; e < E; e += 64) n += wg_steps(offs, e, S);
+  int n = 0;
+  for (int e = lane; e < upto; e += 64) n += wg_steps(offs, e, S) + GW_SEG;
   for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-  return uni64(n) * tiles;
+  return __builtin_amdgcn_readfirstlane(n);
 }
-// the expert of unit u, and its first unit
-__device__ __forceinline__ void wg_find(const int* offs, int E, int S, int tiles, long u, int& e, long& first) {
+// the group of unit u, and its first unit
+__device__ __forceinline__ void wg_find(const int* offs, int E, int S, int u, int& e, int& first) {
   const int lane = threadIdx.x & 63;
-  long run = 0;
+  int run = 0;
   e = 0;
   first = 0;
   for (int e0 = 0; e0 < E; e0 += 64) {
-    const long n = e0 + lane < E ? (long)wg_steps(offs, e0 + lane, S) * tiles : 0;
-    long inc = n;
+    const int n = e0 + lane < E ? wg_steps(offs, e0 + lane, S) + GW_SEG : 0;
+    int inc = n;
     for (int d = 1; d < 64; d <<= 1) {
-      const long v = __shfl_up(inc, d);
+      const int v = __shfl_up(inc, d);
       if (lane >= d) inc += v;
     }
     const unsigned long long past = __ballot(run + inc > u);
@@ -716,7 +714,7 @@ __device__ __forceinline__ void wg_find(const int* offs, int E, int S, int tiles
     run += __shfl(inc, 63);
   }
   e = __builtin_amdgcn_readfirstlane(e);
-  first = uni64(first);
+  first = __builtin_amdgcn_readfirstlane(first);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -736,16 +734,18 @@ __device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32
 
 template <bool X8, bool GATHER>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
-group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
+group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave >> 1, wc = wave & 1;
   const int tiles = tiles_n * tiles_k;
   const int w = xcd_order(blockIdx.x, gridDim.x);
-  const WgCut cut = wg_cut(wg_units(g.offs, g.E, g.S, tiles), gridDim.x, w);
-  int e;
-  long first;
-  wg_find(g.offs, g.E, g.S, tiles, cut.u0, e, first);
+  const int U = wg_units(g.offs, g.E, g.S), u0 = wg_cut(U, lanes, w / tiles), u1 = wg_cut(U, lanes, w / tiles + 1);
+  int tn, tk;
+  band_tile(w % tiles, tiles_n, tiles_k, tn, tk);
+  const int n0 = tn * GP_B, k0 = tk * GP_B;
+  int e, first;
+  wg_find(g.offs, g.E, g.S, u0, e, first);
   // fragment (half h, columns 32 i ..): the lane's 16-lane group takes rows 16 h + 8 (lane >> 5) .. and
   // columns 32 i + (lane & 16) ..: granule (2 i + (lane >> 4 & 1)) ^ f(row), which is an xor with 2 i
   const int l4 = (lane >> 2) & 3, h5 = lane >> 5;
@@ -761,21 +761,13 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
   const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32;
   const int xf = (xr & 3) | ((xr >> 1) & 4);
   const int xo = GP_PANEL + xr * 512 + (((2 * xq) ^ xf) << 5);        // (granule 2 q + 1: ^ 32)
-  long u = cut.u0;
-  while (u < cut.u1) {
-    int steps = wg_steps(g.offs, e, g.S);
-    while (u >= first + (long)steps * tiles) {      // the next group
-      first += (long)steps * tiles;
-      ++e;
-      steps = wg_steps(g.offs, e, g.S);
-    }
+  for (; e < g.E && first < u1; ++e) {
+    const int steps = wg_steps(g.offs, e, g.S), rows0 = first + GW_SEG;      // (the group's rows begin here)
+    first = rows0 + steps;
+    const int s0 = max(0, u0 - rows0), s1 = min(steps, u1 - rows0);
+    if (s0 >= s1) continue;
     int lo, hi_row;
     group_rows(g.offs, e, g.S, lo, hi_row);
-    const int ti = (int)((u - first) / steps), s0 = (int)((u - first) % steps);
-    const int s1 = (int)min((long)steps, s0 + (cut.u1 - u));
-    int tn, tk;
-    band_tile(ti, tiles_n, tiles_k, tn, tk);
-    const int n0 = tn * GP_B, k0 = tk * GP_B;
     // (scalar for certain: the buffers below are made of them)
     const int p0 = __builtin_amdgcn_readfirstlane(lo + s0 * GW_UNIT);
     const int p1 = __builtin_amdgcn_readfirstlane(min(hi_row, lo + s1 * GW_UNIT));
@@ -911,54 +903,50 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
                  g.K - k0 - wc * 128, g.K, lane);
     else
       mm_out_f32(acc, g.ws + (size_t)(2 * w + (s0 > 0 ? 0 : 1)) * GW_SLAB + wr * 128 * GP_B + wc * 128, 128, 128, GP_B, lane);
-    u += s1 - s0;
   }
 }
 
-// Tiles that two or more workgroups made: their parts in row order.  grid (tiles of an expert, E, 4
-// quarters); the same cut as the product's.
-__global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int W, int ovec) {
+// Groups that two or more lanes made: their parts in row order.  grid (tiles, E, 16 strips of 16 rows).
+__global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes, int ovec) {
   const int tiles = tiles_n * tiles_k, ti = blockIdx.x, e = blockIdx.y;
-  const int lane = threadIdx.x & 63;
-  long before = 0, n = 0;
-  for (int i = lane; i < g.E; i += 64) {
-    const int s = wg_steps(g.offs, i, g.S);
-    n += s;
-    if (i < e) before += s;
-  }
-  for (int d = 32; d; d >>= 1) {
-    n += __shfl_xor(n, d);
-    before += __shfl_xor(before, d);
-  }
-  const long U = n * tiles;
-  const int steps = wg_steps(g.offs, e, g.S);
-  const long a = before * tiles + (long)ti * steps, b = a + steps - 1;
-  const int w0 = wg_owner(U, W, a), w1 = wg_owner(U, W, b);
-  if (w0 == w1) return;
+  const int U = wg_units(g.offs, g.E, g.S), rows0 = wg_units(g.offs, e, g.S) + GW_SEG, steps = wg_steps(g.offs, e, g.S);
+  const int l0 = wg_owner(U, lanes, rows0), l1 = wg_owner(U, lanes, rows0 + steps - 1);
+  if (l0 == l1) return;
   int tn, tk;
   band_tile(ti, tiles_n, tiles_k, tn, tk);
   const int n0 = tn * GP_B, k0 = tk * GP_B;
-  // the part that starts the tile is the last of w0 (slot 1), the others are the first of theirs
-  auto slab = [&](int w) { return g.ws + (size_t)(2 * w + (w == w0 ? 1 : 0)) * GW_SLAB; };
-  const int row0 = blockIdx.z * 64;
-  for (int i = threadIdx.x; i < 64 * (GP_B / 4); i += 256) {
-    const int r = row0 + i / (GP_B / 4), c = (i % (GP_B / 4)) * 4;
+  // the lane that starts the group left it in its second tile, the others in their first
+  const float* s0 = g.ws + (size_t)(2 * (l0 * tiles + ti) + 1) * GW_SLAB;
+  const float* s1 = g.ws + (size_t)(2 * ((l0 + 1) * tiles + ti)) * GW_SLAB;
+  const size_t next = (size_t)2 * tiles * GW_SLAB;
+  const int r0 = blockIdx.z * 16 + (threadIdx.x >> 6), c = (threadIdx.x & 63) * 4;
+  f32x4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4*>(s0 + (r0 + 4 * i) * GP_B + c);
+  for (int l = l0 + 1; l <= l1; ++l, s1 += next) {
+    f32x4 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const f32x4*>(s1 + (r0 + 4 * i) * GP_B + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += a[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + 4 * i;
     if (n0 + r >= g.N || k0 + c >= g.K) continue;
-    f32x4 v = *reinterpret_cast<const f32x4*>(slab(w0) + r * GP_B + c);
-    for (int q = w0 + 1; q <= w1; ++q) v += *reinterpret_cast<const f32x4*>(slab(q) + r * GP_B + c);
     float* d = g.dw + ((size_t)e * g.N + n0 + r) * g.K + k0 + c;
     if (ovec) {
-      *reinterpret_cast<f32x4*>(d) = v;
+      *reinterpret_cast<f32x4*>(d) = v[i];
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (k0 + c + j < g.K) d[j] = v[j];
+        if (k0 + c + j < g.K) d[j] = v[i][j];
     }
   }
 }
 
 // db of the large tile's path: column sums of dz, chunks of GW_DBROWS rows of a group (256 columns: 32
-// lanes of 8 columns, 8 rows at a time), then the group's chunks in order.  Beside the product rather
+// lanes of 8 columns, 8 rows at a time), then the group's chunks, 8 threads a column, in a fixed order.  Beside the product rather
 // than in it: a ninth fragment column there costs its loop registers or a branch.
 constexpr int GW_DBROWS = 256;
 __global__ void __launch_bounds__(256) group_db_part_kernel(GroupWgArgs g, float* part) {
@@ -989,7 +977,8 @@ __global__ void __launch_bounds__(256) group_db_part_kernel(GroupWgArgs g, float
 }
 
 __global__ void __launch_bounds__(256) group_db_sum_kernel(GroupWgArgs g, const float* part) {
-  const int e = blockIdx.y, col = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63;
+  __shared__ float red[8][32];
+  const int e = blockIdx.y, c = threadIdx.x & 31, q0 = threadIdx.x >> 5, col = blockIdx.x * 32 + c, lane = threadIdx.x & 63;
   int before = 0, lo, hi;
   for (int i = lane; i < e; i += 64) {
     group_rows(g.offs, i, g.S, lo, hi);
@@ -997,24 +986,53 @@ __global__ void __launch_bounds__(256) group_db_sum_kernel(GroupWgArgs g, const 
   }
   for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
   group_rows(g.offs, e, g.S, lo, hi);
-  const int n = (hi - lo + GW_DBROWS - 1) / GW_DBROWS;
-  if (col >= g.N) return;
+  // (offsets out of order could make more chunks than there is room for)
+  const int n = min((hi - lo + GW_DBROWS - 1) / GW_DBROWS, g.S / GW_DBROWS + g.E - before);
   float t = 0.f;
-  for (int q = 0; q < n; ++q) t += part[(size_t)(before + q) * g.N + col];
-  g.db[(size_t)e * g.N + col] = t;
+  if (col < g.N) {
+#pragma unroll 4
+    for (int q = q0; q < n; q += 8) t += part[(size_t)(before + q) * g.N + col];
+  }
+  red[q0][c] = t;
+  __syncthreads();
+  if (q0 == 0 && col < g.N) {
+#pragma unroll
+    for (int q = 1; q < 8; ++q) t += red[q][c];
+    g.db[(size_t)e * g.N + col] = t;
+  }
 }
 
-// Where the large tile is taken, and its workgroups (one per CU: 128 KB of LDS each): operands with 16-byte
-// rows, and enough work for every CU (GP_MIN_UNITS steps each; below that the 128 x 128 tile's smaller
-// pieces fill the chip better).
-constexpr int GW_WGS = 256, GP_MIN_UNITS = 2;
+// Where the large tile is taken: operands with 16-byte rows, and enough work for every CU (GP_MIN_UNITS
+// steps of 64 rows each; below that the 128 x 128 tile's smaller pieces fill the chip better).
+constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
 static bool wgrad_big(const GroupWgArgs& g) {
   const bool x8 = g.xs != nullptr;
   if ((uintptr_t)g.dz % 16 || (uintptr_t)g.x % 16 || g.N % 8 || g.ldz % 8) return false;
   if (g.K % (x8 ? 16 : 8) || g.ldx % (x8 ? 16 : 8)) return false;
-  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD) return false;      // (32-bit offsets)
+  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD || g.E > 65535) return false;      // (32-bit offsets; grid)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
-  return tiles * (g.S / GW_UNIT) >= (long)GW_WGS * GP_MIN_UNITS;
+  return tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS;
+}
+// Lanes: the fewest rounds of the CUs times a lane's length (its rows, and one group's own cost), within
+// 512 workgroups (a workspace of 256 MB) unless the tiles alone are more.
+static int wgrad_lanes(const GroupWgArgs& g) {
+  const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
+  const double units = (double)(g.S / GW_UNIT) + (double)g.E * (1 + GW_SEG);
+  int best = 1;
+  double least = 0.0;
+  for (int l = 1; l == 1 || l * tiles <= 512; ++l) {
+    const double t = (double)((l * tiles + GW_CUS - 1) / GW_CUS) * (units / l + GW_SEG);
+    if (l == 1 || t < least) {
+      least = t;
+      best = l;
+    }
+  }
+  return best;
+}
+// Slabs, then the parts of db.  A single lane cuts no group.
+static long wgrad_slab_floats(const GroupWgArgs& g) {
+  const int l = wgrad_lanes(g);
+  return l == 1 ? 0 : 2l * l * ((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B) * GW_SLAB;
 }
 
 // Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
@@ -1030,7 +1048,7 @@ static int wgrad_splits(int S, int N, int K, int E) {
 }
 
 HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
-  if (wgrad_big(*gp)) return 2l * GW_WGS * GW_SLAB + (gp->db ? (long)(gp->S / GW_DBROWS + gp->E) * gp->N : 0);
+  if (wgrad_big(*gp)) return wgrad_slab_floats(*gp) + (gp->db ? (long)(gp->S / GW_DBROWS + gp->E) * gp->N : 0);
   const int ns = wgrad_splits(gp->S, gp->N, gp->K, gp->E);
   return ns > 1 ? (long)ns * gp->E * gp->N * (gp->K + 1) : 0;
 }
@@ -1041,19 +1059,20 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   if (g.N == 0) return 0;
   if (wgrad_big(g)) {
     const int tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
-    if (!g.ws || (uintptr_t)g.ws % 16 || g.E > 65535) return (int)hipErrorInvalidValue;
+    const int lanes = wgrad_lanes(g);
+    if ((lanes > 1 || g.db) && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
-    const dim3 grid(GW_WGS), blk(GP_THREADS);
-    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk);
-    else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk);
-    else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk);
-    else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk);
-    hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 4), dim3(256), 0, st, g, tn, tk, GW_WGS, ovec);
+    const dim3 grid((unsigned)(tn * tk * lanes)), blk(GP_THREADS);
+    if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, lanes);
+    else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk, lanes);
+    else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk, lanes);
+    else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, lanes);
+    if (lanes > 1)
+      hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 16), dim3(256), 0, st, g, tn, tk, lanes, ovec);
     if (g.db) {
-      float* part = g.ws + 2l * GW_WGS * GW_SLAB;
-      const int nc = (g.N + 255) / 256;
-      hipLaunchKernelGGL(group_db_part_kernel, dim3(g.S / GW_DBROWS + g.E, nc), dim3(256), 0, st, g, part);
-      hipLaunchKernelGGL(group_db_sum_kernel, dim3(nc, g.E), dim3(256), 0, st, g, part);
+      float* part = g.ws + wgrad_slab_floats(g);
+      hipLaunchKernelGGL(group_db_part_kernel, dim3(g.S / GW_DBROWS + g.E, (g.N + 255) / 256), dim3(256), 0, st, g, part);
+      hipLaunchKernelGGL(group_db_sum_kernel, dim3((g.N + 31) / 32, g.E), dim3(256), 0, st, g, part);
     }
     HFM_LAUNCH_CHECK();
   }

@@ -295,7 +295,7 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
         lib = _lib.get_lib()
         a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), 0,
                         row_stride(dz), row_stride(xv), S, xv.shape[0], K, N, E, top_k, 1)
-        n = lib.hfm_group_wgrad_ws_floats(C.byref(a))
+        n = lib.hfm_group_wgrad_ws_floats(C.byref(a))      # split products and column sums
         ws = torch.empty(n, dtype=torch.float32, device=dz.device) if n else None
         a.ws = ptr(ws)
         check(lib.hfm_group_wgrad(C.byref(a), st), "group_wgrad")
