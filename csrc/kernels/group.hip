@@ -12,6 +12,8 @@
 //
 // A workgroup finds its expert by a scan over the group sizes in its own registers.  Accumulation is
 // fp32 on MFMA; nothing is summed by atomics.
+#include <math.h>
+
 #include <type_traits>
 
 #include "act8.h"
@@ -254,33 +256,36 @@ __device__ __forceinline__ void dma16_buf(const void* base, uint32_t bytes, uint
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)voff, (int)soff, 0, 0);
 }
 
-// D: DMA pieces of a wave per step.  stage(i, step): piece i (0 .. D - 1) of a step, zeros from the step `ns`
-// on (the loop runs on a pair of steps at a time and three steps ahead, without a branch);
-// load_a(i, buf), load_b(j, buf): fragments; extra(parity, step): what else a step brings (8-bit inputs).
-template <int D, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[4][4], ST stage, LA load_a, LB load_b, EX extra) {
-  bf16x8 fa[8], fb[2][8];
-  auto step = [&](auto PAR, int s) {
-    constexpr int c = decltype(PAR)::value, n = c ^ 1;
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");        // (the DMA of step s + 2 stays in flight)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");          // (no access moves over the barrier)
-    __builtin_amdgcn_sched_barrier(0);
-    extra(PAR, s);
-    const char* nb = smem + ((s + 1) & (GP_RING - 1)) * GP_BUF;
+// One step of a wave.  D: its DMA pieces per step.  stage(i): piece i of the step three ahead; load_a(i),
+// load_b(j): fragments of the next step; PAR: which of the two sets of column fragments is multiplied.
+template <int NI, int D, int PAR, typename ST, typename LA, typename LB, typename EX>
+__device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a,
+                                        LB load_b, EX extra) {
+  constexpr int NA = 2 * NI, c = PAR, n = c ^ 1;      // row fragment r: 16-deep half r / NI, rows 32 (r % NI) ..
+  static_assert(NI >= 3 && NI <= 4 && D <= 2 * NA - 4, "a place for every load");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");        // (the DMA of the step after next stays in flight)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");          // (no access moves over the barrier)
+  __builtin_amdgcn_sched_barrier(0);
+  extra();
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const int r = k >> 2, j = k & 3;      // round r: row fragment r (16-deep half r >> 2, rows 32 (r & 3) ..)
-      acc[r & 3][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[c][(r >> 2) * 4 + j], acc[r & 3][j], 0, 0, 0);
-      // at most one load between two MFMAs: a wave issues an instruction every 4 cycles, an MFMA runs 32
-      if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1, nb);
-      if (j == 1 && r < 4) fb[n][2 * r] = load_b(2 * r, nb);
-      if (j == 2 && r < 4) fb[n][2 * r + 1] = load_b(2 * r + 1, nb);
-      if (j == 3 && r < D) stage(r, s + GP_RING - 1);
-      if (k == 31) fa[7] = load_a(7, nb);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
+  for (int k = 0; k < 4 * NA; ++k) {
+    const int r = k >> 2, j = k & 3;
+    acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[c][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
+    // at most one load between two MFMAs: a wave issues an instruction every 4 cycles, an MFMA runs 32
+    if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1);
+    if (j == 1 && r < 4) fb[n][2 * r] = load_b(2 * r);
+    if (j == 2 && r < 4) fb[n][2 * r + 1] = load_b(2 * r + 1);
+    if (j == 3 && r < D) stage(r);
+    if (j == 1 && r >= 4 && NA + r - 4 < D) stage(NA + r - 4);
+    if (k == 4 * NA - 1) fa[NA - 1] = load_a(NA - 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The first three steps' DMA under way, the first step's fragments in registers.
+template <int NI, int D, typename ST, typename LA, typename LB>
+__device__ __forceinline__ void mm_begin(bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a, LB load_b) {
 #pragma unroll
   for (int s = 0; s < GP_RING - 1; ++s)
 #pragma unroll
@@ -289,10 +294,23 @@ __device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[4][4],
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    fb[0][i] = load_b(i, smem);
-    fa[i] = load_a(i, smem);
-  }
+  for (int i = 0; i < 8; ++i) fb[0][i] = load_b(i);
+#pragma unroll
+  for (int i = 0; i < 2 * NI; ++i) fa[i] = load_a(i);
+}
+
+// A whole reduction of ns steps.  stage(i, step): zeros from the step `ns` on (the loop runs on a pair of steps
+// at a time and three steps ahead, without a branch: its registers do not survive one).
+template <int NI, int D, typename ST, typename LA, typename LB, typename EX>
+__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], ST stage, LA load_a, LB load_b, EX extra) {
+  bf16x8 fa[2 * NI], fb[2][8];
+  mm_begin<NI, D>(fa, fb, stage, [&](int i) { return load_a(i, smem); }, [&](int j) { return load_b(j, smem); });
+  auto step = [&](auto PAR, int s) {
+    const char* nb = smem + ((s + 1) & (GP_RING - 1)) * GP_BUF;
+    mm_step<NI, D, decltype(PAR)::value>(
+        acc, fa, fb, [&](int i) { stage(i, s + GP_RING - 1); }, [&](int i) { return load_a(i, nb); },
+        [&](int j) { return load_b(j, nb); }, [&]() { extra(PAR, s); });
+  };
   for (int s = 0; s < ns; s += 2) {
     step(std::integral_constant<int, 0>{}, s);
     step(std::integral_constant<int, 1>{}, s + 1);
@@ -348,120 +366,222 @@ __device__ __forceinline__ void mm_out_f32(const f32x16 (&acc)[4][4], float* bas
 // in fp32 as above, or in bf16 two columns a lane: the lanes of a column pair trade a row each
 // (pack two rows, one lane swap, one byte permute), so that a store is four rows' 64 B.
 // MASK 1: bf16 layer input, 2: its 8-bit codes; where that is not above zero the output is.
-template <int MASK, bool F32>
-__device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&acc)[4][4], int e, int row0, int rows, int n0,
+template <int NI, int MASK, bool F32>
+__device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&acc)[NI][4], int e, int row0, int rows, int n0,
                                           int lane) {
   if (rows <= 0) return;
   constexpr int ES = F32 ? 4 : 2, MS = MASK == 1 ? 2 : 1;
   const int fr = lane & 31, h = lane >> 5, odd = lane & 1;
-  const int ldo = (int)g.ldo, ldm = (int)g.ldm, left = min(rows, 128);
+  const int ldo = (int)g.ldo, ldm = (int)g.ldm, left = min(rows, 32 * NI);
   const __amdgpu_buffer_rsrc_t o = out_rows(reinterpret_cast<char*>(g.out) + (size_t)row0 * g.ldo * ES, (uint32_t)left * ldo * ES);
   const __amdgpu_buffer_rsrc_t mr =
       out_rows(reinterpret_cast<const char*>(g.mask) + (size_t)row0 * g.ldm * MS, (uint32_t)left * ldm * MS);
   const float lo = g.relu ? 0.f : -INFINITY;
   const uint32_t sel = odd ? 0x07060302u : 0x01000504u;
+  constexpr int NQ = F32 ? 16 : 8;
+  auto row_of = [](int i, int q) {
+    const int k = F32 ? q : 2 * q;
+    return i * 32 + (k >> 2) * 8 + (k & 3);
+  };
+  // a column block's mask, read while the one before it is written
+  uint32_t m[2][NI][NQ];
+  const int rr = F32 ? h * 4 : h * 4 + odd;
+  auto mask_of = [&](int j) {
+    if (MASK == 0) return;
+    const int c = n0 + j * 32 + fr, cc = F32 ? c : c & ~1;
+    const int mt = (int)(cc < g.N ? (uint32_t)(rr * ldm + cc) * MS : GP_FAR);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int at = row_of(i, q) * ldm * MS;
+        if (MASK == 1) m[j & 1][i][q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, mt, at, 0)
+                                            : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(mr, mt, at, 0);
+        if (MASK == 2) m[j & 1][i][q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(mr, mt, at, 0)
+                                            : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, mt, at, 0);
+      }
+  };
+  float bias[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int c = n0 + j * 32 + fr;
-    const float bias = g.bias && c < g.N ? g.bias[(size_t)e * g.N + c] : 0.f;
-    const int cc = F32 ? c : c & ~1, rr = F32 ? h * 4 : h * 4 + odd;
+    bias[j] = g.bias && c < g.N ? g.bias[(size_t)e * g.N + c] : 0.f;
+  }
+  mask_of(0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = n0 + j * 32 + fr;
+    const int cc = F32 ? c : c & ~1;
     const uint32_t at = cc < g.N ? (uint32_t)(rr * ldo + cc) * ES : GP_FAR;
-    const uint32_t mt = cc < g.N ? (uint32_t)(rr * ldm + cc) * MS : GP_FAR;
+    if (j < 3) mask_of(j + 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      constexpr int NQ = F32 ? 16 : 8;
-      uint32_t m[NQ];
+    for (int i = 0; i < NI; ++i) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const int k = F32 ? q : 2 * q, row = i * 32 + (k >> 2) * 8 + (k & 3);
-        if (MASK == 1) m[q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, (int)mt, row * ldm * MS, 0)
-                                  : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(mr, (int)mt, row * ldm * MS, 0);
-        if (MASK == 2) m[q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(mr, (int)mt, row * ldm * MS, 0)
-                                  : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, (int)mt, row * ldm * MS, 0);
-      }
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int k = F32 ? q : 2 * q, row = i * 32 + (k >> 2) * 8 + (k & 3);
-        float v = __builtin_elementwise_maximum(fmaf(acc[i][j][k], g.scale, bias), lo);
+        const int k = F32 ? q : 2 * q;
+        float v = __builtin_elementwise_maximum(fmaf(acc[i][j][k], g.scale, bias[j]), lo);
         uint32_t w;
         if (F32) {
-          if (MASK == 1 && !(__uint_as_float(m[q] << 16) > 0.f)) v = 0.f;
-          if (MASK == 2 && !a8_positive(m[q])) v = 0.f;
+          if (MASK == 1 && !(__uint_as_float(m[j & 1][i][q] << 16) > 0.f)) v = 0.f;
+          if (MASK == 2 && !a8_positive(m[j & 1][i][q])) v = 0.f;
           w = __float_as_uint(v);
         } else {
           typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-          const float u = __builtin_elementwise_maximum(fmaf(acc[i][j][k + 1], g.scale, bias), lo);
+          const float u = __builtin_elementwise_maximum(fmaf(acc[i][j][k + 1], g.scale, bias[j]), lo);
           const uint32_t p = __builtin_bit_cast(uint32_t, bf16x2{f2bf(v), f2bf(u)});
           const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)p, 0xB1, 0xF, 0xF, true);     // lane ^ 1
           w = __builtin_amdgcn_perm(p, t, sel);
-          if (MASK == 1) w = (__uint_as_float(m[q] << 16) > 0.f ? w & 0xFFFFu : 0u) |
-                             (__uint_as_float(m[q] & 0xFFFF0000u) > 0.f ? w & 0xFFFF0000u : 0u);
-          if (MASK == 2) w = (a8_positive(m[q] & 0xFFu) ? w & 0xFFFFu : 0u) | (a8_positive(m[q] >> 8) ? w & 0xFFFF0000u : 0u);
+          const uint32_t mv = m[j & 1][i][q];
+          if (MASK == 1) w = (__uint_as_float(mv << 16) > 0.f ? w & 0xFFFFu : 0u) |
+                             (__uint_as_float(mv & 0xFFFF0000u) > 0.f ? w & 0xFFFF0000u : 0u);
+          if (MASK == 2) w = (a8_positive(mv & 0xFFu) ? w & 0xFFFFu : 0u) | (a8_positive(mv >> 8) ? w & 0xFFFF0000u : 0u);
         }
-        __builtin_amdgcn_raw_buffer_store_b32(w, o, (int)at, row * ldo * ES, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(w, o, (int)at, row_of(i, q) * ldo * ES, 0);
       }
     }
   }
 }
 
-// ---- NT: rows of A and B are K-contiguous.  A panel's step is 256 rows x 64 B; 16-byte chunk c of row r
-// lies at c ^ ((r >> 2) & 3): the 16 rows of a fragment read meet in 16 different chunks of 256 B.  K a
-// multiple of 8; the last step's chunks past K come from the zero source.
+// ---- NT: rows of A and B are K-contiguous, and 32-deep steps would ask the L2 for half lines (57 % of its
+// channels' cycles were requests, 28 % now): so two buffers of 64-deep steps (rows of 128 B, 16-byte chunk c
+// of row r at c ^ ((r >> 1) & 7)).  A step is two halves of 32: in half 0 the fragments of half 1 are read, and in half 1, after its second round, comes
+// the step's one barrier: the wave has read all of its buffer, and its DMA of the next step has landed.
+// Then the next step's first fragments are read, and the DMA of the step after it goes into this
+// step's buffer (12 pieces here, the rest at the start of the next half 0): 8 to 14 rounds of 128
+// cycles to arrive.  A piece is three instructions: the buffers do the bounds (with addresses of 64 bits
+// and a selected source of zeros it was eight, and the loop 8 % slower).  K a multiple of 8.
+constexpr uint32_t GP_NONE = 0xFFFF0000u;                // an offset past every buffer here, with a step's added too
+constexpr int GN2_K = 64, GN2_PANEL = GP_B * GN2_K * 2, GN2_BUF = 2 * GN2_PANEL;
+
+template <int NI>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
 group_nt_mm_kernel(GroupNtArgs g, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) char smem[GP_RING * GP_BUF];
+  __shared__ __attribute__((aligned(16))) char smem[2 * GN2_BUF];
   // (the grid has room for one more row tile per group: the tiles that there are go round the XCDs)
-  const int tiles_m = group_tiles<GP_B>(g.offs, g.E, g.S);
+  const int tiles_m = group_tiles<64 * NI>(g.offs, g.E, g.S);
   if ((int)blockIdx.x >= tiles_m * tiles_n) return;
   int tm, tn;
   band_tile(xcd_order(blockIdx.x, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   int e, r0, r1;
-  if (!group_find<GP_B>(g.offs, g.E, g.S, tm, e, r0, r1)) return;
+  if (!group_find<64 * NI>(g.offs, g.E, g.S, tm, e, r0, r1)) return;
   const int n0 = tn * GP_B;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave >> 1, wc = wave & 1;
   const int fr = lane & 31, fq = lane >> 5;
-  // fragment (half h, rows 32 i ..): row fr, chunk 2 h + fq
-  const int f0 = fr * 64 + ((fq ^ ((fr >> 2) & 3)) << 4), f1 = f0 ^ 32;
-  const int la = wr * 128 * 64, lb = GP_PANEL + wc * 128 * 64;
-  // staging pieces of 16 rows x 64 B: 4 of A and 4 of B per wave.  Rows past the group's end and
-  // columns past N read the last one (their outputs are not stored).
-  const bf16* src[8];
-  bool none[4];                                              // (a source that is no slot: zeros)
-  const int ck = ((lane & 3) ^ ((lane >> 4) & 3)) * 8;       // (row of the piece: lane >> 2)
+  // fragment (16-deep quarter q, rows 32 i ..): row fr, chunk 2 q + fq
+  const int sw = (fr >> 1) & 7;
+  int fo[4];
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const int r = (wave * 4 + (p & 3)) * 16 + (lane >> 2);
-    if (p < 4) {
-      const int row = group_row(g.src, min(r0 + r, r1 - 1), g.rows, g.top_k);
-      src[p] = g.a + (size_t)max(row, 0) * g.lda + ck;
-      none[p] = row < 0;
-    } else {
-      src[p] = g.b + (size_t)e * g.es + (size_t)min(n0 + r, g.N - 1) * g.ldb + ck;
+  for (int q = 0; q < 4; ++q) fo[q] = fr * 128 + (((2 * q + fq) ^ sw) << 4);
+  const int la = wr * 32 * NI * 128, lb = GN2_PANEL + wc * 128 * 128;
+  // staging pieces of 8 rows x 128 B: 2 NI of A and 8 of B per wave, from buffers that end with the group's
+  // rows (with x, where rows are taken through src) and with w's: what lies past them reads as zeros.
+  constexpr int PA = 2 * NI, PN = PA + 8;
+  const int pr = lane >> 3;                                  // row of a piece
+  const int ck0 = ((lane & 7) ^ ((pr >> 1) & 7)) * 8;        // its chunk's column (even pieces of 8 rows; odd: ^ 32)
+  const int odd0 = (wave * PA) & 1;
+  auto odd_piece = [&](int p) { return p < PA ? ((p + odd0) & 1) != 0 : ((p - PA) & 1) != 0; };
+  uint32_t off[PN];
+#pragma unroll
+  for (int p = 0; p < PN; ++p) {
+    const int r = (p < PA ? wave * PA + p : wave * 8 + p - PA) * 8 + pr;
+    const uint32_t ck = odd_piece(p) ? ck0 ^ 32 : ck0;
+    if (p >= PA) off[p] = 2u * ((uint32_t)r * (uint32_t)g.ldb + ck);
+    else if (!g.src) off[p] = 2u * ((uint32_t)r * (uint32_t)g.lda + ck);
+    else {
+      const int row = r0 + r < r1 ? group_row(g.src, r0 + r, g.rows, g.top_k) : -1;
+      off[p] = row < 0 ? GP_NONE : 2u * ((uint32_t)row * (uint32_t)g.lda + ck);
     }
   }
-  f32x16 acc[4][4] = {};
-  mm_loop<8>(
-      smem, (g.K + GP_K - 1) / GP_K, acc,
-      [&](int p, int s) {
-        const void* q = src[p] + s * GP_K;
-        const bool zero = (s * GP_K + ck >= g.K) | (p < 4 ? none[p & 3] : false);
-        q = zero ? (const void*)g_zero16 : q;
-        dma16(q, smem + (s & (GP_RING - 1)) * GP_BUF + (p >= 4 ? GP_PANEL : 0) + (wave * 4 + (p & 3)) * 1024);
-      },
-      [&](int i, const char* b) { return *reinterpret_cast<const bf16x8*>(b + la + (i < 4 ? f0 : f1) + (i & 3) * 32 * 64); },
-      [&](int j, const char* b) { return *reinterpret_cast<const bf16x8*>(b + lb + (j < 4 ? f0 : f1) + (j & 3) * 32 * 64); },
-      [](auto, int) {});
-  const int row0 = r0 + wr * 128, n1 = n0 + wc * 128;
+  const __amdgpu_buffer_rsrc_t ab = out_rows(g.src ? g.a : g.a + (size_t)r0 * g.lda,
+                                             2u * (uint32_t)((g.src ? g.rows : min(r1 - r0, 64 * NI)) * (uint32_t)g.lda));
+  const __amdgpu_buffer_rsrc_t bb = out_rows(g.b + (size_t)e * g.es + (size_t)n0 * g.ldb,
+                                             2u * (uint32_t)min(g.N - n0, GP_B) * (uint32_t)g.ldb);
+  auto stage = [&](int p, int t) {
+    // (a chunk past K: zeros too)
+    const uint32_t v = t * GN2_K + (odd_piece(p) ? ck0 ^ 32 : ck0) < g.K ? off[p] : GP_NONE;
+    char* to = smem + (t & 1) * GN2_BUF + (p < PA ? (wave * PA + p) * 1024 : GN2_PANEL + (wave * 8 + p - PA) * 1024);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(p < PA ? ab : bb, (__attribute__((address_space(3))) void*)to, 16, (int)v,
+                                             t * GN2_K * 2, 0, 0);
+  };
+  // fragments r = 0 .. 2 NI - 1 of a half: quarter 2 h + r / NI, rows 32 (r % NI) ..
+  auto load_a = [&](int r, int h, const char* b) {
+    return *reinterpret_cast<const bf16x8*>(b + la + fo[2 * h + r / NI] + (r % NI) * 32 * 128);
+  };
+  auto load_b = [&](int j, int h, const char* b) {
+    return *reinterpret_cast<const bf16x8*>(b + lb + fo[2 * h + (j >> 2)] + (j & 3) * 32 * 128);
+  };
+  constexpr int NA = 2 * NI, EARLY = 2 * (NA - 2);           // pieces that follow the barrier (two a round)
+  const int nt = (g.K + GN2_K - 1) / GN2_K;
+#pragma unroll
+  for (int p = 0; p < PN; ++p) stage(p, 0);
+#pragma unroll
+  for (int p = 0; p < EARLY; ++p) stage(p, 1);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EARLY) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  bf16x8 fa[NA], fb[2][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) fb[0][j] = load_b(j, 0, smem);
+#pragma unroll
+  for (int r = 0; r < NA - 1; ++r) fa[r] = load_a(r, 0, smem);
+  f32x16 acc[NI][4] = {};
+  for (int t = 0; t < nt; ++t) {
+    const char* cur = smem + (t & 1) * GN2_BUF;
+    const char* nxt = smem + ((t + 1) & 1) * GN2_BUF;
+    // (a row fragment is read after its round, the last one after the next half's first MFMA: nothing is
+    // read just before a half begins, where the compiler waits for all reads)
+    constexpr int FB0 = 2, FB1 = NI == 4 ? 2 : 3;            // column fragments a round, in halves 0 and 1
+    // half 0
+#pragma unroll
+    for (int k = 0; k < 4 * NA; ++k) {
+      const int r = k >> 2, j = k & 3;
+      acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[0][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
+      if (k == 0) fa[NA - 1] = load_a(NA - 1, 0, cur);
+      if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1, 1, cur);
+      if (j == 2) {
+#pragma unroll
+        for (int i = FB0 * r; i < FB0 * r + FB0 && i < 8; ++i) fb[1][i] = load_b(i, 1, cur);
+      }
+      if ((j & 1) && EARLY + 2 * r + (j >> 1) < PN) stage(EARLY + 2 * r + (j >> 1), t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // half 1
+#pragma unroll
+    for (int k = 0; k < 4 * NA; ++k) {
+      const int r = k >> 2, j = k & 3;
+      acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[1][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
+      if (k == 0) fa[NA - 1] = load_a(NA - 1, 1, cur);
+      if (k == 7) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");      // (no access moves over the barrier)
+      }
+      if (r >= 2) {
+        if (j == 0) {
+          fa[r - 1] = load_a(r - 1, 0, nxt);
+          if (r == 2) fa[0] = load_a(0, 0, nxt);
+        }
+        if (j == 2) {
+#pragma unroll
+          for (int i = FB1 * (r - 2); i < FB1 * (r - 2) + FB1 && i < 8; ++i) fb[0][i] = load_b(i, 0, nxt);
+        }
+        if (j & 1) stage(2 * (r - 2) + (j >> 1), t + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (nothing in flight into LDS at the end)
+  const int row0 = r0 + wr * 32 * NI, n1 = n0 + wc * 128;
   if (!g.mask) {
-    if (g.out_f32) mm_out_nt<0, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<0, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    if (g.out_f32) mm_out_nt<NI, 0, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<NI, 0, false>(g, acc, e, row0, r1 - row0, n1, lane);
   } else if (!g.mask8) {
-    if (g.out_f32) mm_out_nt<1, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<1, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    if (g.out_f32) mm_out_nt<NI, 1, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<NI, 1, false>(g, acc, e, row0, r1 - row0, n1, lane);
   } else {
-    if (g.out_f32) mm_out_nt<2, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<2, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    if (g.out_f32) mm_out_nt<NI, 2, true>(g, acc, e, row0, r1 - row0, n1, lane);
+    else mm_out_nt<NI, 2, false>(g, acc, e, row0, r1 - row0, n1, lane);
   }
 }
 
@@ -474,11 +594,23 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   // the large tile stores (and reads the mask) in column pairs of bf16
   const bool pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && g.ldm % 2 == 0 && (uintptr_t)g.out % 4 == 0 &&
                      (uintptr_t)g.mask % (g.mask8 ? 2 : 4) == 0 && g.ldo < GP_MAXLD && g.ldm < GP_MAXLD;
-  if (vec && pairs && g.K >= 64) {
+  // ... and takes rows through 32-bit offsets: all of x where src says which, else 256 rows
+  const bool near = (g.src ? (long)g.rows * g.lda : 256l * g.lda) < 0x7F000000l && 256l * g.ldb < 0x7F000000l && g.K < 0x7F00;
+  if (vec && pairs && near && g.K >= 64) {
+    // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
+    // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
+    // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 192: MEASURED).
     const int tn = (g.N + GP_B - 1) / GP_B;
-    const long blocks = (long)(g.S / GP_B + g.E) * tn;
+    const double step = 0.85 / 256 * ((g.K + GP_K - 1) / GP_K);
+    auto cost = [&](int rows) {
+      const double tiles = (g.E == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * g.E) * tn;
+      return ceil(tiles / 256) * (step * rows + 12.0);
+    };
+    const int rows = cost(192) < cost(256) ? 192 : 256;
+    const long blocks = (long)(g.S / rows + g.E) * tn;
     if (blocks >= GP_MIN_TILES && blocks <= 0x7FFFFFFFl) {
-      hipLaunchKernelGGL(group_nt_mm_kernel, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
+      if (rows == 256) hipLaunchKernelGGL(group_nt_mm_kernel<4>, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
+      else hipLaunchKernelGGL(group_nt_mm_kernel<3>, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
       HFM_LAUNCH_CHECK();
     }
   }
@@ -652,7 +784,7 @@ __global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
 // columns]; the fragments (8 rows of one column per lane) come from transposing LDS reads
 // (ds_read_b64_tr_b16: a 16-lane group reads 4 rows x 16 columns, lane l gets column l's 4 rows).
 // A panel row is 512 B, so a fragment's 16 rows would meet in the same banks: 32-byte granule c of row r
-// lies at c ^ f(r), f(r) = (r & 3) | (r >> 1 & 4), which spreads them over all 8 granules of 256 B.
+// lies at c ^ f(r), f(r) = (r & 3) << 1 | (r >> 3 & 1): a half-wave's 4 rows x 2 granules take all 8 of 256 B.
 // 8-bit x: 32 codes a thread (one scale) are loaded two steps ahead, turned into bf16 times the
 // scale (one conversion per pair, exact) and written into the same image.
 //
@@ -749,17 +881,17 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   // fragment (half h, columns 32 i ..): the lane's 16-lane group takes rows 16 h + 8 (lane >> 5) .. and
   // columns 32 i + (lane & 16) ..: granule (2 i + (lane >> 4 & 1)) ^ f(row), which is an xor with 2 i
   const int l4 = (lane >> 2) & 3, h5 = lane >> 5;
-  const int rowoff = (h5 * 8 + l4) * 512 + (lane & 3) * 8 + ((((lane >> 4) & 1) ^ l4 ^ (h5 << 2)) << 5);
+  const int rowoff = (h5 * 8 + l4) * 512 + (lane & 3) * 8 + ((((lane >> 4) & 1) ^ (l4 << 1) ^ h5) << 5);
   int la = rowoff + wr * 256, lb = GP_PANEL + rowoff + wc * 256;
   // staging pieces: 2 rows of 512 B, 4 of each operand per wave.  Row 2 i + hi of the wave's 8 has
-  // f = ((2 i + hi) & 3) | 4 (wave & 1), so the lane's 16-byte chunk is one column for even i and
-  // that column ^ 32 for odd i.
+  // f = 2 ((2 i + hi) & 3) + (wave & 1), so the lane's 16-byte chunk is one column for even i and
+  // that column ^ 64 for odd i.
   const int hi = lane >> 5, c16 = lane & 31;
-  const int ce = (((c16 >> 1) ^ (hi | ((wave & 1) << 2))) * 2 + (c16 & 1)) * 8;
+  const int ce = (((c16 >> 1) ^ ((hi << 1) | (wave & 1))) * 2 + (c16 & 1)) * 8;
   const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
   // 8-bit x: 32 codes (granules 2 q, 2 q + 1) of row xr
   const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32;
-  const int xf = (xr & 3) | ((xr >> 1) & 4);
+  const int xf = ((xr & 3) << 1) | ((xr >> 3) & 1);
   const int xo = GP_PANEL + xr * 512 + (((2 * xq) ^ xf) << 5);        // (granule 2 q + 1: ^ 32)
   for (; e < g.E && first < u1; ++e) {
     const int steps = wg_steps(g.offs, e, g.S), rows0 = first + GW_SEG;      // (the group's rows begin here)
@@ -775,8 +907,8 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     f32x16 acc[4][4] = {};
     // columns past N or K read column 0 (their outputs are not stored)
     const uint32_t ao0 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + ce < g.N ? n0 + ce : 0));
-    const uint32_t ao1 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + (ce ^ 32) < g.N ? n0 + (ce ^ 32) : 0));
-    const int bc0 = k0 + ce < g.K ? k0 + ce : 0, bc1 = k0 + (ce ^ 32) < g.K ? k0 + (ce ^ 32) : 0;
+    const uint32_t ao1 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + (ce ^ 64) < g.N ? n0 + (ce ^ 64) : 0));
+    const int bc0 = k0 + ce < g.K ? k0 + ce : 0, bc1 = k0 + (ce ^ 64) < g.K ? k0 + (ce ^ 64) : 0;
     const uint32_t bo0 = GATHER ? 0u : 2u * (uint32_t)(hi * (int)g.ldx + bc0);
     const uint32_t bo1 = GATHER ? 0u : 2u * (uint32_t)(hi * (int)g.ldx + bc1);
     // GATHER: rows of x of a step's pieces (or of its codes), read two steps before they are used;
@@ -876,7 +1008,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         codes_of(0, 4);
         rows_of(1, 5);
         rows_of(0, 6);
-        mm_loop<4>(smem, ns, acc, piece_a, load_a, load_b, [&](auto PAR, int s) {
+        mm_loop<4, 4>(smem, ns, acc, piece_a, load_a, load_b, [&](auto PAR, int s) {
           constexpr int set = decltype(PAR)::value ^ 1;
           hide();
           codes_to(set, s + 3);
@@ -885,7 +1017,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         });
       } else {
         // GATHER: a step's rows are read two steps before its DMA starts
-        mm_loop<8>(
+        mm_loop<4, 8>(
             smem, ns, acc,
             [&](int i, int s) {
               if (i < 4) piece_a(i, s);
