@@ -52,56 +52,68 @@ __device__ __forceinline__ float gate_value(const void* l, size_t i, int bf) {
   return fminf(v, 3.402823466e38f);
 }
 
-// The top_k experts of one token by a group of G lanes (G a power of two, lane gl of the group holds
-// experts gl + G q).  Lane j of the group ends with choice j (expert, weight; -1, 0 if none).
-template <int V>
-__device__ __forceinline__ void route_token(float (&v)[V], int E, int k, int renorm, int G, int gl, int& my_e,
-                                            float& my_w) {
-  float sum_all = 0.f, top = -INFINITY;
+// Maximum and sum over each group of G lanes (G a power of two), in all of its lanes, by lane swaps
+// in the vector unit: a shuffle through LDS takes over 100 cycles, and a choice needs one for each of
+// log2 G steps (16384 x 64, top 2: MEASURED us with shuffles, MEASURED with these).
+template <int G, typename F>
+__device__ __forceinline__ float group_all(float v, F op) {
+#define HFM_DPP(ctrl) __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), ctrl, 0xF, 0xF, true))
+  if (G >= 2) v = op(v, HFM_DPP(0xB1));        // quad: 1 0 3 2
+  if (G >= 4) v = op(v, HFM_DPP(0x4E));        // quad: 2 3 0 1
+  if (G >= 8) v = op(v, HFM_DPP(0x141));       // half row mirrored (quads are uniform by now)
+  if (G >= 16) v = op(v, HFM_DPP(0x140));      // row mirrored
+#undef HFM_DPP
+  if (G >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if (G >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
+}
+
+// The top_k experts of one token by a group of G lanes (lane gl of the group holds experts gl + G q).
+// Lane j of the group ends with choice j (expert, weight; -1, 0 if none).
+template <int G, int V>
+__device__ __forceinline__ void route_token(float (&v)[V], int k, int renorm, int lane, int& my_e, float& my_w) {
+  const int gl = lane & (G - 1);
+  const unsigned long long mine = (G == 64 ? ~0ull : ((1ull << G) - 1) << (lane & ~(G - 1)));
+  float top = -INFINITY, my_v = -INFINITY, o[V];
   my_e = -1;
-  float my_v = -INFINITY;
-  float o[V];
 #pragma unroll
   for (int q = 0; q < V; ++q) o[q] = v[q];
   for (int j = 0; j < k; ++j) {
-    float bv = -INFINITY;
-    int bi = 0x7FFFFFFF;
+    float m = v[0];
 #pragma unroll
-    for (int q = 0; q < V; ++q)          // (ascending index: a strict > keeps the lowest on ties)
-      if (v[q] > bv) {
-        bv = v[q];
-        bi = gl + G * q;
-      }
-    for (int d = G >> 1; d; d >>= 1) {
-      const float ov = __shfl_xor(bv, d);
-      const int oi = __shfl_xor(bi, d);
-      if (ov > bv || (ov == bv && oi < bi)) {
-        bv = ov;
-        bi = oi;
-      }
+    for (int q = 1; q < V; ++q) m = fmaxf(m, v[q]);
+    m = group_all<G>(m, [](float a, float b) { return fmaxf(a, b); });
+    if (j == 0) top = m;
+    // the lowest index among equals: the first q that has one, its first lane
+    int at = -1;
+#pragma unroll
+    for (int q = V - 1; q >= 0; --q) {
+      const unsigned long long has = __ballot(v[q] == m) & mine;
+      if (has) at = G * q + ((__ffsll(has) - 1) & (G - 1));
     }
-    if (bv == -INFINITY) break;           // (the same in all lanes of the group)
-    if (j == 0) top = bv;
+    if (m == -INFINITY) at = -1;              // (all closed)
     if (gl == j) {
-      my_e = bi;
-      my_v = bv;
+      my_e = at;
+      my_v = m;
     }
 #pragma unroll
     for (int q = 0; q < V; ++q)
-      if (bi == gl + G * q) v[q] = -INFINITY;
+      if (at == gl + G * q) v[q] = -INFINITY;
   }
   const float ex = my_e >= 0 ? expf(my_v - top) : 0.f;
-  float den;
-  if (renorm) {
-    den = ex;
-  } else {
+  float den = ex;
+  if (!renorm) {
     den = 0.f;
-    if (top != -INFINITY) {
 #pragma unroll
-      for (int q = 0; q < V; ++q) den += o[q] == -INFINITY ? 0.f : expf(o[q] - top);
-    }
+    for (int q = 0; q < V; ++q) den += o[q] == -INFINITY ? 0.f : expf(o[q] - top);
   }
-  for (int d = G >> 1; d; d >>= 1) den += __shfl_xor(den, d);
+  den = group_all<G>(den, [](float a, float b) { return a + b; });
   my_w = den > 0.f ? ex / den : 0.f;
 }
 
@@ -118,10 +130,11 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base
   const int ng = RT_THREADS / ep, gr = tid / ep;
   for (int e = tid % ep; e < a.E; e += ep) {
     int before = 0, all = 0;
+#pragma unroll 8
     for (int r = gr; r < a.nblk; r += ng) {
       const int c = a.bh[(size_t)r * a.E + e];
       all += c;
-      if (r < b) before += c;
+      before += r < b ? c : 0;
     }
     atomicAdd(&base[e], before);           // (integers: the order does not matter)
     atomicAdd(&tot[e], all);
@@ -169,8 +182,8 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base
 // per token), then the rank of each slot among the wave's earlier slots of its expert (64 slots at a
 // time: the lanes with the same expert by one ballot per index bit).  One block (few tokens) places
 // its slots at once, several leave it to route_place_kernel.
-template <int V>
-__global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a, int G) {
+template <int G, int V>
+__global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a) {
   extern __shared__ int lds[];
   int* wh = lds;                                                // [waves, E]
   short* se = reinterpret_cast<short*>(lds + RT_WAVES * a.E);   // [waves, RT_CHUNK]
@@ -183,23 +196,31 @@ __global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a, int G) {
   const int t0 = b * a.tpb, t1 = min(a.T, t0 + a.tpb);
   const int per = (a.tpb + RT_WAVES - 1) / RT_WAVES;
   const int w0 = min(t1, t0 + wave * per), w1 = min(t1, t0 + (wave + 1) * per);
-  const int gl = lane & (G - 1), gi = lane / G, ngr = 64 / G;
-  const int ct = RT_CHUNK / a.k;                                 // tokens per chunk
+  const int gl = lane & (G - 1), gi = lane / G;
+  constexpr int NG = 64 / G;                                     // tokens at a time
+  const int ct = RT_CHUNK / a.k / NG * NG;                       // tokens per chunk
   int bits = 0;
   while ((1 << bits) < a.E) ++bits;
+  float nv[V];                                                   // the next tokens' logits, under way
+  auto fetch = [&](int t) {
+    const bool on = t < w1 && (!a.valid || a.valid[t]);
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const int e = gl + G * q;
+      nv[q] = on && e < a.E ? gate_value(a.logits, (size_t)t * a.ld + e, a.bf) : -INFINITY;
+    }
+  };
+  fetch(w0 + gi);
   for (int c0 = w0; c0 < w1; c0 += ct) {
     const int c1 = min(w1, c0 + ct);
-    for (int t = c0 + gi; t - gi < c1; t += ngr) {
-      const bool on = t < c1 && (!a.valid || a.valid[t]);
+    for (int t = c0 + gi; t - gi < c1; t += NG) {
       float v[V];
 #pragma unroll
-      for (int q = 0; q < V; ++q) {
-        const int e = gl + G * q;
-        v[q] = on && e < a.E ? gate_value(a.logits, (size_t)t * a.ld + e, a.bf) : -INFINITY;
-      }
+      for (int q = 0; q < V; ++q) v[q] = nv[q];
+      fetch(t + NG);
       int e;
       float w;
-      route_token<V>(v, a.E, a.k, a.renorm, G, gl, e, w);
+      route_token<G, V>(v, a.k, a.renorm, lane, e, w);
       if (t < c1 && gl < a.k) {
         a.expert[(size_t)t * a.k + gl] = e;
         a.weight[(size_t)t * a.k + gl] = w;
@@ -227,7 +248,9 @@ __global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a, int G) {
   }
   __syncthreads();
   // slots of the block's earlier waves (in place), the block's histogram
+  int* base = reinterpret_cast<int*>(se + RT_WAVES * RT_CHUNK);
   int* pre = gridDim.x == 1 ? wh : a.wpre + (size_t)b * RT_WAVES * a.E;
+  if (gridDim.x == 1) a.bh = base + 2 * RT_MAXE + 1;
   for (int e = tid; e < a.E; e += RT_THREADS) {
     int run = 0;
     for (int w = 0; w < RT_WAVES; ++w) {
@@ -240,7 +263,6 @@ __global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a, int G) {
   if (gridDim.x != 1) return;
   __threadfence_block();
   __syncthreads();
-  int* base = reinterpret_cast<int*>(se + RT_WAVES * RT_CHUNK);
   route_place(a, 0, base, base + 2 * RT_MAXE, wh);
 }
 
@@ -263,7 +285,10 @@ HFM_API int hfm_route_blocks(int T, int E) {
   const int n = (T + 4 * round - 1) / (4 * round);
   return n < RT_MAXBLK ? n : RT_MAXBLK;
 }
-HFM_API int hfm_route_ws_ints(int T, int E) { return hfm_route_blocks(T, E) * E * (1 + RT_WAVES); }
+HFM_API int hfm_route_ws_ints(int T, int E) {
+  const int n = hfm_route_blocks(T, E);
+  return n == 1 ? 0 : n * E * (1 + RT_WAVES);      // (one block keeps its counts in LDS)
+}
 
 HFM_API int hfm_route(const RouteArgs* ap, hipStream_t st) {
   RouteArgs a = *ap;
@@ -275,43 +300,60 @@ HFM_API int hfm_route(const RouteArgs* ap, hipStream_t st) {
   a.tpb = a.T > 0 ? (a.T + a.nblk - 1) / a.nblk : 1;
   a.wpre = a.bh + (size_t)a.nblk * a.E;
   size_t lds = (size_t)RT_WAVES * a.E * 4 + RT_WAVES * RT_CHUNK * 2;
-  if (a.nblk == 1) lds += (2 * RT_MAXE + 1) * 4;
+  if (a.nblk == 1) lds += (3 * RT_MAXE + 1) * 4;
   const dim3 grid(a.nblk), blk(RT_THREADS);
-  const int V = (a.E + 63) / 64;
-  if (V <= 1) hipLaunchKernelGGL(route_kernel<1>, grid, blk, lds, st, a, G);
-  else if (V <= 2) hipLaunchKernelGGL(route_kernel<2>, grid, blk, lds, st, a, G);
-  else if (V <= 4) hipLaunchKernelGGL(route_kernel<4>, grid, blk, lds, st, a, G);
-  else if (V <= 8) hipLaunchKernelGGL(route_kernel<8>, grid, blk, lds, st, a, G);
-  else hipLaunchKernelGGL(route_kernel<16>, grid, blk, lds, st, a, G);
+#define HFM_ROUTE(G, V) hipLaunchKernelGGL((route_kernel<G, V>), grid, blk, lds, st, a)
+  switch (G) {
+    case 1: HFM_ROUTE(1, 1); break;
+    case 2: HFM_ROUTE(2, 1); break;
+    case 4: HFM_ROUTE(4, 1); break;
+    case 8: HFM_ROUTE(8, 1); break;
+    case 16: HFM_ROUTE(16, 1); break;
+    case 32: HFM_ROUTE(32, 1); break;
+    default:
+      if (a.E <= 64) HFM_ROUTE(64, 1);
+      else if (a.E <= 128) HFM_ROUTE(64, 2);
+      else if (a.E <= 256) HFM_ROUTE(64, 4);
+      else if (a.E <= 512) HFM_ROUTE(64, 8);
+      else HFM_ROUTE(64, 16);
+  }
+#undef HFM_ROUTE
   if (a.nblk > 1) hipLaunchKernelGGL(route_place_kernel, grid, blk, 0, st, a);
   HFM_LAUNCH_CHECK();
 }
 
 // A group of G lanes per token again.  p_i needs no second softmax: the first choice has the largest
 // logit m and the weight exp(0) / den, so p_i = exp(l_i - m) w_0.
+template <int K>
 __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a, int G) {
   const int lane = threadIdx.x & 63;
   const int gl = lane & (G - 1);
-  const int t = (blockIdx.x * 256 + threadIdx.x) / G;
-  if (t >= a.T) return;                    // (whole groups)
-  const int* ex = a.expert + (size_t)t * a.k;
-  const float* w = a.weight + (size_t)t * a.k;
-  const float* g = a.dweight + (size_t)t * a.k;
-  float dot = 0.f;
-  for (int j = 0; j < a.k; ++j)
+  const int t = (int)(((long)blockIdx.x * 256 + threadIdx.x) / G);
+  if (t >= a.T) return;
+  int ex[K];
+  float w[K], g[K], dot = 0.f;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const size_t o = (size_t)t * a.k + j;
+    ex[j] = j < a.k ? a.expert[o] : -1;
+    w[j] = j < a.k ? a.weight[o] : 0.f;
+    g[j] = j < a.k ? a.dweight[o] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j)
     if (ex[j] >= 0) dot = fmaf(w[j], g[j], dot);
-  const int e0 = ex[0];
-  const bool any = e0 >= 0 && e0 < a.E;
-  const float m = any ? gate_value(a.logits, (size_t)t * a.ld + e0, a.bf) : 0.f;
-  const float w0 = w[0];
+  const bool any = ex[0] >= 0 && ex[0] < a.E;
+  const float m = any && !a.renorm ? gate_value(a.logits, (size_t)t * a.ld + ex[0], a.bf) : 0.f;
+#pragma unroll 4
   for (int i = gl; i < a.E; i += G) {
     float d = 0.f;
     if (any) {
       if (!a.renorm) {
         const float l = gate_value(a.logits, (size_t)t * a.ld + i, a.bf);
-        if (l != -INFINITY) d = -expf(l - m) * w0 * dot;
+        if (l != -INFINITY) d = -expf(l - m) * w[0] * dot;
       }
-      for (int j = 0; j < a.k; ++j)
+#pragma unroll
+      for (int j = 0; j < K; ++j)
         if (ex[j] == i) d = a.renorm ? w[j] * (g[j] - dot) : fmaf(w[j], g[j], d);
     }
     const size_t o = (size_t)t * a.ldo + i;
@@ -325,7 +367,12 @@ HFM_API int hfm_route_bwd(const RouteBwdArgs* ap, hipStream_t st) {
   if (a.T < 0 || a.E < 1 || a.E > RT_MAXE || a.k < 1 || a.k > RT_MAXK) return (int)hipErrorInvalidValue;
   if (a.T == 0) return 0;
   const int G = route_group(a.E), per = 256 / G;
-  hipLaunchKernelGGL(route_bwd_kernel, dim3((a.T + per - 1) / per), dim3(256), 0, st, a, G);
+  const dim3 grid((a.T + per - 1) / per), blk(256);
+  if (a.k <= 1) hipLaunchKernelGGL(route_bwd_kernel<1>, grid, blk, 0, st, a, G);
+  else if (a.k <= 2) hipLaunchKernelGGL(route_bwd_kernel<2>, grid, blk, 0, st, a, G);
+  else if (a.k <= 4) hipLaunchKernelGGL(route_bwd_kernel<4>, grid, blk, 0, st, a, G);
+  else if (a.k <= 8) hipLaunchKernelGGL(route_bwd_kernel<8>, grid, blk, 0, st, a, G);
+  else hipLaunchKernelGGL(route_bwd_kernel<16>, grid, blk, 0, st, a, G);
   HFM_LAUNCH_CHECK();
 }
 HFM_API int hfm_route_args_bytes() { return (int)sizeof(RouteArgs); }

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import Act8Args, check, ptr
-from .checks import contiguous, launch, need, out_or_new, row_stride, rows2d
+from .checks import flat, launch, out_or_new, row_stride, rows2d
 
 BLOCK = 32            # columns per scale
 
@@ -42,11 +42,22 @@ def empty(M: int, N: int, device) -> Act8:
                 torch.empty(M, scale_cols(N), dtype=torch.uint8, device=device))
 
 
+_U8 = (torch.uint8,)
+
+
 def check_act8(a: Act8, M: int, N: int, what: str) -> None:
-    need(isinstance(a, Act8), f"{what} must be an Act8")
-    rows2d(a.codes, f"{what}.codes", (torch.uint8,), M, N)
-    need(a.scales.dtype == torch.uint8 and tuple(a.scales.shape) == (M, scale_cols(N)) and contiguous(a.scales),
-         f"{what}.scales must be a contiguous uint8 [{M}, {scale_cols(N)}]")
+    if not isinstance(a, Act8):
+        raise ValueError(f"{what} must be an Act8")
+    rows2d(a.codes, what + ".codes", _U8, M, N)
+    flat(a.scales, what + ".scales", torch.uint8, (M, scale_cols(N)))
+
+
+def check_own_act8(a: Act8, what: str) -> None:
+    """``a`` is an Act8 whose parts fit one another."""
+    if not isinstance(a, Act8):
+        raise ValueError(f"{what} must be an Act8")
+    rows2d(a.codes, what + ".codes", _U8)
+    flat(a.scales, what + ".scales", torch.uint8, (a.codes.shape[0], scale_cols(a.codes.shape[1])))
 
 
 _VALUES = (torch.float32, torch.bfloat16)
@@ -70,12 +81,11 @@ def pack(x: torch.Tensor, out: Optional[Act8] = None) -> Act8:
 def unpack(a: Act8, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values that ``a`` stands for, in fp32 or bf16 (exact in both, but where a value of a
     block with the smallest scales lies below the type's normal range)."""
-    need(isinstance(a, Act8), "a must be an Act8")
-    need(a.codes.dim() == 2, "a.codes must be 2-D")
+    check_own_act8(a, "a")
     M, N = a.codes.shape
-    check_act8(a, M, N, "a")
-    need(dtype in _VALUES, f"unpack to fp32 or bf16, not {dtype}")
-    out = out_or_new(out, (M, N), dtype, a.codes.device)
+    if dtype not in _VALUES:
+        raise ValueError(f"unpack to fp32 or bf16, not {dtype}")
+    out = out_or_new(out, M, N, dtype, a.codes.device)
     args = Act8Args(0, ptr(a.codes), ptr(a.scales), ptr(out), row_stride(out), row_stride(a.codes), M, N,
                     1 if dtype == torch.bfloat16 else 0)
     with launch("act8.unpack", *a, out) as st:

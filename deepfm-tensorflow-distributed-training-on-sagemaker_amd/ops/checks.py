@@ -3,7 +3,8 @@
 
 Shapes, types and strides are checked before the device, so a wrong call is refused the same way
 with or without a GPU.  Launches go to the current stream of the operands' device, whichever device
-is current; nothing synchronizes, so calls can be captured into a HIP graph.
+is current; nothing synchronizes, so calls can be captured into a HIP graph.  A small call's time is
+the host's: the checks of a good call build no text.
 """
 from __future__ import annotations
 
@@ -15,44 +16,46 @@ import torch
 LIMIT = 1 << 31          # rows, columns: int32 in the kernels
 
 
-def need(ok: bool, msg: str) -> None:
-    if not ok:
-        raise ValueError(msg)
-
-
-def contiguous(t: torch.Tensor) -> bool:
-    return t.is_contiguous()
-
-
 def row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    """Elements from a row to the next (of a single row: any that hold it)."""
+    s = t.stride(0)
+    return s if t.shape[0] > 1 else max(s, t.shape[1])
 
 
 def rows2d(t: torch.Tensor, what: str, dtypes: Sequence[torch.dtype], M: Optional[int] = None,
            N: Optional[int] = None) -> None:
     """``t`` is [M, N] of one of ``dtypes`` with unit column stride and rows that do not overlap."""
-    need(isinstance(t, torch.Tensor), f"{what} must be a tensor")
-    need(t.dim() == 2, f"{what} must be 2-D, got {tuple(t.shape)}")
-    need(t.dtype in dtypes, f"{what} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
-    need((M is None or t.shape[0] == M) and (N is None or t.shape[1] == N),
-         f"{what} must be [{'any' if M is None else M}, {'any' if N is None else N}], got {tuple(t.shape)}")
-    need(t.shape[0] < LIMIT and t.shape[1] < LIMIT, f"{what} is too large: {tuple(t.shape)}")
-    if t.numel():
-        need(t.shape[1] == 1 or t.stride(1) == 1, f"{what}'s columns must be adjacent")
-        need(t.shape[0] == 1 or t.stride(0) >= t.shape[1], f"{what}'s rows must not overlap")
+    if isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes:
+        m, n = t.shape
+        s0, s1 = t.stride()
+        if ((M is None or m == M) and (N is None or n == N) and m < LIMIT and n < LIMIT
+                and (((s1 == 1 or n == 1) and (s0 >= n or m == 1)) or m == 0 or n == 0)):
+            return
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what} must be a tensor")
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D, got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if (M is not None and t.shape[0] != M) or (N is not None and t.shape[1] != N):
+        raise ValueError(f"{what} must be [{'any' if M is None else M}, {'any' if N is None else N}], "
+                         f"got {tuple(t.shape)}")
+    if max(t.shape) >= LIMIT:
+        raise ValueError(f"{what} is too large: {tuple(t.shape)}")
+    raise ValueError(f"{what} must have adjacent columns and rows that do not overlap, got strides {t.stride()}")
 
 
-def flat(t: torch.Tensor, what: str, dtype: torch.dtype, shape) -> None:
+def flat(t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple) -> None:
     """``t`` is a contiguous tensor of exactly this type and shape."""
-    need(isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) == tuple(shape) and contiguous(t),
-         f"{what} must be a contiguous {dtype} {tuple(shape)}"
-         + (f", got {t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""))
+    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_contiguous()):
+        got = f", got {t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""
+        raise ValueError(f"{what} must be a contiguous {dtype} {tuple(shape)}{got}")
 
 
-def out_or_new(out: Optional[torch.Tensor], shape, dtype, device, what: str = "out") -> torch.Tensor:
+def out_or_new(out: Optional[torch.Tensor], M: int, N: int, dtype, device, what: str = "out") -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    rows2d(out, what, (dtype,), *shape)
+        return torch.empty(M, N, dtype=dtype, device=device)
+    rows2d(out, what, (dtype,), M, N)
     return out
 
 
@@ -85,5 +88,6 @@ def launch(what: str, *tensors):
     if dev.type != "cuda":
         raise ValueError(f"{what} runs on the GPU: operands are on {dev}")
     if dev.index == torch.cuda.current_device():
-        return _Here(torch.cuda.current_stream().cuda_stream)
+        # (the handle itself: torch.cuda.current_stream() takes 5 us to wrap it)
+        return _Here(torch._C._cuda_getCurrentRawStream(dev.index))
     return _on(dev)

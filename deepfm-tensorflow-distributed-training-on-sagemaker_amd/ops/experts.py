@@ -37,8 +37,8 @@ import torch
 
 from . import _lib
 from ._lib import ExchArgs, GroupNtArgs, GroupWgArgs, RouteArgs, RouteBwdArgs, check, ptr
-from .act8 import Act8, check_act8
-from .checks import flat, launch, need, out_or_new, row_stride, rows2d
+from .act8 import Act8, check_act8, check_own_act8
+from .checks import flat, launch, out_or_new, row_stride, rows2d
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 16
@@ -66,22 +66,28 @@ def _bf(t) -> int:
 def _check_gate(logits, top_k):
     rows2d(logits, "logits", _VALUES)
     T, E = logits.shape
-    need(1 <= E <= MAX_EXPERTS, f"1 to {MAX_EXPERTS} experts, got {E}")
-    need(isinstance(top_k, int) and 1 <= top_k <= min(E, MAX_TOP_K),
-         f"top_k must be 1 to {min(E, MAX_TOP_K)}, got {top_k}")
-    need(T * top_k <= _MAX_SLOTS, f"{T} x {top_k} slots are more than {_MAX_SLOTS}")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, got {E}")
+    if not (isinstance(top_k, int) and 1 <= top_k <= min(E, MAX_TOP_K)):
+        raise ValueError(f"top_k must be 1 to {min(E, MAX_TOP_K)}, got {top_k}")
+    if T * top_k > _MAX_SLOTS:
+        raise ValueError(f"{T} x {top_k} slots are more than {_MAX_SLOTS}")
     return T, E
 
 
 def _check_routes(r: Routes, T: Optional[int] = None) -> Tuple[int, int]:
-    need(isinstance(r, Routes), "routes must be a Routes")
-    need(r.expert.dim() == 2 and 1 <= r.expert.shape[1] <= MAX_TOP_K, f"routes.expert must be [T, 1 to {MAX_TOP_K}]")
-    n, k = r.expert.shape
-    need(T is None or n == T, f"routes are of {n} tokens, the rows of {T}")
-    need(n * k <= _MAX_SLOTS, "too many slots")
-    flat(r.expert, "routes.expert", torch.int32, (n, k))
-    flat(r.weight, "routes.weight", torch.float32, (n, k))
-    flat(r.pos, "routes.pos", torch.int32, (n, k))
+    if not isinstance(r, Routes):
+        raise ValueError("routes must be a Routes")
+    if r.expert.dim() != 2 or not 1 <= r.expert.shape[1] <= MAX_TOP_K:
+        raise ValueError(f"routes.expert must be [T, 1 to {MAX_TOP_K}]")
+    n, k = shape = r.expert.shape
+    if T is not None and n != T:
+        raise ValueError(f"routes are of {n} tokens, the rows of {T}")
+    if n * k > _MAX_SLOTS:
+        raise ValueError(f"{n} x {k} slots are more than {_MAX_SLOTS}")
+    flat(r.expert, "routes.expert", torch.int32, shape)
+    flat(r.weight, "routes.weight", torch.float32, shape)
+    flat(r.pos, "routes.pos", torch.int32, shape)
     flat(r.src, "routes.src", torch.int32, (n * k,))
     return n, k
 
@@ -101,11 +107,13 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, valid: Opt
         out = Routes(torch.empty(T, top_k, **i32), torch.empty(T, top_k, dtype=torch.float32, device=dev),
                      torch.empty(T, top_k, **i32), torch.empty(T * top_k, **i32), torch.empty(E + 1, **i32))
     else:
-        need(_check_routes(out, T)[1] == top_k, "out has another top_k")
+        if _check_routes(out, T)[1] != top_k:
+            raise ValueError("out has another top_k")
         flat(out.offs, "out.offs", torch.int32, (E + 1,))
     with launch("route", logits, valid, *out) as st:
         lib = _lib.get_lib()
-        ws = torch.empty(lib.hfm_route_ws_ints(T, E), dtype=torch.int32, device=dev)
+        n = lib.hfm_route_ws_ints(T, E)
+        ws = torch.empty(n, dtype=torch.int32, device=dev) if n else None
         a = RouteArgs(ptr(logits), ptr(valid), *(ptr(t) for t in out), ptr(ws), 0, row_stride(logits), T, E, top_k,
                       1 if renormalize else 0, _bf(logits), 0, 0)
         check(lib.hfm_route(C.byref(a), st), "route")
@@ -120,7 +128,7 @@ def route_bwd(logits: torch.Tensor, routes: Routes, dweight: torch.Tensor, renor
     T, k = _check_routes(routes, logits.shape[0])
     _, E = _check_gate(logits, k)
     flat(dweight, "dweight", torch.float32, (T, k))
-    out = out_or_new(out, (T, E), logits.dtype, logits.device)
+    out = out_or_new(out, T, E, logits.dtype, logits.device)
     a = RouteBwdArgs(ptr(logits), ptr(routes.expert), ptr(routes.weight), ptr(dweight), ptr(out),
                      row_stride(logits), row_stride(out), T, E, k, 1 if renormalize else 0, _bf(logits))
     with launch("route_bwd", logits, *routes, dweight, out) as st:
@@ -140,7 +148,7 @@ def dispatch(x: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None
     rows2d(x, "x", _VALUES)
     T, k = _check_routes(routes, x.shape[0])
     D = x.shape[1]
-    out = out_or_new(out, (T * k, D), x.dtype, x.device)
+    out = out_or_new(out, T * k, D, x.dtype, x.device)
     _exchange(_EX_DISPATCH, "dispatch", x, None, out, routes, None, None, T, k, D, T * k)
     return out
 
@@ -150,8 +158,9 @@ def dispatch_bwd(dxs: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] 
     rows2d(dxs, "dxs", _VALUES)
     T, k = _check_routes(routes)
     D = dxs.shape[1]
-    need(dxs.shape[0] == T * k, f"dxs must have {T * k} rows, got {dxs.shape[0]}")
-    out = out_or_new(out, (T, D), dxs.dtype, dxs.device)
+    if dxs.shape[0] != T * k:
+        raise ValueError(f"dxs must have {T * k} rows, got {dxs.shape[0]}")
+    out = out_or_new(out, T, D, dxs.dtype, dxs.device)
     _exchange(_EX_DISPATCH_BWD, "dispatch_bwd", dxs, None, out, routes, None, None, T, k, D, T * k)
     return out
 
@@ -162,8 +171,9 @@ def combine(ys: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None
     rows2d(ys, "ys", _VALUES)
     T, k = _check_routes(routes)
     D = ys.shape[1]
-    need(ys.shape[0] == T * k, f"ys must have {T * k} rows, got {ys.shape[0]}")
-    out = out_or_new(out, (T, D), ys.dtype, ys.device)
+    if ys.shape[0] != T * k:
+        raise ValueError(f"ys must have {T * k} rows, got {ys.shape[0]}")
+    out = out_or_new(out, T, D, ys.dtype, ys.device)
     _exchange(_EX_COMBINE, "combine", ys, None, out, routes, routes.weight, None, T, k, D, T * k)
     return out
 
@@ -175,7 +185,7 @@ def combine_bwd(dy: torch.Tensor, ys: torch.Tensor, routes: Routes,
     T, k = _check_routes(routes, dy.shape[0])
     D = dy.shape[1]
     rows2d(ys, "ys", (dy.dtype,), T * k, D)
-    out = out_or_new(out, (T * k, D), dy.dtype, dy.device)
+    out = out_or_new(out, T * k, D, dy.dtype, dy.device)
     dweight = torch.empty(T, k, dtype=torch.float32, device=dy.device)
     _exchange(_EX_COMBINE_BWD, "combine_bwd", dy, ys, out, routes, routes.weight, dweight, T, k, D, T * k)
     return out, dweight
@@ -187,21 +197,27 @@ def _check_groups(offs, E):
 
 
 def _check_gather(src, top_k, S):
-    need(isinstance(top_k, int) and top_k >= 1, f"top_k must be a positive int, got {top_k}")
+    if not (isinstance(top_k, int) and top_k >= 1):
+        raise ValueError(f"top_k must be a positive int, got {top_k}")
     if src is not None:
         flat(src, "src", torch.int32, (S,))
-    else:
-        need(top_k == 1, "top_k without src")
+    elif top_k != 1:
+        raise ValueError("top_k without src")
 
 
-def _check_weight(w, what, E=None, N=None, K=None):
-    need(isinstance(w, torch.Tensor) and w.dim() == 3 and w.dtype == torch.bfloat16, f"{what} must be a 3-D bf16 tensor")
-    need((E is None or w.shape[0] == E) and (N is None or w.shape[1] == N) and (K is None or w.shape[2] == K),
-         f"{what} must be [{E or 'E'}, {N or 'N'}, {K or 'K'}], got {tuple(w.shape)}")
-    need(w.shape[0] >= 1, f"{what} has no experts")
-    if w.numel():
-        need(w.shape[2] == 1 or w.stride(2) == 1, f"{what}'s last axis must be adjacent")
-        need(w.stride(1) >= 0 and w.stride(0) >= 0, f"{what} has negative strides")
+def _check_weight(w, what, K):
+    if not (isinstance(w, torch.Tensor) and w.dim() == 3 and w.dtype == torch.bfloat16):
+        raise ValueError(f"{what} must be a 3-D bf16 tensor")
+    e, n, k = w.shape
+    if k != K or e < 1:
+        raise ValueError(f"{what} must be [1 or more, any, {K}], got {tuple(w.shape)}")
+    if w.numel() and ((k != 1 and w.stride(2) != 1) or w.stride(1) < 0 or w.stride(0) < 0):
+        raise ValueError(f"{what}'s last axis must be adjacent, got strides {w.stride()}")
+
+
+def _check_out_type(dtype):
+    if dtype not in _VALUES:
+        raise ValueError(f"out must be bf16 or fp32, not {dtype}")
 
 
 def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], offs: torch.Tensor,
@@ -212,7 +228,7 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     [S]) row(p) = src[p] // top_k, the token of the slot; an entry of ``src`` that is no slot of a row
     of x reads as a row of zeros.  Without ``src``, S is x's rows."""
     rows2d(x, "x", _BF)
-    _check_weight(w, "w", K=x.shape[1])
+    _check_weight(w, "w", x.shape[1])
     E, N, K = w.shape
     _check_groups(offs, E)
     S = x.shape[0] if src is None else src.shape[0]
@@ -221,8 +237,8 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
         flat(bias, "bias", torch.float32, (E, N))
     if out is not None:
         out_dtype = out.dtype
-    need(out_dtype in _VALUES, f"out must be bf16 or fp32, not {out_dtype}")
-    out = out_or_new(out, (S, N), out_dtype, x.device)
+    _check_out_type(out_dtype)
+    out = out_or_new(out, S, N, out_dtype, x.device)
     a = GroupNtArgs(ptr(x), ptr(w), ptr(bias), 0, ptr(out), ptr(offs), ptr(src), row_stride(x), w.stride(1),
                     w.stride(0), 0, row_stride(out), S, x.shape[0], K, N, E, top_k, 1 if relu else 0, 0,
                     0 if _bf(out) else 1, 1.0)
@@ -239,7 +255,7 @@ def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
     zero.  dz bf16 [S, N]; ``wt`` bf16 [E, K, N] is the transposed copy of w."""
     rows2d(dz, "dz", _BF)
     S = dz.shape[0]
-    _check_weight(wt, "wt", K=dz.shape[1])
+    _check_weight(wt, "wt", dz.shape[1])
     E, K, N = wt.shape
     _check_groups(offs, E)
     m, ldm, m8 = None, 0, 0
@@ -251,8 +267,8 @@ def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
         m, ldm = mask, row_stride(mask)
     if out is not None:
         out_dtype = out.dtype
-    need(out_dtype in _VALUES, f"out must be bf16 or fp32, not {out_dtype}")
-    out = out_or_new(out, (S, K), out_dtype, dz.device)
+    _check_out_type(out_dtype)
+    out = out_or_new(out, S, K, out_dtype, dz.device)
     a = GroupNtArgs(ptr(dz), ptr(wt), 0, ptr(m), ptr(out), ptr(offs), 0, row_stride(dz), wt.stride(1), wt.stride(0),
                     ldm, row_stride(out), S, S, N, K, E, 1, 0, m8, 0 if _bf(out) else 1, float(scale))
     with launch("group_dgrad", dz, wt, offs, m, out) as st:
@@ -272,17 +288,18 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
     S, N = dz.shape
     x8 = isinstance(x, Act8)
     if x8:
-        need(x.codes.dim() == 2, "x.codes must be 2-D")
-        check_act8(x, x.codes.shape[0], x.codes.shape[1], "x")
+        check_own_act8(x, "x")
     else:
         rows2d(x, "x", _BF)
     xv = x.codes if x8 else x
     K = xv.shape[1]
-    need(isinstance(offs, torch.Tensor) and offs.dim() == 1 and offs.shape[0] >= 2, "offs must be int32 [E + 1]")
+    if not (isinstance(offs, torch.Tensor) and offs.dim() == 1 and offs.shape[0] >= 2):
+        raise ValueError("offs must be int32 [E + 1]")
     E = offs.shape[0] - 1
     _check_groups(offs, E)
     _check_gather(src, top_k, S)
-    need(src is not None or xv.shape[0] == S, f"x must have {S} rows, got {xv.shape[0]}")
+    if src is None and xv.shape[0] != S:
+        raise ValueError(f"x must have {S} rows, got {xv.shape[0]}")
     if out is None:
         dw = torch.empty(E, N, K, dtype=torch.float32, device=dz.device)
         db = torch.empty(E, N, dtype=torch.float32, device=dz.device) if bias else None
