@@ -127,6 +127,21 @@ __device__ __forceinline__ uint2 load8_code(const uint8_t* row, int c, int n) {
   return v;
 }
 
+// One output of the NT product: scale, bias, relu (NaN stays), mask, rounding.
+__device__ __forceinline__ void group_put(const GroupNtArgs& g, int p, int n, float acc, float bias) {
+  float v = acc * g.scale + bias;
+  if (g.relu && v < 0.f) v = 0.f;
+  if (g.mask) {
+    const size_t m = (size_t)p * g.ldm + n;
+    const bool on = g.mask8 ? a8_positive(reinterpret_cast<const uint8_t*>(g.mask)[m])
+                            : bf2f(reinterpret_cast<const bf16*>(g.mask)[m]) > 0.f;
+    if (!on) v = 0.f;
+  }
+  const size_t o = (size_t)p * g.ldo + n;
+  if (g.out_f32) reinterpret_cast<float*>(g.out)[o] = v;
+  else reinterpret_cast<bf16*>(g.out)[o] = f2bf(v);
+}
+
 // ------------------------------------------------------------------ NT product, 128 x 128 tile
 // 256 threads = 4 waves of 64 x 64 outputs (4 x 4 MFMA 16x16x32), 64-deep steps through two LDS
 // buffers of 32 KB: the next step's 16-byte row chunks are in registers while this one multiplies.
@@ -211,19 +226,50 @@ __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int p = r0 + wr + i * 16 + fq * 4 + q;
-        if (p >= r1) continue;
-        float v = acc[i][j][q] * g.scale + bias;
-        if (g.relu && v < 0.f) v = 0.f;        // (NaN stays)
-        if (g.mask) {
-          const size_t m = (size_t)p * g.ldm + n;
-          const bool on = g.mask8 ? a8_positive(reinterpret_cast<const uint8_t*>(g.mask)[m])
-                                  : bf2f(reinterpret_cast<const bf16*>(g.mask)[m]) > 0.f;
-          if (!on) v = 0.f;
-        }
-        const size_t o = (size_t)p * g.ldo + n;
-        if (g.out_f32) reinterpret_cast<float*>(g.out)[o] = v;
-        else reinterpret_cast<bf16*>(g.out)[o] = f2bf(v);
+        if (p < r1) group_put(g, p, n, acc[i][j][q], bias);
       }
+  }
+}
+
+// ------------------------------------------------------------------ NT product, few rows
+// 32 x 32 outputs of a workgroup whose 8 waves share the reduction: wave w takes the 16-deep steps w, w + 8, ...
+// (together they read 256 neighbouring bytes of a row), fragments straight from memory, 8 steps under way at
+// once, and the 8 partial tiles are summed through LDS.  A request's rows leave a larger tile with a
+// handful of workgroups that go through the whole reduction one after another: 192 rows, 8 experts,
+// 1248 -> 400: 25 us by the 128 x 128 tile, 6.2 here.  Where rows and columns have 16-byte chunks.
+constexpr int GS_B = 32, GS_WAVES = 8, GS_DEEP = 8;
+__global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs g, int tiles_n) {
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  __shared__ float part[GS_WAVES][GS_B][GS_B + 1];
+  int e, r0, r1;
+  if (!group_find<GS_B>(g.offs, g.E, g.S, blockIdx.x / tiles_n, e, r0, r1)) return;
+  const int n0 = (blockIdx.x % tiles_n) * GS_B;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, fr = lane & 31, fq = lane >> 5;
+  const int row = r0 + fr < r1 ? group_row(g.src, r0 + fr, g.rows, g.top_k) : -1;
+  const bf16* a = row >= 0 ? g.a + (size_t)row * g.lda : nullptr;
+  const bf16* b = n0 + fr < g.N ? g.b + (size_t)e * g.es + (size_t)(n0 + fr) * g.ldb : nullptr;
+  f32x16 acc = {};
+  for (int k0 = wave * 16 + fq * 8; k0 - fq * 8 < g.K; k0 += GS_DEEP * GS_WAVES * 16) {
+    bf16x8 fa[GS_DEEP], fb[GS_DEEP];
+#pragma unroll
+    for (int i = 0; i < GS_DEEP; ++i) {
+      fa[i] = load8_bf<true>(a, k0 + i * GS_WAVES * 16, g.K);
+      fb[i] = load8_bf<true>(b, k0 + i * GS_WAVES * 16, g.K);
+    }
+#pragma unroll
+    for (int i = 0; i < GS_DEEP; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[i], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int q = 0; q < 16; ++q) part[wave][(q >> 2) * 8 + fq * 4 + (q & 3)][fr] = acc[q];
+  __syncthreads();
+  const int r = threadIdx.x >> 4, p = r0 + r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = (threadIdx.x & 15) * 2 + i, n = n0 + c;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < GS_WAVES; ++w) v += part[w][r][c];
+    if (p < r1 && n < g.N) group_put(g, p, n, v, g.bias ? g.bias[(size_t)e * g.N + n] : 0.f);
   }
 }
 
@@ -599,7 +645,7 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   if (vec && pairs && near && g.K >= 64) {
     // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
     // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
-    // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 192: MEASURED).
+    // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 117 at 192).
     const int tn = (g.N + GP_B - 1) / GP_B;
     const double step = 0.85 / 256 * ((g.K + GP_K - 1) / GP_K);
     auto cost = [&](int rows) {
@@ -616,6 +662,17 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   }
   const int tn = (g.N + GN_B - 1) / GN_B;
   const long blocks = (long)(g.S / GN_B + g.E) * tn;      // (each group adds less than one tile)
+  // Few rows: a 128 x 128 tile's workgroup takes 1.4 us for each of its 64-deep steps, two at a time on a CU;
+  // the 32 x 32 tiles' operands come from the L2s at 8 TB/s or so.  32 x 32 against 128 x 128 in us: 32 rows,
+  // 4096 -> 4096: 19, 60; 128 rows: 34, 66; 256 rows: 66, 66; 1024 rows: 262, 67; 1024 rows of 8 experts, 1024
+  // -> 1024: 20, 28; 2048: 35, 29; 5000 rows, 256 -> 1024: 35, 21; 8192 rows of 8 experts, 128 -> 64: 4.8, 17.
+  const int fn = (g.N + GS_B - 1) / GS_B;
+  const long few = (long)(g.S / GS_B + g.E) * fn;
+  if (vec && few <= 1l << 20 &&
+      few * g.K * (4.0 * GS_B / 8e6) < ceil(blocks / 512.0) * ((g.K + GN_K - 1) / GN_K) * 1.4) {
+    hipLaunchKernelGGL(group_nt_few_kernel, dim3((unsigned)few), dim3(GS_WAVES * 64), 0, st, g, fn);
+    HFM_LAUNCH_CHECK();
+  }
   if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
   if (vec) hipLaunchKernelGGL(group_nt_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
   else hipLaunchKernelGGL(group_nt_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
