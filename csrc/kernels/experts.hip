@@ -379,9 +379,12 @@ HFM_API int hfm_route_args_bytes() { return (int)sizeof(RouteArgs); }
 HFM_API int hfm_route_bwd_args_bytes() { return (int)sizeof(RouteBwdArgs); }
 
 // ------------------------------------------------------------------ exchange
-// One wave per token, V elements (16 bytes where the rows allow it) per lane and turn; a token's row
-// is read once for all its slots (dispatch, combine_bwd), or its slots' rows summed in order
-// (combine, dispatch_bwd).  Bound by the rows' bytes.
+// One wave per token, 16 bytes per lane and turn, a row's last elements (fewer than 16 bytes) one by one;
+// a token's row is read once for all its slots (dispatch, combine_bwd), or its slots' rows summed in
+// order (combine, dispatch_bwd).  Bound by the rows' bytes.  A 16-byte access of global memory may start at
+// any element: rows of an odd width take the same accesses as aligned ones (10007 rows of 313 floats with
+// 4 slots, the four exchanges: 88 us, 95 with single elements, 3 TB/s; 16384 rows of 1248 bf16 with 2 slots: 118
+// us, 4.2 TB/s).
 struct ExchArgs {
   const void* a;           // x / dxs / ys / dy
   const void* b;           // combine_bwd: ys
@@ -391,41 +394,79 @@ struct ExchArgs {
   float* dweight;          // [T, k] (combine_bwd)
   long lda, ldb, ldo;      // row strides in elements
   int T, k, D, S;          // S: rows of the expert order
-  int bf, vec;             // vec: elements per access (8 / 4 for 16 bytes, or 1)
+  int bf;                  // bf16 rows (else fp32)
 };
 
 template <typename T, int V>
-struct RowVec {
-  typedef T type __attribute__((ext_vector_type(V)));
-};
-template <typename T>
-struct RowVec<T, 1> {
-  typedef T type;
+struct RowVec {               // (aligned to an element only)
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
 template <typename T, int V>
 __device__ __forceinline__ void row_load(const T* p, float (&f)[V]) {
   typename RowVec<T, V>::type v = *reinterpret_cast<const typename RowVec<T, V>::type*>(p);
-  if constexpr (V == 1) f[0] = (float)v;
-  else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = (float)v[i];
-  }
+  for (int i = 0; i < V; ++i) f[i] = (float)v[i];
 }
 template <typename T, int V>
 __device__ __forceinline__ void row_store(T* p, const float (&f)[V]) {
   typename RowVec<T, V>::type v;
-  if constexpr (V == 1) v = (T)f[0];
-  else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (T)f[i];
-  }
+  for (int i = 0; i < V; ++i) v[i] = (T)f[i];
   *reinterpret_cast<typename RowVec<T, V>::type*>(p) = v;
 }
 
 enum { EX_DISPATCH = 0, EX_DISPATCH_BWD = 1, EX_COMBINE = 2, EX_COMBINE_BWD = 3 };
 
+// Columns c .. c + V - 1 of token t's rows.
 template <typename T, int V, int K, int MODE>
+__device__ __forceinline__ void exchange_cols(const ExchArgs& a, int t, int c, const int (&p)[K], const float (&w)[K],
+                                              float (&dot)[K]) {
+  const T* A = reinterpret_cast<const T*>(a.a);
+  const T* B = reinterpret_cast<const T*>(a.b);
+  T* O = reinterpret_cast<T*>(a.out);
+  if (MODE == EX_DISPATCH) {
+    typedef typename RowVec<T, V>::type vec;
+    const vec v = *reinterpret_cast<const vec*>(A + (size_t)t * a.lda + c);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (p[j] >= 0) *reinterpret_cast<vec*>(O + (size_t)p[j] * a.ldo + c) = v;
+  } else if (MODE == EX_COMBINE_BWD) {
+    float g[V], y[K][V];
+    row_load<T, V>(A + (size_t)t * a.lda + c, g);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (p[j] >= 0) row_load<T, V>(B + (size_t)p[j] * a.ldb + c, y[j]);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (p[j] >= 0) {
+        float d[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          d[i] = w[j] * g[i];
+          dot[j] = fmaf(g[i], y[j][i], dot[j]);
+        }
+        row_store<T, V>(O + (size_t)p[j] * a.ldo + c, d);
+      }
+  } else {
+    float s[V], y[K][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (p[j] >= 0) row_load<T, V>(A + (size_t)p[j] * a.lda + c, y[j]);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (p[j] >= 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = MODE == EX_COMBINE ? fmaf(w[j], y[j][i], s[i]) : s[i] + y[j][i];
+      }
+    row_store<T, V>(O + (size_t)t * a.ldo + c, s);
+  }
+}
+
+template <typename T, int K, int MODE>
 __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
+  constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
@@ -438,49 +479,9 @@ __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
     w[j] = MODE == EX_COMBINE || MODE == EX_COMBINE_BWD ? (j < a.k ? a.weight[(size_t)t * a.k + j] : 0.f) : 1.f;
     dot[j] = 0.f;
   }
-  const T* A = reinterpret_cast<const T*>(a.a);
-  const T* B = reinterpret_cast<const T*>(a.b);
-  T* O = reinterpret_cast<T*>(a.out);
-  for (int c = lane * V; c < a.D; c += 64 * V) {
-    if (MODE == EX_DISPATCH) {
-      typedef typename RowVec<T, V>::type vec;
-      const vec v = *reinterpret_cast<const vec*>(A + (size_t)t * a.lda + c);
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (p[j] >= 0) *reinterpret_cast<vec*>(O + (size_t)p[j] * a.ldo + c) = v;
-    } else if (MODE == EX_COMBINE_BWD) {
-      float g[V], y[K][V];
-      row_load<T, V>(A + (size_t)t * a.lda + c, g);
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (p[j] >= 0) row_load<T, V>(B + (size_t)p[j] * a.ldb + c, y[j]);
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (p[j] >= 0) {
-          float d[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            d[i] = w[j] * g[i];
-            dot[j] = fmaf(g[i], y[j][i], dot[j]);
-          }
-          row_store<T, V>(O + (size_t)p[j] * a.ldo + c, d);
-        }
-    } else {
-      float s[V], y[K][V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (p[j] >= 0) row_load<T, V>(A + (size_t)p[j] * a.lda + c, y[j]);
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (p[j] >= 0) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) s[i] = MODE == EX_COMBINE ? fmaf(w[j], y[j][i], s[i]) : s[i] + y[j][i];
-        }
-      row_store<T, V>(O + (size_t)t * a.ldo + c, s);
-    }
-  }
+  const int D16 = a.D / V * V;
+  for (int c = lane * V; c < D16; c += 64 * V) exchange_cols<T, V, K, MODE>(a, t, c, p, w, dot);
+  if (D16 + lane < a.D) exchange_cols<T, 1, K, MODE>(a, t, D16 + lane, p, w, dot);
   if (MODE == EX_COMBINE_BWD) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
@@ -490,35 +491,26 @@ __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
   }
 }
 
-template <typename T, int V, int MODE>
+template <typename T, int MODE>
 static void exchange_k(const ExchArgs& a, hipStream_t st) {
   const dim3 grid((a.T + 3) / 4), blk(256);
-  if (a.k <= 1) hipLaunchKernelGGL((exchange_kernel<T, V, 1, MODE>), grid, blk, 0, st, a);
-  else if (a.k <= 2) hipLaunchKernelGGL((exchange_kernel<T, V, 2, MODE>), grid, blk, 0, st, a);
-  else if (a.k <= 4) hipLaunchKernelGGL((exchange_kernel<T, V, 4, MODE>), grid, blk, 0, st, a);
-  else if (a.k <= 8) hipLaunchKernelGGL((exchange_kernel<T, V, 8, MODE>), grid, blk, 0, st, a);
-  else hipLaunchKernelGGL((exchange_kernel<T, V, 16, MODE>), grid, blk, 0, st, a);
+  if (a.k <= 1) hipLaunchKernelGGL((exchange_kernel<T, 1, MODE>), grid, blk, 0, st, a);
+  else if (a.k <= 2) hipLaunchKernelGGL((exchange_kernel<T, 2, MODE>), grid, blk, 0, st, a);
+  else if (a.k <= 4) hipLaunchKernelGGL((exchange_kernel<T, 4, MODE>), grid, blk, 0, st, a);
+  else if (a.k <= 8) hipLaunchKernelGGL((exchange_kernel<T, 8, MODE>), grid, blk, 0, st, a);
+  else hipLaunchKernelGGL((exchange_kernel<T, 16, MODE>), grid, blk, 0, st, a);
 }
 
 template <int MODE>
 static void exchange_mode(const ExchArgs& a, hipStream_t st) {
-  if (a.bf) {
-    if (a.vec > 1) exchange_k<bf16, 8, MODE>(a, st);
-    else exchange_k<bf16, 1, MODE>(a, st);
-  } else {
-    if (a.vec > 1) exchange_k<float, 4, MODE>(a, st);
-    else exchange_k<float, 1, MODE>(a, st);
-  }
+  if (a.bf) exchange_k<bf16, MODE>(a, st);
+  else exchange_k<float, MODE>(a, st);
 }
 
 HFM_API int hfm_exchange(int mode, const ExchArgs* ap, hipStream_t st) {
-  ExchArgs a = *ap;
+  const ExchArgs& a = *ap;
   if (a.T < 0 || a.k < 1 || a.k > RT_MAXK || a.D < 0) return (int)hipErrorInvalidValue;
   if (a.T == 0) return 0;
-  // 16-byte accesses where every row of every operand starts on 16 bytes and ends on them
-  const int per = a.bf ? 8 : 4;
-  const uintptr_t at = (uintptr_t)a.a | (uintptr_t)a.b | (uintptr_t)a.out;
-  a.vec = (at % 16 == 0 && a.D % per == 0 && a.lda % per == 0 && a.ldb % per == 0 && a.ldo % per == 0) ? per : 1;
   switch (mode) {
     case EX_DISPATCH: exchange_mode<EX_DISPATCH>(a, st); break;
     case EX_DISPATCH_BWD: exchange_mode<EX_DISPATCH_BWD>(a, st); break;

@@ -219,7 +219,7 @@ class RouteBwdArgs(C.Structure):
 class ExchArgs(C.Structure):
     _fields_ = [("a", c_void_p), ("b", c_void_p), ("out", c_void_p), ("pos", c_void_p), ("weight", c_void_p),
                 ("dweight", c_void_p), ("lda", c_long), ("ldb", c_long), ("ldo", c_long), ("T", c_int),
-                ("k", c_int), ("D", c_int), ("S", c_int), ("bf", c_int), ("vec", c_int)]
+                ("k", c_int), ("D", c_int), ("S", c_int), ("bf", c_int)]
 
 
 class Act8Args(C.Structure):

@@ -138,7 +138,7 @@ def route_bwd(logits: torch.Tensor, routes: Routes, dweight: torch.Tensor, renor
 
 def _exchange(mode, what, a, b, out, r: Routes, weight, dweight, T, k, D, S):
     args = ExchArgs(ptr(a), ptr(b), ptr(out), ptr(r.pos), ptr(weight), ptr(dweight), row_stride(a),
-                    row_stride(b) if b is not None else 0, row_stride(out), T, k, D, S, _bf(a), 0)
+                    row_stride(b) if b is not None else 0, row_stride(out), T, k, D, S, _bf(a))
     with launch(what, a, b, out, r.pos, weight, dweight) as st:
         check(_lib.get_lib().hfm_exchange(mode, C.byref(args), st), what)
 
