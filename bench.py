@@ -214,6 +214,8 @@ def main():
     ap.add_argument("--embedding_mode", default="auto")
     ap.add_argument("--mlp_dtype", default="bf16", choices=["bf16", "fp8"],
                     help="deep-tower forward GEMM operands (fp8 = OCP e4m3 MFMA, config #5)")
+    ap.add_argument("--act_dtype", default="bf16", choices=["bf16", "fp8"],
+                    help="activations a per-layer tower keeps for its backward pass (fp8 = e4m3 codes and scales)")
     ap.add_argument("--exchange_rows", default="fp32", choices=["fp32", "bf16"],
                     help="row-sharded exchange (N > 1): fp32 served rows (the default, the library's "
                          "and the reference's precision: bitwise the one-GPU reads) or bf16 v (a "
@@ -298,7 +300,7 @@ def main():
                          sparse_update=args.sparse_update, seed=1234, batch_size=B, device=dev,
                          comm=comm, field_ranges=synth.field_ranges(), mlp_dtype=args.mlp_dtype,
                          emb_dtype=args.emb_dtype, exchange_rows=args.exchange_rows,
-                         batch_norm=args.batch_norm)
+                         batch_norm=args.batch_norm, act_dtype=args.act_dtype)
     _progress()
     if args.field_major_ids:
         # ids stored field-major ([F, B] storage, [B, F] view: the layout the Estimator's HBM
@@ -453,6 +455,7 @@ def main():
                 "exec": os.environ.get("HIPFM_BENCH_RUNG", ("graph+run-sort" if os.environ.get("HIPFM_RUN_SORT", "1") == "1"
                                                               else "graph+prefetch") if use_graph else "eager"),
                 "mlp_dtype": args.mlp_dtype + (" fwd GEMMs, bf16 backward" if args.mlp_dtype == "fp8" else ""),
+                **({"act_dtype": "fp8 checkpoints"} if args.act_dtype == "fp8" else {}),
                 "emb_dtype": args.emb_dtype + (" rows + slots (stochastic rounding), fp32 math"
                                                if args.emb_dtype == "bf16" else " tables + slots"),
                 "ids_layout": "field-major [F, B]" if args.field_major_ids else "row-major [B, F]",

@@ -1150,7 +1150,7 @@ struct HeadArgs {
   float* logit;         // [M] (nullable)
   float* dlogit;        // [M]
   bf16* dz;             // [M, L]
-  bf16* dz_t;           // [L, M]
+  bf16* dz_t;           // [L, M] (nullable)
   float* partial;       // [gridDim.x, L + 2]
   float* dh;            // batch-norm towers: raw dL/dh_L = dlogit * w_out, f32 [M, L] (the BN
                         // backward applies dropout/ReLU itself); dz/dz_t are then unused
@@ -1217,7 +1217,7 @@ __global__ void __launch_bounds__(256) head_kernel(HeadArgs a) {
           const int col = q * Q + j + t;
           const float g = hv[j + t] > 0.f ? dl * a.w_out[col] * a.scale_l : 0.f;
           pk[t] = f2bf(g);
-          a.dz_t[(size_t)col * a.M + b] = pk[t];
+          if (a.dz_t) a.dz_t[(size_t)col * a.M + b] = pk[t];
         }
         *reinterpret_cast<bf16x8*>(dzr + j) = pk;
       }
@@ -1322,7 +1322,7 @@ __global__ void __launch_bounds__(256) head_wide_kernel(HeadArgs a) {
         }
         col[j] = f2bf(v);
       }
-      if (a.train && !a.dh) {
+      if (a.train && !a.dh && a.dz_t) {
         if (full) {
           *reinterpret_cast<bf16x8*>(a.dz_t + (size_t)c * a.M + bb + g * 8) = col;
         } else {
@@ -1471,7 +1471,7 @@ __global__ void __launch_bounds__(256) head_wide_bwd_kernel(HeadArgs a) {
       }
     }
   }
-  if (!a.dh) {
+  if (!a.dh && a.dz_t) {
     const int r0 = bb + rg * 8;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

@@ -91,6 +91,8 @@ _DEFS = [
     ("sparse_update", str, "tf1_dense", "tf1_dense (reference non-lazy semantics: every row moves "
      "every step, full-table L2) | lazy (touched rows only)"),
     ("mlp_dtype", str, "bf16", "bf16 | fp8 (deep-part GEMM input precision; accumulation is fp32)"),
+    ("act_dtype", str, "bf16", "bf16 | fp8: the deep part's activations as kept for the backward pass (fp8: "
+     "e4m3 with a power-of-two scale per row and 32 columns; per-layer towers without batch norm)"),
     ("emb_dtype", str, "fp32", "fp32 | bf16: fm_v rows + their optimizer slots (bf16: stochastic "
      "rounding, lazy updates, gather-fused tower; config #5 mixed-precision embeddings)"),
     ("save_checkpoints_steps", int, 0, "checkpoint every N steps (0: use save_checkpoints_secs)"),
@@ -165,6 +167,7 @@ class RunConfig:
     embedding_mode: str = "auto"
     sparse_update: str = "tf1_dense"
     mlp_dtype: str = "bf16"
+    act_dtype: str = "bf16"
     emb_dtype: str = "fp32"
     save_checkpoints_steps: int = 0
     save_checkpoints_secs: int = 600
@@ -224,6 +227,8 @@ class RunConfig:
             raise ValueError(f"unknown sparse_update {self.sparse_update!r}")
         if self.mlp_dtype not in ("bf16", "fp8"):
             raise ValueError(f"unknown mlp_dtype {self.mlp_dtype!r} (bf16 | fp8)")
+        if self.act_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"unknown act_dtype {self.act_dtype!r} (bf16 | fp8)")
         if self.emb_dtype not in ("fp32", "bf16"):
             raise ValueError(f"unknown emb_dtype {self.emb_dtype!r} (fp32 | bf16)")
         if self.schedule not in ("hvd", "ps"):

@@ -112,7 +112,8 @@ class Estimator:
                                       sparse_update=cfg.sparse_update, seed=cfg.seed,
                                       batch_size=cfg.batch_size, device=self.device, comm=self.comm,
                                       batch_norm=cfg.batch_norm, batch_norm_decay=cfg.batch_norm_decay,
-                                      mlp_dtype=cfg.mlp_dtype, emb_dtype=cfg.emb_dtype, field_ranges=ranges)
+                                      mlp_dtype=cfg.mlp_dtype, act_dtype=cfg.act_dtype, emb_dtype=cfg.emb_dtype,
+                                      field_ranges=ranges)
         else:
             from .models.reference import GoldenDeepFM
             self.model = GoldenDeepFM(cfg.feature_size, cfg.field_size, cfg.embedding_size, cfg.layers,

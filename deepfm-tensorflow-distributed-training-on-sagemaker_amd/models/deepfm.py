@@ -33,6 +33,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..ops import act8 as A8
 from ..ops import kernels as KN
 from .runner import GraphRunnerMixin, graph_capture  # noqa: F401  (graph_capture: re-exported)
 from .state import NativeStateMixin
@@ -150,7 +151,7 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
                  batch_norm_decay: float = 0.9, adam_epsilon: float = 1e-8,
                  adagrad_init: float = 1e-8, fused: Optional[bool] = None,
                  field_ranges: Optional[Sequence[Tuple[int, int]]] = None, mlp_dtype: str = "bf16",
-                 emb_dtype: str = "fp32", exchange_rows: Optional[str] = None):
+                 emb_dtype: str = "fp32", exchange_rows: Optional[str] = None, act_dtype: str = "bf16"):
         self.batch_norm = bool(batch_norm)
         # row-sharded exchange: the served rows carry v as bf16 (the compute dtype; owners keep fp32
         # master rows and optimizer state) or fp32 (bitwise the one-GPU step's reads)
@@ -163,6 +164,11 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
         # fp8: the deep tower's forward GEMMs take OCP e4m3 operands (per-row / per-channel
         # power-of-two scales, fp32 accumulation); backward and master weights stay bf16 / fp32
         self.fp8 = mlp_dtype == "fp8"
+        # fp8: the per-layer tower keeps its activations for the backward pass as e4m3 codes (ops/act8.py),
+        # 1.03 bytes each instead of 4 (H and its transpose), and multiplies straight from the codes
+        if act_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"act_dtype must be bf16 or fp8, got {act_dtype!r}")
+        self.act8 = act_dtype == "fp8"
         # mixed-precision embeddings (BASELINE config #5): fm_v rows and their optimizer slots
         # stored bf16 (stochastically rounded, counter-based: reproducible), fm_w and every
         # computation fp32 -- half the table bytes and traffic of the gather and the row update
@@ -210,6 +216,9 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
         self.d0 = F * K
         self.K0p = pad32(self.d0)
         self.Np = [pad32(L) for L in self.layers]
+        if self.act8 and (self.batch_norm or not self._per_layer_tower(fused)):
+            raise ValueError("act_dtype=fp8 runs on the per-layer tower without batch norm (the fused tower keeps no "
+                             "transposed copies to save; fused=False or HIPFM_FUSED_TOWER=0 selects the layers)")
         # a per-layer (unfused) tower with a wide first layer pads its input to 128 columns: the
         # layer-0 weight-gradient and dX0 GEMMs then tile on the LDS-staged 128 x 128 tile (at
         # K0p = 320 they ran on the 64 x 64 register tile: 0.75 of a 5.4 ms 4096x3 step,
@@ -527,10 +536,19 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
         if self.fp8:
             self.E8 = torch.zeros(M, K0p, dtype=torch.uint8, device=dev)
             self.sE = torch.ones(M, **f32)
-        self.H = [torch.zeros(M, n, **bf) for n in self.Np]
-        self.Ht = [torch.zeros(n, M, **bf) for n in self.Np]
-        self.dZ = [torch.zeros(M, n, **bf) for n in self.Np]
-        self.dZt = [torch.zeros(n, M, **bf) for n in self.Np]
+        if self.act8:
+            # H and dZ live for one layer (two buffers in turns); the codes stay until the backward pass
+            hb, zb = ([torch.zeros(M * max(self.Np), **bf) for _ in range(2)] for _ in range(2))
+            self.H = [hb[i % 2][:M * n].view(M, n) for i, n in enumerate(self.Np)]
+            self.dZ = [zb[i % 2][:M * n].view(M, n) for i, n in enumerate(self.Np)]
+            self.H8 = [A8.empty(M, n, dev) for n in self.Np[:-1]]
+            self.group_rows = torch.tensor([0, M], **i32)      # one group: every row
+            self.Ht = self.dZt = None
+        else:
+            self.H = [torch.zeros(M, n, **bf) for n in self.Np]
+            self.Ht = [torch.zeros(n, M, **bf) for n in self.Np]
+            self.dZ = [torch.zeros(M, n, **bf) for n in self.Np]
+            self.dZt = [torch.zeros(n, M, **bf) for n in self.Np]
         self.dX0 = torch.zeros(M, K0p, **bf)            # layer-1 input gradient (bf16)
         if getattr(self, "l0s", 0):                      # split gather + layer 0: fp32 partials
             self.l0z = torch.zeros(self.l0s, M, self.Np[0], **f32)
@@ -559,6 +577,9 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
                     s //= 2
                 self.wg_cfg.append((None, s))
                 continue
+            if self.act8:           # group_wgrad writes the final gradient and brings its own workspace
+                self.wg_cfg.append((None, 0))
+                continue
             t = LP._pick_tile(Mg, Ng, row_major_stream=False, Kd=Kd)
             if t not in (KN.TILE_LDS, KN.TILE_PP) and LP._LDS_GEMM and LP._lds_tile_ok(Mg, Ng, Kd, splitk=4):
                 t = KN.TILE_LDS     # (few output tiles, but the batch reduction splits 4+ ways)
@@ -578,7 +599,8 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
         # fp32 product scratch of the library-GEMM forward / dgrad (layers._epi_blas_ok)
         cn = [] if (self.fused or self.batch_norm) else (
             [self.Np[i] for i in range(len(self.layers)) if LP._epi_blas_ok(M, self.Np[i], self.Kp[i])]
-            + [self.Np[i - 1] for i in range(1, len(self.layers)) if LP._epi_blas_ok(M, self.Np[i - 1], self.Np[i])])
+            + [self.Np[i - 1] for i in range(1, len(self.layers))
+               if not self.act8 and LP._epi_blas_ok(M, self.Np[i - 1], self.Np[i])])
         self.cbuf = torch.empty(M * max(cn) if cn else 0, **f32)
         # sparse path
         n = M * F

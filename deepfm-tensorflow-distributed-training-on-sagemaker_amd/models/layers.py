@@ -10,6 +10,8 @@ from typing import Optional
 
 import torch
 
+from ..ops import act8 as A8
+from ..ops import experts as EX
 from ..ops import kernels as KN
 from ..ops._lib import BnArgs, EpiArgs, HeadArgs, RowSumJob, SlabJob
 from ..utils.knobs import flag
@@ -105,7 +107,7 @@ class LayerPathMixin:
             ep.drop = 1 if drop else 0
             ep.step = self.step.data_ptr()
             ep.out = self.H[i].data_ptr()
-            ep.out_t = self.Ht[i].data_ptr() if train else 0
+            ep.out_t = self.Ht[i].data_ptr() if train and not self.act8 else 0
             N = self.Np[i]
             if self.batch_norm:
                 ep.out, ep.out_t = self.Rb[i].data_ptr(), 0
@@ -121,6 +123,8 @@ class LayerPathMixin:
                 KN.gemm_nt(KN.EPI_FWD if train else KN.EPI_FWD_EVAL, _pick_tile(M, N, Kd=self.Kp[i]), X,
                            self.Kp[i], self.W16[i], self.Kp[i], M, N, self.Kp[i], 1, ep)
             X = self.H[i]
+            if train and self.act8 and i + 1 < len(self.layers):
+                A8.pack(X, out=self.H8[i])
         return idx, tv
 
     def _bn_args(self, i: int, B: int, drop: bool) -> BnArgs:
@@ -186,33 +190,53 @@ class LayerPathMixin:
         a.logit = 0
         a.dlogit = self.dlogit.data_ptr()
         a.dz = self.dZ[-1].data_ptr()
-        a.dz_t = self.dZt[-1].data_ptr()
+        a.dz_t = self.dZt[-1].data_ptr() if self.dZt is not None else 0
         a.partial = self.partial.data_ptr()
         a.dh = self.dH[-1].data_ptr() if (self.batch_norm and train) else 0
         KN.head(a)
 
     # ------------------------------------------------------------------ backward pieces
+    def _wgrad(self, i: int):
+        """Layer i's weight gradient from the transposed operands (bias: row sums of the finalize)."""
+        M = self.M
+        Xt = self.Et if i == 0 else self.Ht[i - 1]
+        t, s = self.wg_cfg[i]
+        ep = EpiArgs()
+        if self.wg_direct[i] and _WG_BLAS:
+            # a plain GEMM with nothing to fuse: bf16 operands, fp32 result written in place
+            go = self.dense_segs[f"Deep-part/mlp{i}/weights"].off
+            gw = self.g[go:go + self.Np[i] * self.Kp[i]].view(self.Np[i], self.Kp[i])
+            torch.mm(self.dZt[i], Xt.t(), out_dtype=torch.float32, out=gw)
+        else:
+            if self.wg_direct[i]:   # unsplit: the GEMM writes the final gradient itself
+                ep.out = self.g.data_ptr() + 4 * self.dense_segs[f"Deep-part/mlp{i}/weights"].off
+            else:
+                ep.out = self.slabs[i].data_ptr()
+            KN.gemm_nt(KN.EPI_F32, t, self.dZt[i], M, Xt, M, self.Np[i], self.Kp[i], M, s, ep)
+
+    def _wgrad_act8(self, i: int):
+        """Layer i's weight and bias gradients from rows of dZ and of E or the 8-bit H."""
+        N, K = self.Np[i], self.Kp[i]
+        gw, gb = (self.dense_segs[f"Deep-part/mlp{i}/{n}"].off for n in ("weights", "biases"))
+        EX.group_wgrad(self.dZ[i], self.E if i == 0 else self.H8[i - 1], self.group_rows,
+                       out=(self.g[gw:gw + N * K].view(1, N, K), self.g[gb:gb + N].view(1, N)))
+
     def _mlp_backward(self, B: int):
         M = self.M
         for i in reversed(range(len(self.layers))):
             if self.batch_norm:
                 self._bn_backward(i, B)
-            Xt = self.Et if i == 0 else self.Ht[i - 1]
-            t, s = self.wg_cfg[i]
-            ep = EpiArgs()
-            if self.wg_direct[i] and _WG_BLAS:
-                # a plain GEMM with nothing to fuse: bf16 operands, fp32 result written in place
-                go = self.dense_segs[f"Deep-part/mlp{i}/weights"].off
-                gw = self.g[go:go + self.Np[i] * self.Kp[i]].view(self.Np[i], self.Kp[i])
-                torch.mm(self.dZt[i], Xt.t(), out_dtype=torch.float32, out=gw)
+            if self.act8:
+                self._wgrad_act8(i)
             else:
-                if self.wg_direct[i]:   # unsplit: the GEMM writes the final gradient itself
-                    ep.out = self.g.data_ptr() + 4 * self.dense_segs[f"Deep-part/mlp{i}/weights"].off
-                else:
-                    ep.out = self.slabs[i].data_ptr()
-                KN.gemm_nt(KN.EPI_F32, t, self.dZt[i], M, Xt, M, self.Np[i], self.Kp[i], M, s, ep)
+                self._wgrad(i)
             ep = EpiArgs()
-            if i > 0 and self.batch_norm:
+            if i > 0 and self.act8:
+                # relu and dropout left x > 0 where the code is above zero (a nonzero value's code is nonzero)
+                keep, N = self.keep[i - 1], self.Np[i - 1]
+                EX.group_dgrad(self.dZ[i], self.WT16[i].view(1, N, self.Np[i]), self.group_rows,
+                               mask=self.H8[i - 1], scale=(1.0 / keep) if keep < 1.0 else 1.0, out=self.dZ[i - 1])
+            elif i > 0 and self.batch_norm:
                 ep.out = self.dH[i - 1].data_ptr()    # f32 dL/dH_{i-1}; BN backward masks it
                 N = self.Np[i - 1]
                 if _epi_blas_ok(M, N, self.Np[i]):    # a plain GEMM: nothing to fuse
@@ -296,12 +320,12 @@ class LayerPathMixin:
         self._nslab_jobs = len(jobs)
         self._slab_maxn = maxn
         rj = []
-        for i in range(len(self.layers)):
+        for i in range(0 if self.act8 else len(self.layers)):
             sbias = self.dense_segs[f"Deep-part/mlp{i}/biases"].off
             rj.append(RowSumJob(g0 + 4 * sbias, self.dZt[i].data_ptr(), self.Np[i], self.M, self.M))
         self._row_jobs = KN.struct_array_to_device(rj, self.device)
         self._nrow_jobs = len(rj)
-        self._row_total = sum(self.Np)
+        self._row_total = sum(j.rows for j in rj)
         # the dense optimizer can ride on the finalize launch only if finalize writes the final
         # gradient of EVERY flat parameter (not so with batch norm: bn.hip writes beta / gamma).
         # Only the segments count: the 64-element alignment gaps between them hold no parameter
