@@ -15,11 +15,10 @@
 // (no atomics): the same inputs give the same bits.
 #include "common.h"
 
-#define RT_MAXE 1024     // experts (LDS histograms: 8 waves x 1024 x 4 B)
+#define RT_MAXE 1024     // experts
 #define RT_MAXK 16
-#define RT_THREADS 512
-#define RT_WAVES (RT_THREADS / 64)
-#define RT_CHUNK 512     // slots a wave keeps between its two phases
+#define RT_WAVES 8       // waves of a block (LDS histograms: 8 waves x 1024 x 4 B, or 16 x 512 x 4 B)
+#define RT_CHUNK 256     // slots a wave keeps between its two phases
 #define RT_MAXBLK 256
 
 struct RouteArgs {
@@ -30,7 +29,8 @@ struct RouteArgs {
   int* pos;                // [T, k]
   int* src;                // [T k]
   int* offs;               // [E + 1]
-  int* bh;                 // workspace [nblk, E]: a block's slots per expert
+  int* bh;                 // workspace [nblk + 1, E]: a block's slots per expert, then those of the blocks
+                           // before it; all slots per expert
   int* wpre;               // workspace [nblk, waves, E]: slots of the block's waves before this one
   long ld;
   int T, E, k, renorm, bf, nblk, tpb;   // tpb: tokens per block
@@ -46,98 +46,126 @@ struct RouteBwdArgs {
   int T, E, k, renorm, bf;
 };
 
-__device__ __forceinline__ float gate_value(const void* l, size_t i, int bf) {
-  float v = bf ? bf2f(reinterpret_cast<const bf16*>(l)[i]) : reinterpret_cast<const float*>(l)[i];
+__device__ __forceinline__ float gate_of(float v) {
   if (!(v == v)) v = -INFINITY;
   return fminf(v, 3.402823466e38f);
 }
+// A logit as an integer of the same order, and back (-0 made +0 before: they are equal).
+constexpr int GATE_CLOSED = (int)(0xFF800000u ^ 0x7FFFFFFFu);       // -inf
+__device__ __forceinline__ int gate_key(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return b ^ ((b >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float key_gate(int b) { return __int_as_float(b ^ ((b >> 31) & 0x7FFFFFFF)); }
 
-// Maximum and sum over each group of G lanes (G a power of two), in all of its lanes, by lane swaps
+// Maximum or sum over each group of G lanes (G a power of two), in all of its lanes, by lane swaps
 // in the vector unit: a shuffle through LDS takes over 100 cycles, and a choice needs one for each of
 // log2 G steps (16384 x 64, top 2: 26 us with shuffles, 11 with these).
-template <int G, typename F>
-__device__ __forceinline__ float group_all(float v, F op) {
-#define HFM_DPP(ctrl) __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), ctrl, 0xF, 0xF, true))
-  if (G >= 2) v = op(v, HFM_DPP(0xB1));        // quad: 1 0 3 2
-  if (G >= 4) v = op(v, HFM_DPP(0x4E));        // quad: 2 3 0 1
-  if (G >= 8) v = op(v, HFM_DPP(0x141));       // half row mirrored (quads are uniform by now)
-  if (G >= 16) v = op(v, HFM_DPP(0x140));      // row mirrored
+template <int G, typename T, typename F>
+__device__ __forceinline__ T group_all(T x, F op) {
+#define HFM_DPP(ctrl) __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), ctrl, 0xF, 0xF, true))
+  if (G >= 2) x = op(x, HFM_DPP(0xB1));        // quad: 1 0 3 2
+  if (G >= 4) x = op(x, HFM_DPP(0x4E));        // quad: 2 3 0 1
+  if (G >= 8) x = op(x, HFM_DPP(0x141));       // half row mirrored (quads are uniform by now)
+  if (G >= 16) x = op(x, HFM_DPP(0x140));      // row mirrored
 #undef HFM_DPP
   if (G >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = op(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1]));
   }
   if (G >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    x = op(__builtin_bit_cast(T, (uint32_t)r[0]), __builtin_bit_cast(T, (uint32_t)r[1]));
   }
-  return v;
+  return x;
 }
 
 // The top_k experts of one token by a group of G lanes (lane gl of the group holds experts gl + G q).
-// Lane j of the group ends with choice j (expert, weight; -1, 0 if none).
+// Lane j of the group ends with choice j (expert, weight; -1, 0 if none).  Bound by its instructions: values
+// are compared as integers (a float maximum comes with two instructions that quiet NaNs), and a lane's
+// own values are put in order first (the k largest, equal ones by index), so that a choice compares one value a
+// lane and its lane moves its list up (20011 x 256 bf16, top 8: 36 us with all float values compared in each choice
+// and 8 waves a block, 25 so).
 template <int G, int V>
-__device__ __forceinline__ void route_token(float (&v)[V], int k, int renorm, int lane, int& my_e, float& my_w) {
+__device__ __forceinline__ void route_token(const float (&o)[V], int k, int renorm, int lane, int& my_e, float& my_w) {
+  static_assert(V == 1 || G == 64, "several values a lane: the whole wave has one token");
   const int gl = lane & (G - 1);
-  const unsigned long long mine = (G == 64 ? ~0ull : ((1ull << G) - 1) << (lane & ~(G - 1)));
-  float top = -INFINITY, my_v = -INFINITY, o[V];
+  auto larger = [](int a, int b) { return max(a, b); };
+  int v[V], id[V], top = GATE_CLOSED, my_v = GATE_CLOSED;
   my_e = -1;
 #pragma unroll
-  for (int q = 0; q < V; ++q) o[q] = v[q];
-  for (int j = 0; j < k; ++j) {
-    float m = v[0];
-#pragma unroll
-    for (int q = 1; q < V; ++q) m = fmaxf(m, v[q]);
-    m = group_all<G>(m, [](float a, float b) { return fmaxf(a, b); });
-    if (j == 0) top = m;
-    // the lowest index among equals: the first q that has one, its first lane
-    int at = -1;
-#pragma unroll
-    for (int q = V - 1; q >= 0; --q) {
-      const unsigned long long has = __ballot(v[q] == m) & mine;
-      if (has) at = G * q + ((__ffsll(has) - 1) & (G - 1));
-    }
-    if (m == -INFINITY) at = -1;              // (all closed)
-    if (gl == j) {
-      my_e = at;
-      my_v = m;
-    }
-#pragma unroll
-    for (int q = 0; q < V; ++q)
-      if (at == gl + G * q) v[q] = -INFINITY;
+  for (int q = 0; q < V; ++q) {
+    v[q] = gate_key(o[q]);
+    id[q] = gl + G * q;
   }
-  const float ex = my_e >= 0 ? expf(my_v - top) : 0.f;
+  if constexpr (G == 64) {
+#pragma unroll
+    for (int p = 0; p < V - 1; ++p) {
+      if (p >= k) break;
+#pragma unroll
+      for (int q = V - 1; q > p; --q) {
+        const bool up = v[q] > v[q - 1];
+        const int a = max(v[q], v[q - 1]), b = min(v[q], v[q - 1]), c = id[q], d = id[q - 1];
+        v[q - 1] = a;
+        v[q] = b;
+        id[q - 1] = up ? c : d;
+        id[q] = up ? d : c;
+      }
+    }
+    for (int j = 0; j < k; ++j) {
+      const int m = __builtin_amdgcn_readfirstlane(group_all<G>(v[0], larger));
+      if (m == GATE_CLOSED) break;             // (no open one is left)
+      if (j == 0) top = m;
+      const unsigned long long has = __ballot(v[0] == m);
+      int at = __builtin_amdgcn_readlane(id[0], __ffsll(has) - 1);       // the lowest index among equals
+      for (unsigned long long more = has & (has - 1); more; more &= more - 1)
+        at = min(at, __builtin_amdgcn_readlane(id[0], __ffsll(more) - 1));
+      my_e = gl == j ? at : my_e;
+      my_v = gl == j ? m : my_v;
+      // (by masks: of a choice between neighbours the compiler makes an index, and of that 600 instructions)
+      const int won = at == id[0] ? -1 : 0;
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        v[q] = (v[q] & ~won) | ((q + 1 < V ? v[q + 1] : GATE_CLOSED) & won);
+        if (V > 1) id[q] = (id[q] & ~won) | ((q + 1 < V ? id[q + 1] : RT_MAXE) & won);
+      }
+    }
+  } else {
+    const unsigned long long mine = ((1ull << G) - 1) << (lane & ~(G - 1));
+    for (int j = 0; j < k; ++j) {
+      const int m = group_all<G>(v[0], larger);
+      if (j == 0) top = m;
+      const int at = (__ffsll(__ballot(v[0] == m) & mine) - 1) & (G - 1);
+      if (gl == j) {
+        my_e = m == GATE_CLOSED ? -1 : at;
+        my_v = m;
+      }
+      if (at == gl) v[0] = GATE_CLOSED;
+    }
+  }
+  const float ex = my_e >= 0 ? expf(key_gate(my_v) - key_gate(top)) : 0.f;
   float den = ex;
   if (!renorm) {
     den = 0.f;
 #pragma unroll
-    for (int q = 0; q < V; ++q) den += o[q] == -INFINITY ? 0.f : expf(o[q] - top);
+    for (int q = 0; q < V; ++q) den += o[q] == -INFINITY ? 0.f : expf(o[q] - key_gate(top));
   }
   den = group_all<G>(den, [](float a, float b) { return a + b; });
   my_w = den > 0.f ? ex / den : 0.f;
 }
 
-// Places of a block's slots, once every block's histogram is known (sums over blocks in LDS).
-__device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base, int* scan, const int* wpre) {
+// Places of a block's slots: `before` the expert's slots in earlier blocks, `all` its slots.
+template <int W>
+__device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base, int* scan, const int* before,
+                                            const int* all, const int* wpre) {
+  constexpr int THREADS = 64 * W;
   const int tid = threadIdx.x;
-  // base[e] = slots of expert e in earlier blocks, tot[e] in all: rows split over thread groups
   int* tot = base + RT_MAXE;
-  for (int e = tid; e < a.E; e += RT_THREADS) base[e] = tot[e] = 0;
-  __syncthreads();
-  int ep = 1;
-  while (ep < a.E) ep <<= 1;
-  if (ep > RT_THREADS) ep = RT_THREADS;
-  const int ng = RT_THREADS / ep, gr = tid / ep;
-  for (int e = tid % ep; e < a.E; e += ep) {
-    int before = 0, all = 0;
-#pragma unroll 8
-    for (int r = gr; r < a.nblk; r += ng) {
-      const int c = a.bh[(size_t)r * a.E + e];
-      all += c;
-      before += r < b ? c : 0;
-    }
-    atomicAdd(&base[e], before);           // (integers: the order does not matter)
-    atomicAdd(&tot[e], all);
+  for (int e = tid; e < a.E; e += THREADS) {
+    base[e] = before ? before[e] : 0;
+    tot[e] = all[e];
   }
   __syncthreads();
   // exclusive scan of tot over the experts, by wave 0
@@ -164,7 +192,7 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base
   __syncthreads();
   const int wave = tid >> 6, lane = tid & 63;
   const int t0 = b * a.tpb, t1 = min(a.T, t0 + a.tpb);
-  const int per = (a.tpb + RT_WAVES - 1) / RT_WAVES;
+  const int per = (a.tpb + W - 1) / W;
   const int s0 = min(t1, t0 + wave * per) * a.k, s1 = min(t1, t0 + (wave + 1) * per) * a.k;
   for (int s = s0 + lane; s < s1; s += 64) {
     const int e = a.expert[s];
@@ -175,48 +203,59 @@ __device__ __forceinline__ void route_place(const RouteArgs& a, int b, int* base
     }
   }
   const int live = *scan, n = a.T * a.k;    // places behind the last live slot
-  for (int p = live + b * RT_THREADS + tid; p < n; p += a.nblk * RT_THREADS) a.src[p] = -1;
+  for (int p = live + b * THREADS + tid; p < n; p += a.nblk * THREADS) a.src[p] = -1;
 }
 
 // grid nblk.  A wave takes a contiguous run of its block's tokens: choices first (a group of G lanes
 // per token), then the rank of each slot among the wave's earlier slots of its expert (64 slots at a
 // time: the lanes with the same expert by one ballot per index bit).  One block (few tokens) places
 // its slots at once, several leave it to route_place_kernel.
-template <int G, int V>
-__global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a) {
+template <int G, int V, int W>
+__global__ void __launch_bounds__(64 * W) route_kernel(RouteArgs a) {
+  constexpr int THREADS = 64 * W;
   extern __shared__ int lds[];
   int* wh = lds;                                                // [waves, E]
-  short* se = reinterpret_cast<short*>(lds + RT_WAVES * a.E);   // [waves, RT_CHUNK]
+  short* se = reinterpret_cast<short*>(lds + W * a.E);   // [waves, RT_CHUNK]
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int i = tid; i < RT_WAVES * a.E; i += RT_THREADS) wh[i] = 0;
+  for (int i = tid; i < W * a.E; i += THREADS) wh[i] = 0;
   __syncthreads();
   int* hist = wh + wave * a.E;
   short* es = se + wave * RT_CHUNK;
   const int b = blockIdx.x;
   const int t0 = b * a.tpb, t1 = min(a.T, t0 + a.tpb);
-  const int per = (a.tpb + RT_WAVES - 1) / RT_WAVES;
+  const int per = (a.tpb + W - 1) / W;
   const int w0 = min(t1, t0 + wave * per), w1 = min(t1, t0 + (wave + 1) * per);
   const int gl = lane & (G - 1), gi = lane / G;
   constexpr int NG = 64 / G;                                     // tokens at a time
   const int ct = RT_CHUNK / a.k / NG * NG;                       // tokens per chunk
   int bits = 0;
   while ((1 << bits) < a.E) ++bits;
-  float nv[V];                                                   // the next tokens' logits, under way
+  // The next tokens' logits, under way: as loaded, from rows and columns that exist, with nothing between
+  // the loads (a condition or a conversion there makes them wait for one another: 100000 x 128 bf16, top 4: 64
+  // us, 55 so)
+  uint32_t raw[V];
+  uint32_t live = 0;
   auto fetch = [&](int t) {
-    const bool on = t < w1 && (!a.valid || a.valid[t]);
+    t = min(t, a.T - 1);
+    live = a.valid ? a.valid[t] : 1;
+    if (a.bf) {
+      const uint16_t* l = reinterpret_cast<const uint16_t*>(a.logits) + (size_t)t * a.ld;
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-      const int e = gl + G * q;
-      nv[q] = on && e < a.E ? gate_value(a.logits, (size_t)t * a.ld + e, a.bf) : -INFINITY;
+      for (int q = 0; q < V; ++q) raw[q] = l[min(gl + G * q, a.E - 1)];
+    } else {
+      const uint32_t* l = reinterpret_cast<const uint32_t*>(a.logits) + (size_t)t * a.ld;
+#pragma unroll
+      for (int q = 0; q < V; ++q) raw[q] = l[min(gl + G * q, a.E - 1)];
     }
   };
-  fetch(w0 + gi);
+  if (w0 < w1) fetch(w0 + gi);
   for (int c0 = w0; c0 < w1; c0 += ct) {
     const int c1 = min(w1, c0 + ct);
     for (int t = c0 + gi; t - gi < c1; t += NG) {
       float v[V];
 #pragma unroll
-      for (int q = 0; q < V; ++q) v[q] = nv[q];
+      for (int q = 0; q < V; ++q)
+        v[q] = live && t < w1 && gl + G * q < a.E ? gate_of(__uint_as_float(a.bf ? raw[q] << 16 : raw[q])) : -INFINITY;
       fetch(t + NG);
       int e;
       float w;
@@ -248,27 +287,63 @@ __global__ void __launch_bounds__(RT_THREADS) route_kernel(RouteArgs a) {
   }
   __syncthreads();
   // slots of the block's earlier waves (in place), the block's histogram
-  int* base = reinterpret_cast<int*>(se + RT_WAVES * RT_CHUNK);
-  int* pre = gridDim.x == 1 ? wh : a.wpre + (size_t)b * RT_WAVES * a.E;
-  if (gridDim.x == 1) a.bh = base + 2 * RT_MAXE + 1;
-  for (int e = tid; e < a.E; e += RT_THREADS) {
+  int* base = reinterpret_cast<int*>(se + W * RT_CHUNK);
+  int* pre = gridDim.x == 1 ? wh : a.wpre + (size_t)b * W * a.E;
+  int* own = gridDim.x == 1 ? base + 2 * RT_MAXE + 1 : a.bh + (size_t)b * a.E;
+  for (int e = tid; e < a.E; e += THREADS) {
     int run = 0;
-    for (int w = 0; w < RT_WAVES; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int c = wh[w * a.E + e];
       pre[w * a.E + e] = run;
       run += c;
     }
-    a.bh[(size_t)b * a.E + e] = run;
+    own[e] = run;
   }
   if (gridDim.x != 1) return;
   __threadfence_block();
   __syncthreads();
-  route_place(a, 0, base, base + 2 * RT_MAXE, wh);
+  route_place<W>(a, 0, base, base + 2 * RT_MAXE, nullptr, own, wh);
 }
 
-__global__ void __launch_bounds__(RT_THREADS) route_place_kernel(RouteArgs a) {
+// Slots of the blocks before each block, per expert, and of all: 16 experts a workgroup, 16 runs of
+// blocks each.  (Every placing block summing what it needs by itself: 20011 x 256: 37 us in all, 35
+// so; 4096 x 1024: 104, 95.)
+__global__ void __launch_bounds__(256) route_scan_kernel(RouteArgs a) {
+  __shared__ int sum[16][17];
+  constexpr int RUN = RT_MAXBLK / 16;
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
+  int n[RUN], run = 0;
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const int b = q * RUN + i;
+    n[i] = b < a.nblk && e < a.E ? a.bh[(size_t)b * a.E + e] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) run += n[i];
+  sum[q][c] = run;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    before += i < q ? sum[i][c] : 0;
+    all += sum[i][c];
+  }
+  if (e >= a.E) return;
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const int b = q * RUN + i;
+    if (b < a.nblk) a.bh[(size_t)b * a.E + e] = before;
+    before += n[i];
+  }
+  if (q == 0) a.bh[(size_t)a.nblk * a.E + e] = all;
+}
+
+template <int W>
+__global__ void __launch_bounds__(64 * W) route_place_kernel(RouteArgs a) {
   __shared__ int base[2 * RT_MAXE + 1];
-  route_place(a, blockIdx.x, base, base + 2 * RT_MAXE, a.wpre + (size_t)blockIdx.x * RT_WAVES * a.E);
+  const int b = blockIdx.x;
+  route_place<W>(a, b, base, base + 2 * RT_MAXE, a.bh + (size_t)b * a.E, a.bh + (size_t)a.nblk * a.E,
+                 a.wpre + (size_t)b * W * a.E);
 }
 
 static int route_group(int E) {
@@ -277,17 +352,22 @@ static int route_group(int E) {
   return G;
 }
 
-// Blocks of a call: one while a block's 8 waves take at most 8 rounds of tokens, else at most 256
-// (a placing block reads every block's histogram), each with 4 rounds or more.
+// Blocks of a call: one while a block's 8 waves take at most 4 rounds of tokens (one launch instead of
+// three; 60 x 64, 8 rounds: 12.8 us so, 9.9 with blocks), else a round each, at most 256 (1000 x 1024: 33 us,
+// with 4 rounds each 82).
 HFM_API int hfm_route_blocks(int T, int E) {
   const int round = RT_WAVES * (64 / route_group(E));
-  if (T <= 8 * round) return 1;
-  const int n = (T + 4 * round - 1) / (4 * round);
+  if (T <= 4 * round) return 1;
+  const int n = (T + round - 1) / round;
   return n < RT_MAXBLK ? n : RT_MAXBLK;
 }
+// Waves of a block: 16 where a token takes a whole wave and their histograms fit the 64 KB, else 8 (both
+// with one value a lane and more in us: 16384 x 64: 13.7, 15.0; 100000 x 128: 65, 92; 20011 x 256: 38, 48; 4096 x
+// 1024: 90, 85; one block: 500 x 16: 12.9, 9.2).
+static int route_waves(int T, int E) { return hfm_route_blocks(T, E) > 1 && E > 32 && E <= 512 ? 16 : RT_WAVES; }
 HFM_API int hfm_route_ws_ints(int T, int E) {
   const int n = hfm_route_blocks(T, E);
-  return n == 1 ? 0 : n * E * (1 + RT_WAVES);      // (one block keeps its counts in LDS)
+  return n == 1 ? 0 : (n + 1) * E + n * E * route_waves(T, E);      // (one block keeps its counts in LDS)
 }
 
 HFM_API int hfm_route(const RouteArgs* ap, hipStream_t st) {
@@ -298,81 +378,94 @@ HFM_API int hfm_route(const RouteArgs* ap, hipStream_t st) {
   const int G = route_group(a.E);
   a.nblk = hfm_route_blocks(a.T, a.E);
   a.tpb = a.T > 0 ? (a.T + a.nblk - 1) / a.nblk : 1;
-  a.wpre = a.bh + (size_t)a.nblk * a.E;
-  size_t lds = (size_t)RT_WAVES * a.E * 4 + RT_WAVES * RT_CHUNK * 2;
+  a.wpre = a.bh + (size_t)(a.nblk + 1) * a.E;
+  const int W = route_waves(a.T, a.E);
+  size_t lds = (size_t)W * a.E * 4 + W * RT_CHUNK * 2;
   if (a.nblk == 1) lds += (3 * RT_MAXE + 1) * 4;
-  const dim3 grid(a.nblk), blk(RT_THREADS);
-#define HFM_ROUTE(G, V) hipLaunchKernelGGL((route_kernel<G, V>), grid, blk, lds, st, a)
+  const dim3 grid(a.nblk), blk(W * 64);
+#define HFM_ROUTE(G, V, W) hipLaunchKernelGGL((route_kernel<G, V, W>), grid, blk, lds, st, a)
   switch (G) {
-    case 1: HFM_ROUTE(1, 1); break;
-    case 2: HFM_ROUTE(2, 1); break;
-    case 4: HFM_ROUTE(4, 1); break;
-    case 8: HFM_ROUTE(8, 1); break;
-    case 16: HFM_ROUTE(16, 1); break;
-    case 32: HFM_ROUTE(32, 1); break;
+    case 1: HFM_ROUTE(1, 1, 8); break;
+    case 2: HFM_ROUTE(2, 1, 8); break;
+    case 4: HFM_ROUTE(4, 1, 8); break;
+    case 8: HFM_ROUTE(8, 1, 8); break;
+    case 16: HFM_ROUTE(16, 1, 8); break;
+    case 32: HFM_ROUTE(32, 1, 8); break;
     default:
-      if (a.E <= 64) HFM_ROUTE(64, 1);
-      else if (a.E <= 128) HFM_ROUTE(64, 2);
-      else if (a.E <= 256) HFM_ROUTE(64, 4);
-      else if (a.E <= 512) HFM_ROUTE(64, 8);
-      else HFM_ROUTE(64, 16);
+      if (a.E > 512) HFM_ROUTE(64, 16, 8);
+      else if (W == 8) {                         // (one block)
+        if (a.E <= 64) HFM_ROUTE(64, 1, 8);
+        else if (a.E <= 128) HFM_ROUTE(64, 2, 8);
+        else if (a.E <= 256) HFM_ROUTE(64, 4, 8);
+        else HFM_ROUTE(64, 8, 8);
+      } else {
+        if (a.E <= 64) HFM_ROUTE(64, 1, 16);
+        else if (a.E <= 128) HFM_ROUTE(64, 2, 16);
+        else if (a.E <= 256) HFM_ROUTE(64, 4, 16);
+        else HFM_ROUTE(64, 8, 16);
+      }
   }
 #undef HFM_ROUTE
-  if (a.nblk > 1) hipLaunchKernelGGL(route_place_kernel, grid, blk, 0, st, a);
+  if (a.nblk > 1) {
+    hipLaunchKernelGGL(route_scan_kernel, dim3((a.E + 15) / 16), dim3(256), 0, st, a);
+    if (W == 8) hipLaunchKernelGGL(route_place_kernel<8>, grid, blk, 0, st, a);
+    else hipLaunchKernelGGL(route_place_kernel<16>, grid, blk, 0, st, a);
+  }
   HFM_LAUNCH_CHECK();
 }
 
-// A group of G lanes per token again.  p_i needs no second softmax: the first choice has the largest
-// logit m and the weight exp(0) / den, so p_i = exp(l_i - m) w_0.
-template <int K>
-__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a, int G) {
-  const int lane = threadIdx.x & 63;
-  const int gl = lane & (G - 1);
-  const int t = (int)(((long)blockIdx.x * 256 + threadIdx.x) / G);
+// A group of G lanes per token: lane j has choice j, and 16 bytes of the row a turn.  The row is written as
+// if no expert were chosen (zeros, or -p dot), then the chosen ones over it.  p_i needs no second
+// softmax: the first choice has the largest logit m and the weight exp(0) / den, so p_i = exp(l_i - m) w_0.
+// (20011 x 256 bf16, top 8, renormalized: 18 us with every element compared with every choice, 7 so.)
+template <typename T, int G>
+__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  const int gl = threadIdx.x & (G - 1);
+  const int t = blockIdx.x * (256 / G) + threadIdx.x / G;
   if (t >= a.T) return;
-  int ex[K];
-  float w[K], g[K], dot = 0.f;
+  const size_t o = (size_t)t * a.k + gl;
+  const int e = gl < a.k ? a.expert[o] : -1;
+  const float w = e >= 0 ? a.weight[o] : 0.f, g = e >= 0 ? a.dweight[o] : 0.f;
+  const float dot = group_all<G>(e >= 0 ? w * g : 0.f, [](float x, float y) { return x + y; });
+  const T* l = reinterpret_cast<const T*>(a.logits) + (size_t)t * a.ld;
+  T* d = reinterpret_cast<T*>(a.dlogits) + (size_t)t * a.ldo;
+  const int e0 = __shfl(e, 0, G);
+  const bool soft = !a.renorm && e0 >= 0 && e0 < a.E;
+  const float m = soft ? gate_of((float)l[e0]) : 0.f, c = -__shfl(w, 0, G) * dot;
+  for (int i = gl * V; i < a.E; i += G * V) {
+    vec v = {};
+    if (i + V <= a.E) {
+      if (soft) {
+        const vec x = *reinterpret_cast<const vec*>(l + i);
 #pragma unroll
-  for (int j = 0; j < K; ++j) {
-    const size_t o = (size_t)t * a.k + j;
-    ex[j] = j < a.k ? a.expert[o] : -1;
-    w[j] = j < a.k ? a.weight[o] : 0.f;
-    g[j] = j < a.k ? a.dweight[o] : 0.f;
-  }
-#pragma unroll
-  for (int j = 0; j < K; ++j)
-    if (ex[j] >= 0) dot = fmaf(w[j], g[j], dot);
-  const bool any = ex[0] >= 0 && ex[0] < a.E;
-  const float m = any && !a.renorm ? gate_value(a.logits, (size_t)t * a.ld + ex[0], a.bf) : 0.f;
-#pragma unroll 4
-  for (int i = gl; i < a.E; i += G) {
-    float d = 0.f;
-    if (any) {
-      if (!a.renorm) {
-        const float l = gate_value(a.logits, (size_t)t * a.ld + i, a.bf);
-        if (l != -INFINITY) d = -expf(l - m) * w[0] * dot;
+        for (int q = 0; q < V; ++q) v[q] = (T)(c * expf(gate_of((float)x[q]) - m));
       }
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (ex[j] == i) d = a.renorm ? w[j] * (g[j] - dot) : fmaf(w[j], g[j], d);
+      *reinterpret_cast<vec*>(d + i) = v;
+    } else {
+      for (int q = i; q < a.E; ++q) d[q] = soft ? (T)(c * expf(gate_of((float)l[q]) - m)) : (T)0.f;
     }
-    const size_t o = (size_t)t * a.ldo + i;
-    if (a.bf) reinterpret_cast<bf16*>(a.dlogits)[o] = f2bf(d);
-    else reinterpret_cast<float*>(a.dlogits)[o] = d;
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // (the wave's stores stay in order)
+  if (e >= 0 && e < a.E) d[e] = (T)(w * (g - dot));
+}
+
+template <typename T>
+static void route_bwd(const RouteBwdArgs& a, hipStream_t st) {
+  const int lanes = (a.E * (int)sizeof(T) + 15) / 16;          // (and one for each choice)
+  const dim3 blk(256);
+  if (lanes <= 16) hipLaunchKernelGGL((route_bwd_kernel<T, 16>), dim3((a.T + 15) / 16), blk, 0, st, a);
+  else if (lanes <= 32) hipLaunchKernelGGL((route_bwd_kernel<T, 32>), dim3((a.T + 7) / 8), blk, 0, st, a);
+  else hipLaunchKernelGGL((route_bwd_kernel<T, 64>), dim3((a.T + 3) / 4), blk, 0, st, a);
 }
 
 HFM_API int hfm_route_bwd(const RouteBwdArgs* ap, hipStream_t st) {
-  const RouteBwdArgs a = *ap;
+  const RouteBwdArgs& a = *ap;
   if (a.T < 0 || a.E < 1 || a.E > RT_MAXE || a.k < 1 || a.k > RT_MAXK) return (int)hipErrorInvalidValue;
   if (a.T == 0) return 0;
-  const int G = route_group(a.E), per = 256 / G;
-  const dim3 grid((a.T + per - 1) / per), blk(256);
-  if (a.k <= 1) hipLaunchKernelGGL(route_bwd_kernel<1>, grid, blk, 0, st, a, G);
-  else if (a.k <= 2) hipLaunchKernelGGL(route_bwd_kernel<2>, grid, blk, 0, st, a, G);
-  else if (a.k <= 4) hipLaunchKernelGGL(route_bwd_kernel<4>, grid, blk, 0, st, a, G);
-  else if (a.k <= 8) hipLaunchKernelGGL(route_bwd_kernel<8>, grid, blk, 0, st, a, G);
-  else hipLaunchKernelGGL(route_bwd_kernel<16>, grid, blk, 0, st, a, G);
+  if (a.bf) route_bwd<bf16>(a, st);
+  else route_bwd<float>(a, st);
   HFM_LAUNCH_CHECK();
 }
 HFM_API int hfm_route_args_bytes() { return (int)sizeof(RouteArgs); }

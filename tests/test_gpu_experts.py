@@ -75,6 +75,35 @@ def test_route_ties_closed_and_extreme(renorm):
     assert torch.isfinite(d).all() and (d.cpu()[(torch.isnan(lg)) | (lg == -inf)] == 0).all()
 
 
+@pytest.mark.parametrize("T,E,k", [(40, 100, 5), (900, 128, 8), (30, 256, 16), (900, 300, 8), (4097, 512, 3), (700, 1024, 4)])
+def test_route_equal_values(T, E, k):
+    """Few different values, so that every choice has equals, in one lane's list and in many; whole rows closed."""
+    g = gen(T + E)
+    lg = torch.randint(-1, 2, (T, E), generator=g).float()
+    lg[lg == 0] = -0.0
+    lg[torch.rand(T, E, generator=g) < 0.3] = 0.0
+    lg[torch.rand(T, E, generator=g) < 0.2] = -math.inf
+    lg[::7] = -math.inf
+    lg[1::7, : E - 2] = -math.inf
+    check_route(lg, k, True)
+    check_route(lg.bfloat16(), k, False, torch.rand(T, generator=g) > 0.1)
+
+
+@pytest.mark.parametrize("E", [5, 37, 130, 515])
+def test_route_gradient_rows_at_any_alignment(E):
+    EX, _ = ops()
+    g = gen(E)
+    big = randn(g, 61, E + 9).to(DEV)
+    dw = randn(g, 61, 3).to(DEV)
+    for dt in (torch.float32, torch.bfloat16):
+        lg, out = big.to(dt)[:, 3:3 + E], torch.full((61, E + 5), 7.0, dtype=dt, device=DEV)
+        for renorm in (True, False):
+            r = EX.route(lg, 3, renormalize=renorm)
+            want = EX.route_bwd(lg.contiguous(), r, dw, renormalize=renorm)
+            EX.route_bwd(lg, r, dw, renormalize=renorm, out=out[:, 1:1 + E])
+            assert torch.equal(out[:, 1:1 + E], want) and (out[:, 0] == 7).all() and (out[:, 1 + E:] == 7).all()
+
+
 def test_route_no_rows_and_strides():
     EX, _ = ops()
     r = EX.route(torch.empty(0, 5, device=DEV), 2)
