@@ -304,8 +304,9 @@ __device__ __forceinline__ void dma16_buf(const void* base, uint32_t bytes, uint
 
 // One step of a wave.  D: its DMA pieces per step.  stage(i): piece i of the step three ahead; load_a(i),
 // load_b(j): fragments of the next step; PAR: which of the two sets of column fragments is multiplied.
+// cs: column sums of A, in the vector unit while the MFMAs run (a lane's share: column lane & 31 of tile i).
 template <int NI, int D, int PAR, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a,
+__device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], float (&cs)[NI], bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a,
                                         LB load_b, EX extra) {
   constexpr int NA = 2 * NI, c = PAR, n = c ^ 1;      // row fragment r: 16-deep half r / NI, rows 32 (r % NI) ..
   static_assert(NI >= 3 && NI <= 4 && D <= 2 * NA - 4, "a place for every load");
@@ -318,6 +319,9 @@ __device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], bf16x8 (&fa)[2 * N
   for (int k = 0; k < 4 * NA; ++k) {
     const int r = k >> 2, j = k & 3;
     acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[c][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    cs[r % NI] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{fa[r][2 * j], fa[r][2 * j + 1]}, bf16x2{f2bf(1.f), f2bf(1.f)},
+                                                 cs[r % NI], false);
     // at most one load between two MFMAs: a wave issues an instruction every 4 cycles, an MFMA runs 32
     if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1);
     if (j == 1 && r < 4) fb[n][2 * r] = load_b(2 * r);
@@ -348,13 +352,13 @@ __device__ __forceinline__ void mm_begin(bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8
 // A whole reduction of ns steps.  stage(i, step): zeros from the step `ns` on (the loop runs on a pair of steps
 // at a time and three steps ahead, without a branch: its registers do not survive one).
 template <int NI, int D, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], ST stage, LA load_a, LB load_b, EX extra) {
+__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], float (&cs)[NI], ST stage, LA load_a, LB load_b, EX extra) {
   bf16x8 fa[2 * NI], fb[2][8];
   mm_begin<NI, D>(fa, fb, stage, [&](int i) { return load_a(i, smem); }, [&](int j) { return load_b(j, smem); });
   auto step = [&](auto PAR, int s) {
     const char* nb = smem + ((s + 1) & (GP_RING - 1)) * GP_BUF;
     mm_step<NI, D, decltype(PAR)::value>(
-        acc, fa, fb, [&](int i) { stage(i, s + GP_RING - 1); }, [&](int i) { return load_a(i, nb); },
+        acc, cs, fa, fb, [&](int i) { stage(i, s + GP_RING - 1); }, [&](int i) { return load_a(i, nb); },
         [&](int j) { return load_b(j, nb); }, [&]() { extra(PAR, s); });
   };
   for (int s = 0; s < ns; s += 2) {
@@ -921,6 +925,11 @@ __device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32
   *reinterpret_cast<uint4*>(p) = make_uint4(a, b, c, d);
 }
 
+// the parts' column sums, behind their tiles: [lane][row of tiles][first, second part][256]
+__device__ __forceinline__ float* wg_sums(const GroupWgArgs& g, int tiles, int lanes) {
+  return g.ws + (size_t)2 * lanes * tiles * GW_SLAB;
+}
+
 template <bool X8, bool GATHER>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
 group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
@@ -962,6 +971,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     const int p1 = __builtin_amdgcn_readfirstlane(min(hi_row, lo + s1 * GW_UNIT));
     const int ns = p1 > p0 ? (p1 - p0 + GP_K - 1) / GP_K : 0;
     f32x16 acc[4][4] = {};
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
     // columns past N or K read column 0 (their outputs are not stored)
     const uint32_t ao0 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + ce < g.N ? n0 + ce : 0));
     const uint32_t ao1 = 2u * (uint32_t)(hi * (int)g.ldz + (n0 + (ce ^ 64) < g.N ? n0 + (ce ^ 64) : 0));
@@ -1065,7 +1075,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         codes_of(0, 4);
         rows_of(1, 5);
         rows_of(0, 6);
-        mm_loop<4, 4>(smem, ns, acc, piece_a, load_a, load_b, [&](auto PAR, int s) {
+        mm_loop<4, 4>(smem, ns, acc, sum, piece_a, load_a, load_b, [&](auto PAR, int s) {
           constexpr int set = decltype(PAR)::value ^ 1;
           hide();
           codes_to(set, s + 3);
@@ -1075,7 +1085,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       } else {
         // GATHER: a step's rows are read two steps before its DMA starts
         mm_loop<4, 8>(
-            smem, ns, acc,
+            smem, ns, acc, sum,
             [&](int i, int s) {
               if (i < 4) piece_a(i, s);
               else piece_b(i - 4, s, xrow[s & 1][i - 4]);
@@ -1087,7 +1097,17 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     __syncthreads();                      // (the next part's staging overwrites what was read here)
     // a whole tile goes to dw, a part to the workspace: slot 2 w if it is the workgroup's first, 2 w + 1
     // if it goes on in the next one
-    if (s0 == 0 && s1 == steps)
+    const bool whole = s0 == 0 && s1 == steps;
+    if (g.db && tk == 0 && wc == 0) {
+      float* d = whole ? g.db + (size_t)e * g.N : wg_sums(g, tiles, lanes) + (size_t)(2 * (w / tiles * tiles_n + tn) + (s0 > 0 ? 0 : 1)) * GP_B - n0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + wr * 128 + i * 32 + (lane & 31);
+        const float v = sum[i] + __shfl_xor(sum[i], 32);
+        if (lane < 32 && (!whole || n < g.N)) d[n] = v;
+      }
+    }
+    if (whole)
       mm_out_f32(acc, g.dw + ((size_t)e * g.N + n0 + wr * 128) * g.K + k0 + wc * 128, g.N - n0 - wr * 128,
                  g.K - k0 - wc * 128, g.K, lane);
     else
@@ -1104,6 +1124,12 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
   int tn, tk;
   band_tile(ti, tiles_n, tiles_k, tn, tk);
   const int n0 = tn * GP_B, k0 = tk * GP_B;
+  if (g.db && tk == 0 && blockIdx.z == 0 && n0 + (int)threadIdx.x < g.N) {
+    const float* s = wg_sums(g, tiles, lanes) + (size_t)2 * (l0 * tiles_n + tn) * GP_B + threadIdx.x;
+    float v = s[GP_B];
+    for (int l = l0 + 1; l <= l1; ++l) v += s[(size_t)2 * (l - l0) * tiles_n * GP_B];
+    g.db[(size_t)e * g.N + n0 + threadIdx.x] = v;
+  }
   // the lane that starts the group left it in its second tile, the others in their first
   const float* s0 = g.ws + (size_t)(2 * (l0 * tiles + ti) + 1) * GW_SLAB;
   const float* s1 = g.ws + (size_t)(2 * ((l0 + 1) * tiles + ti)) * GW_SLAB;
@@ -1134,63 +1160,6 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
   }
 }
 
-// db of the large tile's path: column sums of dz, chunks of GW_DBROWS rows of a group (256 columns: 32
-// lanes of 8 columns, 8 rows at a time), then the group's chunks, 8 threads a column, in a fixed order.  Beside the product rather
-// than in it: a ninth fragment column there costs its loop registers or a branch.
-constexpr int GW_DBROWS = 256;
-__global__ void __launch_bounds__(256) group_db_part_kernel(GroupWgArgs g, float* part) {
-  int e, r0, r1;
-  if (!group_find<GW_DBROWS>(g.offs, g.E, g.S, blockIdx.x, e, r0, r1)) return;
-  __shared__ float red[8][256];
-  const int c = threadIdx.x & 31, rl = threadIdx.x >> 5, n = blockIdx.y * 256 + c * 8;
-  const int end = min(r1, r0 + GW_DBROWS);
-  float s[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] = 0.f;
-  if (n < g.N) {
-#pragma unroll 4
-    for (int p = r0 + rl; p < end; p += 8) {
-      const bf16x8 v = *reinterpret_cast<const bf16x8*>(g.dz + (size_t)p * g.ldz + n);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += bf2f(v[j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) red[rl][c * 8 + j] = s[j];
-  __syncthreads();
-  const int col = blockIdx.y * 256 + threadIdx.x;
-  float t = 0.f;
-#pragma unroll
-  for (int q = 0; q < 8; ++q) t += red[q][threadIdx.x];
-  if (col < g.N) part[(size_t)blockIdx.x * g.N + col] = t;
-}
-
-__global__ void __launch_bounds__(256) group_db_sum_kernel(GroupWgArgs g, const float* part) {
-  __shared__ float red[8][32];
-  const int e = blockIdx.y, c = threadIdx.x & 31, q0 = threadIdx.x >> 5, col = blockIdx.x * 32 + c, lane = threadIdx.x & 63;
-  int before = 0, lo, hi;
-  for (int i = lane; i < e; i += 64) {
-    group_rows(g.offs, i, g.S, lo, hi);
-    before += (hi - lo + GW_DBROWS - 1) / GW_DBROWS;
-  }
-  for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-  group_rows(g.offs, e, g.S, lo, hi);
-  // (offsets out of order could make more chunks than there is room for)
-  const int n = min((hi - lo + GW_DBROWS - 1) / GW_DBROWS, g.S / GW_DBROWS + g.E - before);
-  float t = 0.f;
-  if (col < g.N) {
-#pragma unroll 4
-    for (int q = q0; q < n; q += 8) t += part[(size_t)(before + q) * g.N + col];
-  }
-  red[q0][c] = t;
-  __syncthreads();
-  if (q0 == 0 && col < g.N) {
-#pragma unroll
-    for (int q = 1; q < 8; ++q) t += red[q][c];
-    g.db[(size_t)e * g.N + col] = t;
-  }
-}
-
 // Where the large tile is taken: operands with 16-byte rows, and enough work for every CU (GP_MIN_UNITS
 // steps of 64 rows each; below that the 128 x 128 tile's smaller pieces fill the chip better).
 constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
@@ -1218,10 +1187,10 @@ static int wgrad_lanes(const GroupWgArgs& g) {
   }
   return best;
 }
-// Slabs, then the parts of db.  A single lane cuts no group.
-static long wgrad_slab_floats(const GroupWgArgs& g) {
-  const int l = wgrad_lanes(g);
-  return l == 1 ? 0 : 2l * l * ((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B) * GW_SLAB;
+// Two parts a workgroup, and their sums.  A single lane cuts no group.
+static long wgrad_ws_floats(const GroupWgArgs& g) {
+  const long l = wgrad_lanes(g), tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
+  return l == 1 ? 0 : 2 * l * tn * (tk * GW_SLAB + GP_B);
 }
 
 // Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
@@ -1237,7 +1206,7 @@ static int wgrad_splits(int S, int N, int K, int E) {
 }
 
 HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
-  if (wgrad_big(*gp)) return wgrad_slab_floats(*gp) + (gp->db ? (long)(gp->S / GW_DBROWS + gp->E) * gp->N : 0);
+  if (wgrad_big(*gp)) return wgrad_ws_floats(*gp);
   const int ns = wgrad_splits(gp->S, gp->N, gp->K, gp->E);
   return ns > 1 ? (long)ns * gp->E * gp->N * (gp->K + 1) : 0;
 }
@@ -1249,7 +1218,7 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   if (wgrad_big(g)) {
     const int tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
     const int lanes = wgrad_lanes(g);
-    if ((lanes > 1 || g.db) && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    if (lanes > 1 && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
     const dim3 grid((unsigned)(tn * tk * lanes)), blk(GP_THREADS);
     if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, lanes);
@@ -1258,11 +1227,6 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
     else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, lanes);
     if (lanes > 1)
       hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 16), dim3(256), 0, st, g, tn, tk, lanes, ovec);
-    if (g.db) {
-      float* part = g.ws + wgrad_slab_floats(g);
-      hipLaunchKernelGGL(group_db_part_kernel, dim3(g.S / GW_DBROWS + g.E, (g.N + 255) / 256), dim3(256), 0, st, g, part);
-      hipLaunchKernelGGL(group_db_sum_kernel, dim3((g.N + 31) / 32, g.E), dim3(256), 0, st, g, part);
-    }
     HFM_LAUNCH_CHECK();
   }
   g.ns = wgrad_splits(g.S, g.N, g.K, g.E);
