@@ -304,24 +304,54 @@ __device__ __forceinline__ void dma16_buf(const void* base, uint32_t bytes, uint
 
 // One step of a wave.  D: its DMA pieces per step.  stage(i): piece i of the step three ahead; load_a(i),
 // load_b(j): fragments of the next step; PAR: which of the two sets of column fragments is multiplied.
-// cs: column sums of A, in the vector unit while the MFMAs run (a lane's share: column lane & 31 of tile i).
-template <int NI, int D, int PAR, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], float (&cs)[NI], bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a,
-                                        LB load_b, EX extra) {
+// cs: where `take`, column sums of A (a lane's share: column lane & 31 of tile i).  Two bf16 an instruction: in
+// every step they cost 90 us of 400 (16384 x 4096 x 4096), in a launch of their own 31, in one of 2 tiles_k steps
+// 13.  The branch is in the assembly, where the compiler does not see it: its accumulators do not survive
+// another block in the loop.
+__device__ __forceinline__ void col_sums(float (&c)[4], const bf16x8 (&fa)[8], int take) {
+  uint4 u[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) u[r] = __builtin_bit_cast(uint4, fa[r]);
+  asm volatile(
+      "s_cmp_lg_u32 %36, 0\n\ts_cbranch_scc0 .Lskip%=\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %4\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %8\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %12\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %16\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %20\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %24\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %28\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %32\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %5\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %9\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %13\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %17\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %21\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %25\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %29\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %33\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %6\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %10\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %14\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %18\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %22\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %26\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %30\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %34\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %7\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %11\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %15\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %19\n\t"
+      "v_dot2c_f32_bf16 %0, 0x3f803f80, %23\n\t" "v_dot2c_f32_bf16 %1, 0x3f803f80, %27\n\t"
+      "v_dot2c_f32_bf16 %2, 0x3f803f80, %31\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %35\n\t"
+      "s_nop 3\n.Lskip%=:"
+      : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])
+      : "v"(u[0].x), "v"(u[0].y), "v"(u[0].z), "v"(u[0].w), "v"(u[1].x), "v"(u[1].y), "v"(u[1].z), "v"(u[1].w), "v"(u[2].x), "v"(u[2].y), "v"(u[2].z), "v"(u[2].w), "v"(u[3].x), "v"(u[3].y), "v"(u[3].z), "v"(u[3].w), "v"(u[4].x), "v"(u[4].y), "v"(u[4].z), "v"(u[4].w), "v"(u[5].x), "v"(u[5].y), "v"(u[5].z), "v"(u[5].w), "v"(u[6].x), "v"(u[6].y), "v"(u[6].z), "v"(u[6].w), "v"(u[7].x), "v"(u[7].y), "v"(u[7].z), "v"(u[7].w), "s"(take)
+      : "scc");
+}
+// extra(k): what else the step does, after MFMA k (-1: before all); WAIT: the loads that may be in flight at its
+// top, those issued after the DMA of the step after this one.
+template <int NI, int D, int WAIT, int PAR, typename ST, typename LA, typename LB, typename EX>
+__device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], float (&cs)[NI], int take, bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8],
+                                        ST stage, LA load_a, LB load_b, EX extra) {
   constexpr int NA = 2 * NI, c = PAR, n = c ^ 1;      // row fragment r: 16-deep half r / NI, rows 32 (r % NI) ..
   static_assert(NI >= 3 && NI <= 4 && D <= 2 * NA - 4, "a place for every load");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");        // (the DMA of the step after next stays in flight)
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WAIT) : "memory");     // (the DMA of the step after next stays in flight)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");          // (no access moves over the barrier)
   __builtin_amdgcn_sched_barrier(0);
-  extra();
+  extra(-1);
 #pragma unroll
   for (int k = 0; k < 4 * NA; ++k) {
     const int r = k >> 2, j = k & 3;
     acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[c][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    cs[r % NI] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{fa[r][2 * j], fa[r][2 * j + 1]}, bf16x2{f2bf(1.f), f2bf(1.f)},
-                                                 cs[r % NI], false);
+    if (k == 3) col_sums(cs, fa, take);          // (row fragments are replaced after their rounds)
     // at most one load between two MFMAs: a wave issues an instruction every 4 cycles, an MFMA runs 32
     if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1);
     if (j == 1 && r < 4) fb[n][2 * r] = load_b(2 * r);
@@ -329,18 +359,20 @@ __device__ __forceinline__ void mm_step(f32x16 (&acc)[NI][4], float (&cs)[NI], b
     if (j == 3 && r < D) stage(r);
     if (j == 1 && r >= 4 && NA + r - 4 < D) stage(NA + r - 4);
     if (k == 4 * NA - 1) fa[NA - 1] = load_a(NA - 1);
+    extra(k);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// The first three steps' DMA under way, the first step's fragments in registers.
-template <int NI, int D, typename ST, typename LA, typename LB>
+// The first three steps' DMA under way, the first step's fragments in registers.  (Where a step's top lets other loads
+// be in flight too, there are none yet behind these: they have landed here.)
+template <int NI, int D, int WAIT, typename ST, typename LA, typename LB>
 __device__ __forceinline__ void mm_begin(bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8], ST stage, LA load_a, LB load_b) {
 #pragma unroll
   for (int s = 0; s < GP_RING - 1; ++s)
 #pragma unroll
     for (int i = 0; i < D; ++i) stage(i, s);
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * D) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(WAIT == D ? 2 * D : 0) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
@@ -351,15 +383,17 @@ __device__ __forceinline__ void mm_begin(bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8
 
 // A whole reduction of ns steps.  stage(i, step): zeros from the step `ns` on (the loop runs on a pair of steps
 // at a time and three steps ahead, without a branch: its registers do not survive one).
-template <int NI, int D, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], float (&cs)[NI], ST stage, LA load_a, LB load_b, EX extra) {
+template <int NI, int D, int WAIT, typename ST, typename LA, typename LB, typename EX>
+__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], float (&cs)[NI], int turn, int period, ST stage, LA load_a, LB load_b, EX extra) {
   bf16x8 fa[2 * NI], fb[2][8];
-  mm_begin<NI, D>(fa, fb, stage, [&](int i) { return load_a(i, smem); }, [&](int j) { return load_b(j, smem); });
+  mm_begin<NI, D, WAIT>(fa, fb, stage, [&](int i) { return load_a(i, smem); }, [&](int j) { return load_b(j, smem); });
   auto step = [&](auto PAR, int s) {
     const char* nb = smem + ((s + 1) & (GP_RING - 1)) * GP_BUF;
-    mm_step<NI, D, decltype(PAR)::value>(
-        acc, cs, fa, fb, [&](int i) { stage(i, s + GP_RING - 1); }, [&](int i) { return load_a(i, nb); },
-        [&](int j) { return load_b(j, nb); }, [&]() { extra(PAR, s); });
+    const int take = __builtin_amdgcn_readfirstlane(turn == 0 ? 1 : 0);
+    turn = __builtin_amdgcn_readfirstlane(turn == 0 ? period - 1 : turn - 1);
+    mm_step<NI, D, WAIT, decltype(PAR)::value>(
+        acc, cs, take, fa, fb, [&](int i) { stage(i, s + GP_RING - 1); }, [&](int i) { return load_a(i, nb); },
+        [&](int j) { return load_b(j, nb); }, [&](int k) { extra(PAR, s, k); });
   };
   for (int s = 0; s < ns; s += 2) {
     step(std::integral_constant<int, 0>{}, s);
@@ -925,9 +959,13 @@ __device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32
   *reinterpret_cast<uint4*>(p) = make_uint4(a, b, c, d);
 }
 
-// the parts' column sums, behind their tiles: [lane][row of tiles][first, second part][256]
-__device__ __forceinline__ float* wg_sums(const GroupWgArgs& g, int tiles, int lanes) {
-  return g.ws + (size_t)2 * lanes * tiles * GW_SLAB;
+// db: the waves that hold the same rows of dz take turns with its steps (wave wc of tile column tk those with s %
+// (2 tiles_k) == 2 tk + wc), and leave 256 sums for each group and lane, behind the tiles of the workspace:
+// [group + lane][row of tiles][tile column, wave][256].  (group + lane tells the parts of the line
+// apart: from one to the next, one of the two grows.)
+__host__ __device__ __forceinline__ size_t wg_slabs(int tiles, int lanes) { return lanes > 1 ? (size_t)2 * lanes * tiles * GW_SLAB : 0; }
+__device__ __forceinline__ float* wg_sums(const GroupWgArgs& g, int tiles_n, int tiles_k, int lanes, int part, int tn) {
+  return g.ws + wg_slabs(tiles_n * tiles_k, lanes) + ((size_t)part * tiles_n + tn) * 2 * tiles_k * GP_B;
 }
 
 template <bool X8, bool GATHER>
@@ -938,7 +976,9 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   const int wr = wave >> 1, wc = wave & 1;
   const int tiles = tiles_n * tiles_k;
   const int w = xcd_order(blockIdx.x, gridDim.x);
-  const int U = wg_units(g.offs, g.E, g.S), u0 = wg_cut(U, lanes, w / tiles), u1 = wg_cut(U, lanes, w / tiles + 1);
+  const int U = wg_units(g.offs, g.E, g.S), L = min(lanes, U);       // (fewer rows than S: no lane without a unit)
+  if (w / tiles >= L) return;
+  const int u0 = wg_cut(U, L, w / tiles), u1 = wg_cut(U, L, w / tiles + 1);
   int tn, tk;
   band_tile(w % tiles, tiles_n, tiles_k, tn, tk);
   const int n0 = tn * GP_B, k0 = tk * GP_B;
@@ -1032,19 +1072,18 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       cd[set][1] = *reinterpret_cast<const uint4*>(x1 ? q + 16 : q);
       cs[set] = g.xs[at * sblk + (x0 ? (k0 + xc) / A8_BLOCK : 0)];
     };
-    auto codes_to = [&](int set, int s) {
-      char* d = smem + (s & (GP_RING - 1)) * GP_BUF;
+    // (in four pieces of 16 bytes)
+    auto codes_put = [&](int set, int s, int q) {
       const float f = a8_scale(cs[set]);
       const uint32_t m = con[set];
+      const uint4 v = cd[set][q >> 1];
+      const uint32_t a = ((q & 1) ? v.z : v.x) & m, b = ((q & 1) ? v.w : v.y) & m;
+      lds_put(smem + (s & (GP_RING - 1)) * GP_BUF + (xo ^ ((q >> 1) << 5)) + (q & 1) * 16, a8_pair_bf16<false>(a, f),
+              a8_pair_bf16<true>(a, f), a8_pair_bf16<false>(b, f), a8_pair_bf16<true>(b, f));
+    };
+    auto codes_to = [&](int set, int s) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 c = make_uint4(cd[set][h].x & m, cd[set][h].y & m, cd[set][h].z & m, cd[set][h].w & m);
-        char* o = d + (xo ^ (h << 5));
-        lds_put(o, a8_pair_bf16<false>(c.x, f), a8_pair_bf16<true>(c.x, f), a8_pair_bf16<false>(c.y, f),
-                a8_pair_bf16<true>(c.y, f));
-        lds_put(o + 16, a8_pair_bf16<false>(c.z, f), a8_pair_bf16<true>(c.z, f), a8_pair_bf16<false>(c.w, f),
-                a8_pair_bf16<true>(c.w, f));
-      }
+      for (int q = 0; q < 4; ++q) codes_put(set, s, q);
     };
     // (la and lb are hidden from the optimizer in every step: 16 addresses made by one xor each, not kept)
     auto hide = [&]() {
@@ -1060,8 +1099,9 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       rows_of(0, 0);
       rows_of(1, 1);
       if constexpr (X8) {
-        // the codes of step s + 3 (read in step s - 2) go to the image in step s, those of s + 5 are read;
-        // they are in LDS before the fragments read at the end of step s, so before step s + 2 reads them
+        // the codes of step s + 3 (read in step s - 2) go to the image in step s, in pieces between the MFMAs, and then those of s + 5 are read; they are in LDS before
+        // the last fragment of step s is read, so before step s + 2 reads them.  At a step's top 3 + 4 + 3 loads
+        // follow the DMA that it waits for: two steps' codes and one's DMA.
         codes_of(0, 0);
         codes_of(1, 1);
         codes_to(0, 0);
@@ -1075,36 +1115,37 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         codes_of(0, 4);
         rows_of(1, 5);
         rows_of(0, 6);
-        mm_loop<4, 4>(smem, ns, acc, sum, piece_a, load_a, load_b, [&](auto PAR, int s) {
+        mm_loop<4, 4, 10>(smem, ns, acc, sum, 2 * tk + wc, 2 * tiles_k, piece_a, load_a, load_b, [&](auto PAR, int s, int k) {
           constexpr int set = decltype(PAR)::value ^ 1;
-          hide();
-          codes_to(set, s + 3);
-          codes_of(set, s + 5);
-          rows_of(set, s + 7);
+          if (k == -1) hide();
+          if (k >= 0 && k % 6 == 5 && k / 6 < 4) codes_put(set, s + 3, k / 6);
+          if (k == 29) {
+            codes_of(set, s + 5);
+            rows_of(set, s + 7);
+          }
         });
       } else {
         // GATHER: a step's rows are read two steps before its DMA starts
-        mm_loop<4, 8>(
-            smem, ns, acc, sum,
+        mm_loop<4, 8, 8>(
+            smem, ns, acc, sum, 2 * tk + wc, 2 * tiles_k,
             [&](int i, int s) {
               if (i < 4) piece_a(i, s);
               else piece_b(i - 4, s, xrow[s & 1][i - 4]);
               if (i == 7) rows_of(s & 1, s + 2);
             },
-            load_a, load_b, [&](auto, int) { hide(); });
+            load_a, load_b, [&](auto, int, int k) { if (k == -1) hide(); });
       }
     }
     __syncthreads();                      // (the next part's staging overwrites what was read here)
     // a whole tile goes to dw, a part to the workspace: slot 2 w if it is the workgroup's first, 2 w + 1
     // if it goes on in the next one
     const bool whole = s0 == 0 && s1 == steps;
-    if (g.db && tk == 0 && wc == 0) {
-      float* d = whole ? g.db + (size_t)e * g.N : wg_sums(g, tiles, lanes) + (size_t)(2 * (w / tiles * tiles_n + tn) + (s0 > 0 ? 0 : 1)) * GP_B - n0;
+    if (g.db) {
+      float* d = wg_sums(g, tiles_n, tiles_k, lanes, e + w / tiles, tn) + (2 * tk + wc) * GP_B + wr * 128;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int n = n0 + wr * 128 + i * 32 + (lane & 31);
         const float v = sum[i] + __shfl_xor(sum[i], 32);
-        if (lane < 32 && (!whole || n < g.N)) d[n] = v;
+        if (lane < 32) d[i * 32 + lane] = v;
       }
     }
     if (whole)
@@ -1115,21 +1156,27 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   }
 }
 
-// Groups that two or more lanes made: their parts in row order.  grid (tiles, E, 16 strips of 16 rows).
+// Groups that two or more lanes made: their parts in row order; db of all.  grid (tiles, E, 16 strips of 16
+// rows, or 1 for db alone).
 __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes, int ovec) {
   const int tiles = tiles_n * tiles_k, ti = blockIdx.x, e = blockIdx.y;
-  const int U = wg_units(g.offs, g.E, g.S), rows0 = wg_units(g.offs, e, g.S) + GW_SEG, steps = wg_steps(g.offs, e, g.S);
-  const int l0 = wg_owner(U, lanes, rows0), l1 = wg_owner(U, lanes, rows0 + steps - 1);
-  if (l0 == l1) return;
   int tn, tk;
   band_tile(ti, tiles_n, tiles_k, tn, tk);
+  const bool sums = g.db && tk == 0 && blockIdx.z == 0;
+  if (lanes == 1 && !sums) return;
+  const int U = wg_units(g.offs, g.E, g.S), rows0 = wg_units(g.offs, e, g.S) + GW_SEG, steps = wg_steps(g.offs, e, g.S);
+  const int L = min(lanes, U), l0 = wg_owner(U, L, rows0), l1 = wg_owner(U, L, rows0 + steps - 1);
   const int n0 = tn * GP_B, k0 = tk * GP_B;
-  if (g.db && tk == 0 && blockIdx.z == 0 && n0 + (int)threadIdx.x < g.N) {
-    const float* s = wg_sums(g, tiles, lanes) + (size_t)2 * (l0 * tiles_n + tn) * GP_B + threadIdx.x;
-    float v = s[GP_B];
-    for (int l = l0 + 1; l <= l1; ++l) v += s[(size_t)2 * (l - l0) * tiles_n * GP_B];
+  if (sums && n0 + (int)threadIdx.x < g.N) {
+    float v = 0.f;
+    for (int l = l0; l <= l1; ++l) {
+      const float* s = wg_sums(g, tiles_n, tiles_k, lanes, e + l, tn) + threadIdx.x;
+#pragma unroll 8
+      for (int i = 0; i < 2 * tiles_k; ++i) v += s[i * GP_B];
+    }
     g.db[(size_t)e * g.N + n0 + threadIdx.x] = v;
   }
+  if (l0 == l1) return;
   // the lane that starts the group left it in its second tile, the others in their first
   const float* s0 = g.ws + (size_t)(2 * (l0 * tiles + ti) + 1) * GW_SLAB;
   const float* s1 = g.ws + (size_t)(2 * ((l0 + 1) * tiles + ti)) * GW_SLAB;
@@ -1187,10 +1234,10 @@ static int wgrad_lanes(const GroupWgArgs& g) {
   }
   return best;
 }
-// Two parts a workgroup, and their sums.  A single lane cuts no group.
+// Two parts a workgroup (a single lane cuts no group), and the sums for db.
 static long wgrad_ws_floats(const GroupWgArgs& g) {
   const long l = wgrad_lanes(g), tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
-  return l == 1 ? 0 : 2 * l * tn * (tk * GW_SLAB + GP_B);
+  return (long)wg_slabs((int)(tn * tk), (int)l) + (g.db ? (g.E + l) * tn * 2 * tk * GP_B : 0);
 }
 
 // Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
@@ -1218,15 +1265,15 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   if (wgrad_big(g)) {
     const int tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
     const int lanes = wgrad_lanes(g);
-    if (lanes > 1 && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    if ((lanes > 1 || g.db) && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
     const dim3 grid((unsigned)(tn * tk * lanes)), blk(GP_THREADS);
     if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, lanes);
     else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk, lanes);
     else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk, lanes);
     else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, lanes);
-    if (lanes > 1)
-      hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, 16), dim3(256), 0, st, g, tn, tk, lanes, ovec);
+    if (lanes > 1 || g.db)
+      hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, lanes > 1 ? 16 : 1), dim3(256), 0, st, g, tn, tk, lanes, ovec);
     HFM_LAUNCH_CHECK();
   }
   g.ns = wgrad_splits(g.S, g.N, g.K, g.E);

@@ -382,6 +382,31 @@ LARGE = [([9000, 0, 257, 1, 5000, 256], 200, 1032), ([20000], 64, 777), ([3] * 1
          ([1, 0, 30000], 136, 264), ([5000, 6000], 512, 1000)]
 
 
+@pytest.mark.parametrize("sizes", [[10], [300], [40, 700], [0, 130, 1], [64 * 9 + 1, 64 * 5], [1] * 6, [0, 0]])
+@pytest.mark.parametrize("x8", [False, True])
+def test_weight_gradient_of_few_rows_in_a_large_order(sizes, x8):
+    """Room for many rows, few of them live: the split over rows is planned on the room."""
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(len(sizes))
+    S, N, K = 16384, 512, 768
+    offs = torch.tensor([0] + sizes).cumsum(0)
+    dz = torch.randn(S, N, device=DEV, generator=g).bfloat16()
+    x = torch.randn(S, K, device=DEV, generator=g).bfloat16()
+    live = int(offs[-1])
+    dz[live:], x[live:] = math.nan, math.nan
+    a = A8.pack(x) if x8 else x
+    xv = (A8.unpack(a, torch.float32) if x8 else x).double()
+    nan = torch.full((1 << 28,), math.nan, device=DEV)         # what the workspace may hold
+    del nan
+    dw, db = EX.group_wgrad(dz, a, offs.int().to(DEV))
+    for e in range(len(sizes)):
+        lo, hi = int(offs[e]), int(offs[e + 1])
+        z, v = dz[lo:hi].double(), xv[lo:hi]
+        c = (hi - lo + 4) * 2.0 ** -23
+        assert bool(((dw[e].double() - z.T @ v).abs() <= c * (z.abs().T @ v.abs())).all()), e
+        assert bool(((db[e].double() - z.sum(0)).abs() <= c * z.abs().sum(0)).all()), e
+
+
 @pytest.mark.parametrize("sizes,K,N", LARGE)
 def test_group_products_many_tiles(sizes, K, N):
     """The same three products where the output has many tiles (the large-tile kernels)."""
