@@ -475,9 +475,9 @@ HFM_API int hfm_route_bwd_args_bytes() { return (int)sizeof(RouteBwdArgs); }
 // One wave per token, 16 bytes per lane and turn, a row's last elements (fewer than 16 bytes) one by one;
 // a token's row is read once for all its slots (dispatch, combine_bwd), or its slots' rows summed in
 // order (combine, dispatch_bwd).  Bound by the rows' bytes.  A 16-byte access of global memory may start at
-// any element: rows of an odd width take the same accesses as aligned ones (10007 rows of 313 floats with
-// 4 slots, the four exchanges: 88 us, 95 with single elements, 3 TB/s; 16384 rows of 1248 bf16 with 2 slots: 118
-// us, 4.2 TB/s).
+// any element: rows of an odd width take the same accesses as aligned ones.  The four exchanges together: 10007
+// rows of 313 floats with 4 slots 77 us, 3.3 TB/s (with single elements 95; with one turn's loads at a time 87);
+// 16384 rows of 1248 bf16 with 2 slots 112 us, 4.4 TB/s (one turn's: 118).
 struct ExchArgs {
   const void* a;           // x / dxs / ys / dy
   const void* b;           // combine_bwd: ys
@@ -494,66 +494,60 @@ template <typename T, int V>
 struct RowVec {               // (aligned to an element only)
   typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
-template <typename T, int V>
-__device__ __forceinline__ void row_load(const T* p, float (&f)[V]) {
-  typename RowVec<T, V>::type v = *reinterpret_cast<const typename RowVec<T, V>::type*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = (float)v[i];
-}
-template <typename T, int V>
-__device__ __forceinline__ void row_store(T* p, const float (&f)[V]) {
-  typename RowVec<T, V>::type v;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = (T)f[i];
-  *reinterpret_cast<typename RowVec<T, V>::type*>(p) = v;
-}
-
 enum { EX_DISPATCH = 0, EX_DISPATCH_BWD = 1, EX_COMBINE = 2, EX_COMBINE_BWD = 3 };
 
-// Columns c .. c + V - 1 of token t's rows.
-template <typename T, int V, int K, int MODE>
-__device__ __forceinline__ void exchange_cols(const ExchArgs& a, int t, int c, const int (&p)[K], const float (&w)[K],
+// Columns c + 64 V u .. + V - 1 of token t's rows, for the U turns u of them that lie before `end`; all rows'
+// loads of the U turns are under way before any is used.
+template <typename T, int V, int U, int K, int MODE>
+__device__ __forceinline__ void exchange_cols(const ExchArgs& a, int t, int c, int end, const int (&p)[K], const float (&w)[K],
                                               float (&dot)[K]) {
-  const T* A = reinterpret_cast<const T*>(a.a);
-  const T* B = reinterpret_cast<const T*>(a.b);
-  T* O = reinterpret_cast<T*>(a.out);
-  if (MODE == EX_DISPATCH) {
-    typedef typename RowVec<T, V>::type vec;
-    const vec v = *reinterpret_cast<const vec*>(A + (size_t)t * a.lda + c);
+  const T* __restrict__ A = reinterpret_cast<const T*>(a.a) + c;
+  const T* __restrict__ B = reinterpret_cast<const T*>(a.b) + c;
+  T* __restrict__ O = reinterpret_cast<T*>(a.out) + c;
+  typedef typename RowVec<T, V>::type vec;
+  auto at = [&](const T* x, size_t row, long ld, int u) -> vec { return *reinterpret_cast<const vec*>(x + row * ld + u * 64 * V); };
+  auto on = [&](int u) { return u == 0 || c + u * 64 * V < end; };
+  vec g[U], y[U][K];
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (p[j] >= 0) *reinterpret_cast<vec*>(O + (size_t)p[j] * a.ldo + c) = v;
-  } else if (MODE == EX_COMBINE_BWD) {
-    float g[V], y[K][V];
-    row_load<T, V>(A + (size_t)t * a.lda + c, g);
+  for (int u = 0; u < U; ++u) {
+    if (!on(u)) continue;
+    if (MODE == EX_DISPATCH || MODE == EX_COMBINE_BWD) g[u] = at(A, t, a.lda, u);
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (p[j] >= 0) row_load<T, V>(B + (size_t)p[j] * a.ldb + c, y[j]);
+    for (int j = 0; j < K; ++j) {
+      if (MODE == EX_COMBINE_BWD && p[j] >= 0) y[u][j] = at(B, p[j], a.ldb, u);
+      if ((MODE == EX_COMBINE || MODE == EX_DISPATCH_BWD) && p[j] >= 0) y[u][j] = at(A, p[j], a.lda, u);
+    }
+  }
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (p[j] >= 0) {
-        float d[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          d[i] = w[j] * g[i];
-          dot[j] = fmaf(g[i], y[j][i], dot[j]);
-        }
-        row_store<T, V>(O + (size_t)p[j] * a.ldo + c, d);
-      }
-  } else {
-    float s[V], y[K][V];
+  for (int u = 0; u < U; ++u) {
+    if (!on(u)) continue;
+    float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (p[j] >= 0) row_load<T, V>(A + (size_t)p[j] * a.lda + c, y[j]);
+    for (int j = 0; j < K; ++j) {
+      if (p[j] < 0) continue;
+      if (MODE == EX_DISPATCH) {
+        *reinterpret_cast<vec*>(O + (size_t)p[j] * a.ldo + u * 64 * V) = g[u];
+      } else if (MODE == EX_COMBINE_BWD) {
+        vec d;
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (p[j] >= 0) {
+        for (int i = 0; i < V; ++i) {
+          d[i] = (T)(w[j] * (float)g[u][i]);
+          dot[j] = fmaf((float)g[u][i], (float)y[u][j][i], dot[j]);
+        }
+        *reinterpret_cast<vec*>(O + (size_t)p[j] * a.ldo + u * 64 * V) = d;
+      } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = MODE == EX_COMBINE ? fmaf(w[j], y[j][i], s[i]) : s[i] + y[j][i];
+        for (int i = 0; i < V; ++i) s[i] = MODE == EX_COMBINE ? fmaf(w[j], (float)y[u][j][i], s[i]) : s[i] + (float)y[u][j][i];
       }
-    row_store<T, V>(O + (size_t)t * a.ldo + c, s);
+    }
+    if (MODE == EX_COMBINE || MODE == EX_DISPATCH_BWD) {
+      vec d;
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = (T)s[i];
+      *reinterpret_cast<vec*>(O + (size_t)t * a.ldo + u * 64 * V) = d;
+    }
   }
 }
 
@@ -573,12 +567,13 @@ __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
     dot[j] = 0.f;
   }
   const int D16 = a.D / V * V;
-  for (int c = lane * V; c < D16; c += 64 * V) exchange_cols<T, V, K, MODE>(a, t, c, p, w, dot);
-  if (D16 + lane < a.D) exchange_cols<T, 1, K, MODE>(a, t, D16 + lane, p, w, dot);
+  constexpr int U = K <= 4 && MODE != EX_DISPATCH ? 2 : 1;           // (dispatch has one load a turn)
+  for (int c = lane * V; c < D16; c += U * 64 * V) exchange_cols<T, V, U, K, MODE>(a, t, c, D16, p, w, dot);
+  if (D16 + lane < a.D) exchange_cols<T, 1, 1, K, MODE>(a, t, D16 + lane, a.D, p, w, dot);
   if (MODE == EX_COMBINE_BWD) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      for (int d = 32; d; d >>= 1) dot[j] += __shfl_xor(dot[j], d);
+      dot[j] = group_all<64>(dot[j], [](float x, float y) { return x + y; });
       if (lane == 0 && j < a.k) a.dweight[(size_t)t * a.k + j] = p[j] >= 0 ? dot[j] : 0.f;
     }
   }
