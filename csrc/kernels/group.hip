@@ -1156,8 +1156,9 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   }
 }
 
-// Groups that two or more lanes made: their parts in row order; db of all.  grid (tiles, E, 16 strips of 16
-// rows, or 1 for db alone).
+// Groups that two or more lanes made: their parts in row order; db of all.  grid (tiles, E, strips of 4 R rows, or
+// 1 for db alone).
+template <int R>
 __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes, int ovec) {
   const int tiles = tiles_n * tiles_k, ti = blockIdx.x, e = blockIdx.y;
   int tn, tk;
@@ -1181,19 +1182,28 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
   const float* s0 = g.ws + (size_t)(2 * (l0 * tiles + ti) + 1) * GW_SLAB;
   const float* s1 = g.ws + (size_t)(2 * ((l0 + 1) * tiles + ti)) * GW_SLAB;
   const size_t next = (size_t)2 * tiles * GW_SLAB;
-  const int r0 = blockIdx.z * 16 + (threadIdx.x >> 6), c = (threadIdx.x & 63) * 4;
-  f32x4 v[4];
+  const int r0 = blockIdx.z * (4 * R) + (threadIdx.x >> 6), c = (threadIdx.x & 63) * 4;
+  f32x4 v[R];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4*>(s0 + (r0 + 4 * i) * GP_B + c);
-  for (int l = l0 + 1; l <= l1; ++l, s1 += next) {
-    f32x4 a[4];
+  for (int i = 0; i < R; ++i) v[i] = *reinterpret_cast<const f32x4*>(s0 + (r0 + 4 * i) * GP_B + c);
+  int l = l0 + 1;
+  for (; l + 3 <= l1; l += 4, s1 += 4 * next) {             // (four parts' loads at a time, summed in order)
+    f32x4 a[4][R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const f32x4*>(s1 + (r0 + 4 * i) * GP_B + c);
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += a[i];
+      for (int i = 0; i < R; ++i) a[m][i] = *reinterpret_cast<const f32x4*>(s1 + m * next + (r0 + 4 * i) * GP_B + c);
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] += a[m][i];
+  }
+  for (; l <= l1; ++l, s1 += next) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] += *reinterpret_cast<const f32x4*>(s1 + (r0 + 4 * i) * GP_B + c);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int r = r0 + 4 * i;
     if (n0 + r >= g.N || k0 + c >= g.K) continue;
     float* d = g.dw + ((size_t)e * g.N + n0 + r) * g.K + k0 + c;
@@ -1208,7 +1218,9 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
 }
 
 // Where the large tile is taken: operands with 16-byte rows, and enough work for every CU (GP_MIN_UNITS
-// steps of 64 rows each; below that the 128 x 128 tile's smaller pieces fill the chip better).
+// steps of 64 rows each; below that the 128 x 128 tile's smaller pieces fill the chip better).  128 x 128 against
+// 256 x 256 in us, one group: 16384 rows, 256 x 256: 32, 44; 32768: 48, 56; 1024 rows, 1024 x 1024: 28, 26; 4096: 52,
+// 35; 16384: 145, 58; 4 groups, 4096 rows, 512 x 512: 38, 35; 16 groups, 32768 rows, 1024 x 1024: 290, 115.
 constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
 static bool wgrad_big(const GroupWgArgs& g) {
   const bool x8 = g.xs != nullptr;
@@ -1218,16 +1230,22 @@ static bool wgrad_big(const GroupWgArgs& g) {
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
   return tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS;
 }
-// Lanes: the fewest rounds of the CUs times a lane's length (its rows, and one group's own cost), within
-// 512 workgroups (a workspace of 256 MB) unless the tiles alone are more.
+// Time in us by l lanes: the rounds of the CUs times a lane's length (its rows, and a group's own cost); then
+// the parts' way through the workspace (0.065 us each, as many as there are cuts through rows) and the
+// longest sum of them.
+static double wgrad_time(const GroupWgArgs& g, long tiles, int l) {
+  const double rows = (double)(g.S / GW_UNIT) + g.E, units = rows + (double)g.E * GW_SEG;
+  const double t = (double)((l * tiles + GW_CUS - 1) / GW_CUS) * (units / l + GW_SEG) * 1.7;
+  return l == 1 ? t : t + 6 + 2 * (l - 1) * (rows / units) * tiles * 0.065 + ((double)l / g.E + 1) * 0.3;
+}
+// Lanes: the least time within 512 workgroups (a workspace of 256 MB) unless the tiles alone are more.
 static int wgrad_lanes(const GroupWgArgs& g) {
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
-  const double units = (double)(g.S / GW_UNIT) + (double)g.E * (1 + GW_SEG);
   int best = 1;
-  double least = 0.0;
-  for (int l = 1; l == 1 || l * tiles <= 512; ++l) {
-    const double t = (double)((l * tiles + GW_CUS - 1) / GW_CUS) * (units / l + GW_SEG);
-    if (l == 1 || t < least) {
+  double least = wgrad_time(g, tiles, 1);
+  for (int l = 2; l * tiles <= 512; ++l) {
+    const double t = wgrad_time(g, tiles, l);
+    if (t < least) {
       least = t;
       best = l;
     }
@@ -1272,8 +1290,13 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
     else if (g.xs) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, false>), grid, blk, 0, st, g, tn, tk, lanes);
     else if (g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<false, true>), grid, blk, 0, st, g, tn, tk, lanes);
     else hipLaunchKernelGGL((group_wgrad_mm_kernel<false, false>), grid, blk, 0, st, g, tn, tk, lanes);
-    if (lanes > 1 || g.db)
-      hipLaunchKernelGGL(group_wgrad_join_kernel, dim3(tn * tk, g.E, lanes > 1 ? 16 : 1), dim3(256), 0, st, g, tn, tk, lanes, ovec);
+    if (lanes > 1 || g.db) {
+      // (16 rows a workgroup, or 4 where that leaves CUs without one: 32768 rows, 256 x 256: 67 us in all, 56 so)
+      if ((long)tn * tk * g.E * 16 >= GW_CUS)
+        hipLaunchKernelGGL(group_wgrad_join_kernel<4>, dim3(tn * tk, g.E, lanes > 1 ? 16 : 1), dim3(256), 0, st, g, tn, tk, lanes, ovec);
+      else
+        hipLaunchKernelGGL(group_wgrad_join_kernel<1>, dim3(tn * tk, g.E, lanes > 1 ? 64 : 1), dim3(256), 0, st, g, tn, tk, lanes, ovec);
+    }
     HFM_LAUNCH_CHECK();
   }
   g.ns = wgrad_splits(g.S, g.N, g.K, g.E);
