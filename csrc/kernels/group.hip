@@ -101,30 +101,52 @@ __device__ __forceinline__ int group_row(const int* src, int p, int rows, int to
   return s >= 0 && r < rows ? r : -1;
 }
 
-// 8 elements of a row from column c, zeros past n (VEC: 16-byte aligned, n a multiple of 8)
-template <bool VEC>
+// 8 elements of a row of n from column c, zeros past n.  The access may start at any element (192 rows of 8 experts,
+// 1249 -> 400: 97 us by single elements, 15 so).
+typedef bf16 any_bf16x8 __attribute__((ext_vector_type(8), aligned(2)));
 __device__ __forceinline__ bf16x8 load8_bf(const bf16* row, int c, int n) {
   bf16x8 v = {};
   if (!row || c >= n) return v;
-  if (VEC) return *reinterpret_cast<const bf16x8*>(row + c);
+  if (c + 8 <= n) return __builtin_bit_cast(bf16x8, *reinterpret_cast<const any_bf16x8*>(row + c));
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 7; ++j)
     if (c + j < n) v[j] = row[c + j];
   return v;
 }
-template <bool VEC>
-__device__ __forceinline__ uint2 load8_code(const uint8_t* row, int c, int n) {
-  uint2 v = make_uint2(0, 0);
+// The same in two halves, for many rows at the same columns: a load that ends with the row, and what moves the row's
+// last elements to their place once all loads are under way (the loads of a last piece's elements would wait
+// for the others: 3000 rows of 4 groups, 999 x 1001: 133 us, 72 so).  WHOLE: n is a multiple of 8, there is no
+// second half (4096 rows of 4 groups, 512 x 512: 31 us, with it 46).
+template <bool WHOLE>
+__device__ __forceinline__ bf16x8 begin8_bf(const bf16* row, int c, int n) {
+  bf16x8 v = {};
   if (!row || c >= n) return v;
-  if (VEC) return *reinterpret_cast<const uint2*>(row + c);
+  if (WHOLE || n >= 8) return __builtin_bit_cast(bf16x8, *reinterpret_cast<const any_bf16x8*>(row + (WHOLE ? c : min(c, n - 8))));
+  return load8_bf(row, c, n);
+}
+__device__ __forceinline__ void end8_bf(bf16x8& v, int c, int n) {
+  const int bits = (c + 8 - n) * 16;
+  if (bits <= 0 || n < 8) return;
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  u64x2 u = __builtin_bit_cast(u64x2, v);
+  u[0] = bits < 64 ? u[0] >> bits | u[1] << (64 - bits) : bits < 128 ? u[1] >> (bits - 64) : 0;
+  u[1] = bits < 64 ? u[1] >> bits : 0;
+  v = __builtin_bit_cast(bf16x8, u);
+}
+template <bool WHOLE>
+__device__ __forceinline__ uint64_t begin8_code(const uint8_t* row, int c, int n) {
+  typedef uint64_t any8 __attribute__((aligned(1)));
+  uint64_t v = 0;
+  if (!row || c >= n) return v;
+  if (WHOLE || n >= 8) return *reinterpret_cast<const any8*>(row + (WHOLE ? c : min(c, n - 8)));
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < n) {
-      const uint32_t b = row[c + j];
-      if (j < 4) v.x |= b << (8 * j);
-      else v.y |= b << (8 * (j - 4));
-    }
+  for (int j = 0; j < 7; ++j)
+    if (c + j < n) v |= (uint64_t)row[c + j] << (8 * j);
   return v;
+}
+__device__ __forceinline__ void end8_code(uint64_t& v, int c, int n) {
+  const int bits = (c + 8 - n) * 8;
+  if (bits > 0 && n >= 8) v = bits < 64 ? v >> bits : 0;
 }
 
 // One output of the NT product: scale, bias, relu (NaN stays), mask, rounding.
@@ -148,7 +170,6 @@ __device__ __forceinline__ void group_put(const GroupNtArgs& g, int p, int n, fl
 // LDS image: rows of 64 elements (128 B), 16-byte chunk c of row r at c ^ ((r >> 1) & 7).
 constexpr int GN_B = 128, GN_K = 64, GN_PANEL = GN_B * GN_K * 2;
 
-template <bool VEC>
 __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_n) {
   __shared__ __attribute__((aligned(16))) char smem[4 * GN_PANEL];
   int e, r0, r1;
@@ -177,8 +198,8 @@ __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      ra[i] = load8_bf<VEC>(pa[i], k0 + ch * 8, g.K);
-      rb[i] = load8_bf<VEC>(pb[i], k0 + ch * 8, g.K);
+      ra[i] = load8_bf(pa[i], k0 + ch * 8, g.K);
+      rb[i] = load8_bf(pb[i], k0 + ch * 8, g.K);
     }
   };
   auto stage = [&](int buf) {
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(256) group_nt_kernel(GroupNtArgs g, int tiles_
 // (together they read 256 neighbouring bytes of a row), fragments straight from memory, 8 steps under way at
 // once, and the 8 partial tiles are summed through LDS.  A request's rows leave a larger tile with a
 // handful of workgroups that go through the whole reduction one after another: 192 rows, 8 experts,
-// 1248 -> 400: 25 us by the 128 x 128 tile, 6.2 here.  Where rows and columns have 16-byte chunks.
+// 1248 -> 400: 25 us by the 128 x 128 tile, 6.2 here.
 constexpr int GS_B = 32, GS_WAVES = 8, GS_DEEP = 8;
 __global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs g, int tiles_n) {
   typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -253,8 +274,8 @@ __global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs
     bf16x8 fa[GS_DEEP], fb[GS_DEEP];
 #pragma unroll
     for (int i = 0; i < GS_DEEP; ++i) {
-      fa[i] = load8_bf<true>(a, k0 + i * GS_WAVES * 16, g.K);
-      fb[i] = load8_bf<true>(b, k0 + i * GS_WAVES * 16, g.K);
+      fa[i] = load8_bf(a, k0 + i * GS_WAVES * 16, g.K);
+      fb[i] = load8_bf(b, k0 + i * GS_WAVES * 16, g.K);
     }
 #pragma unroll
     for (int i = 0; i < GS_DEEP; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[i], acc, 0, 0, 0);
@@ -706,14 +727,13 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   // -> 1024: 20, 28; 2048: 35, 29; 5000 rows, 256 -> 1024: 35, 21; 8192 rows of 8 experts, 128 -> 64: 4.8, 17.
   const int fn = (g.N + GS_B - 1) / GS_B;
   const long few = (long)(g.S / GS_B + g.E) * fn;
-  if (vec && few <= 1l << 20 &&
+  if (few <= 1l << 20 &&
       few * g.K * (4.0 * GS_B / 8e6) < ceil(blocks / 512.0) * ((g.K + GN_K - 1) / GN_K) * 1.4) {
     hipLaunchKernelGGL(group_nt_few_kernel, dim3((unsigned)few), dim3(GS_WAVES * 64), 0, st, g, fn);
     HFM_LAUNCH_CHECK();
   }
   if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
-  if (vec) hipLaunchKernelGGL(group_nt_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
-  else hipLaunchKernelGGL(group_nt_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
+  hipLaunchKernelGGL(group_nt_kernel, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
   HFM_LAUNCH_CHECK();
 }
 
@@ -743,7 +763,7 @@ __device__ __forceinline__ void transpose8(const uint4 (&in)[8], uint4 (&out)[8]
   }
 }
 
-template <bool VEC, bool X8>
+template <bool WHOLE, bool X8>
 __global__ void __launch_bounds__(256) group_wgrad_kernel(GroupWgArgs g, int tiles_n, int tiles_k) {
   __shared__ __attribute__((aligned(16))) char smem[4 * GN_PANEL];
   int bid = blockIdx.x;
@@ -768,30 +788,47 @@ __global__ void __launch_bounds__(256) group_wgrad_kernel(GroupWgArgs g, int til
   const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
   uint4 in[8];
   auto fetch = [&](int pbase) {
+    uint64_t w[8];
+    uint32_t sc[8];
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
       const int p = pbase + mb * 8 + m;
       bf16x8 v = {};
       if (p < p1) {
         if (!isx) {
-          v = load8_bf<VEC>(g.dz + (size_t)p * g.ldz, col, g.N);
+          v = begin8_bf<WHOLE>(g.dz + (size_t)p * g.ldz, col, g.N);
         } else {
           const int row = group_row(g.src, p, g.rows, g.top_k);
-          if (row >= 0) {
-            if (X8) {
-              const uint2 w = load8_code<VEC>(reinterpret_cast<const uint8_t*>(g.x) + (size_t)row * g.ldx, col, g.K);
-              const float s = col < g.K ? a8_scale(g.xs[(size_t)row * sblk + col / A8_BLOCK]) : 0.f;
-              float f[8];
-              a8_unpack8(w, s, f);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = f2bf(f[j]);
-            } else {
-              v = load8_bf<VEC>(reinterpret_cast<const bf16*>(g.x) + (size_t)row * g.ldx, col, g.K);
-            }
+          if (X8) {
+            w[m] = row >= 0 ? begin8_code<WHOLE>(reinterpret_cast<const uint8_t*>(g.x) + (size_t)row * g.ldx, col, g.K) : 0;
+            sc[m] = row >= 0 && col < g.K ? g.xs[(size_t)row * sblk + col / A8_BLOCK] : 0;
+          } else if (row >= 0) {
+            v = begin8_bf<WHOLE>(reinterpret_cast<const bf16*>(g.x) + (size_t)row * g.ldx, col, g.K);
           }
         }
+      } else if (X8) {
+        w[m] = sc[m] = 0;
       }
-      in[m] = *reinterpret_cast<const uint4*>(&v);
+      in[m] = __builtin_bit_cast(uint4, v);
+    }
+    if (X8 && isx) {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        if (!WHOLE) end8_code(w[m], col, g.K);
+        float f[8];
+        a8_unpack8(make_uint2((uint32_t)w[m], (uint32_t)(w[m] >> 32)), a8_scale(sc[m]), f);
+        bf16x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = f2bf(f[j]);
+        in[m] = __builtin_bit_cast(uint4, v);
+      }
+    } else if (!WHOLE && col + 8 > (isx ? g.K : g.N)) {
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        bf16x8 v = __builtin_bit_cast(bf16x8, in[m]);
+        end8_bf(v, col, isx ? g.K : g.N);
+        in[m] = __builtin_bit_cast(uint4, v);
+      }
     }
   };
   auto stage = [&](int buf) {
@@ -1258,13 +1295,13 @@ static long wgrad_ws_floats(const GroupWgArgs& g) {
   return (long)wg_slabs((int)(tn * tk), (int)l) + (g.db ? (g.E + l) * tn * 2 * tk * GP_B : 0);
 }
 
-// Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 8 steps of
-// 64 rows on average.
+// Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 4 steps of 64 rows on
+// average (770 rows, 55 x 40: 21 us; with 8 steps: 42; 4096 rows of 4 groups, 512 x 512: 31, 40).
 static int wgrad_splits(int S, int N, int K, int E) {
   const long tiles = (long)E * ((N + GN_B - 1) / GN_B) * ((K + GN_B - 1) / GN_B);
   if (tiles <= 0) return 1;
   long ns = 512 / tiles;
-  const long most = (long)S / E / 512;
+  const long most = (long)S / E / 256;
   if (ns > most) ns = most;
   if (ns > 32) ns = 32;
   return ns < 1 ? 1 : (int)ns;
@@ -1301,18 +1338,15 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   }
   g.ns = wgrad_splits(g.S, g.N, g.K, g.E);
   if (g.ns > 1 && !g.ws) return (int)hipErrorInvalidValue;
-  const bool x8 = g.xs != nullptr;
-  const bool vec = (uintptr_t)g.dz % 16 == 0 && g.N % 8 == 0 && g.ldz % 8 == 0 && (uintptr_t)g.x % (x8 ? 8 : 16) == 0 &&
-                   g.K % 8 == 0 && g.ldx % 8 == 0;
   const int tn = (g.N + GN_B - 1) / GN_B, tk = g.K > 0 ? (g.K + GN_B - 1) / GN_B : 1;
   const long blocks = (long)tn * tk * g.E * g.ns;
   if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks), blk(256);
-  if (x8) {
-    if (vec) hipLaunchKernelGGL((group_wgrad_kernel<true, true>), grid, blk, 0, st, g, tn, tk);
-    else hipLaunchKernelGGL((group_wgrad_kernel<false, true>), grid, blk, 0, st, g, tn, tk);
+  if (g.N % 8 == 0 && g.K % 8 == 0) {
+    if (g.xs) hipLaunchKernelGGL((group_wgrad_kernel<true, true>), grid, blk, 0, st, g, tn, tk);
+    else hipLaunchKernelGGL((group_wgrad_kernel<true, false>), grid, blk, 0, st, g, tn, tk);
   } else {
-    if (vec) hipLaunchKernelGGL((group_wgrad_kernel<true, false>), grid, blk, 0, st, g, tn, tk);
+    if (g.xs) hipLaunchKernelGGL((group_wgrad_kernel<false, true>), grid, blk, 0, st, g, tn, tk);
     else hipLaunchKernelGGL((group_wgrad_kernel<false, false>), grid, blk, 0, st, g, tn, tk);
   }
   if (g.ns > 1) {
