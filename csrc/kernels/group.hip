@@ -29,6 +29,7 @@ struct GroupNtArgs {
   long lda, ldb, es, ldm, ldo;
   int S, rows, K, N, E, top_k, relu, mask8, out_f32;
   float scale;
+  void* ws;                // hfm_group_nt_ws_bytes
 };
 
 struct GroupWgArgs {
@@ -39,7 +40,7 @@ struct GroupWgArgs {
   const int* src;
   float* dw;               // [E, N, K]
   float* db;               // [E, N] or null
-  float* ws;               // [ns, E, N, K] + [ns, E, N] (ns > 1)
+  float* ws;               // hfm_group_wgrad_ws_floats
   long ldz, ldx;
   int S, rows, K, N, E, top_k, ns;
 };
@@ -148,6 +149,44 @@ __device__ __forceinline__ void end8_code(uint64_t& v, int c, int n) {
   const int bits = (c + 8 - n) * 8;
   if (bits > 0 && n >= 8) v = bits < 64 ? v >> bits : 0;
 }
+
+// Rows of any alignment into rows of whole 16-byte chunks, zeros behind their ends (and in place of rows that are
+// none), for the large tiles' LDS-DMA: a wave a row.  The copies cost the operands' bytes twice where the
+// 128 x 128 tile takes up to ten times as long as the large one.
+struct PadArgs {
+  const char* from;        // row r at from + (r / per) * gs + (r % per) * lds, or at `map`'s row
+  char* to;                // row r at to + r * ldd
+  const int* map;          // sources as in group_row, or null
+  long gs, lds, ldd, rows;
+  int per, bytes, have, top_k;
+};
+__global__ void __launch_bounds__(256) group_pad_kernel(PadArgs a) {
+  typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
+  const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int row = group_row(a.map, a.map ? (int)r : 0, a.have, a.top_k);
+  const char* from = a.map ? a.from + (size_t)max(row, 0) * a.lds : a.from + (size_t)(r / a.per) * a.gs + (size_t)(r % a.per) * a.lds;
+  char* to = a.to + (size_t)r * a.ldd;
+  for (int c = (threadIdx.x & 63) * 16; c < a.ldd; c += 1024) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row >= 0) {
+      if (c + 16 <= a.bytes) {
+        v = __builtin_bit_cast(uint4, *reinterpret_cast<const any16*>(from + c));
+      } else {
+        uint8_t b[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) b[i] = c + i < a.bytes ? (uint8_t)from[c + i] : 0;
+        __builtin_memcpy(&v, b, 16);
+      }
+    }
+    *reinterpret_cast<uint4*>(to + c) = v;
+  }
+}
+static void group_pad(const PadArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(group_pad_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+}
+constexpr long GROUP_PAD_MAX = 1l << 32;                   // (grid)
+static long up16(long bytes) { return (bytes + 15) / 16 * 16; }
 
 // One output of the NT product: scale, bias, relu (NaN stays), mask, rounding.
 __device__ __forceinline__ void group_put(const GroupNtArgs& g, int p, int n, float acc, float bias) {
@@ -471,11 +510,13 @@ __device__ __forceinline__ void mm_out_f32(const f32x16 (&acc)[4][4], float* bas
 // in fp32 as above, or in bf16 two columns a lane: the lanes of a column pair trade a row each
 // (pack two rows, one lane swap, one byte permute), so that a store is four rows' 64 B.
 // MASK 1: bf16 layer input, 2: its 8-bit codes; where that is not above zero the output is.
-template <int NI, int MASK, bool F32>
+// OUT: 0 bf16 in column pairs, 1 fp32, 2 bf16 one by one (rows or masks of odd widths).
+template <int NI, int MASK, int OUT>
 __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&acc)[NI][4], int e, int row0, int rows, int n0,
                                           int lane) {
   if (rows <= 0) return;
-  constexpr int ES = F32 ? 4 : 2, MS = MASK == 1 ? 2 : 1;
+  constexpr bool ONE = OUT != 0;
+  constexpr int ES = OUT == 1 ? 4 : 2, MS = MASK == 1 ? 2 : 1;
   const int fr = lane & 31, h = lane >> 5, odd = lane & 1;
   const int ldo = (int)g.ldo, ldm = (int)g.ldm, left = min(rows, 32 * NI);
   const __amdgpu_buffer_rsrc_t o = out_rows(reinterpret_cast<char*>(g.out) + (size_t)row0 * g.ldo * ES, (uint32_t)left * ldo * ES);
@@ -483,26 +524,26 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
       out_rows(reinterpret_cast<const char*>(g.mask) + (size_t)row0 * g.ldm * MS, (uint32_t)left * ldm * MS);
   const float lo = g.relu ? 0.f : -INFINITY;
   const uint32_t sel = odd ? 0x07060302u : 0x01000504u;
-  constexpr int NQ = F32 ? 16 : 8;
+  constexpr int NQ = ONE ? 16 : 8;
   auto row_of = [](int i, int q) {
-    const int k = F32 ? q : 2 * q;
+    const int k = ONE ? q : 2 * q;
     return i * 32 + (k >> 2) * 8 + (k & 3);
   };
   // a column block's mask, read while the one before it is written
   uint32_t m[2][NI][NQ];
-  const int rr = F32 ? h * 4 : h * 4 + odd;
+  const int rr = ONE ? h * 4 : h * 4 + odd;
   auto mask_of = [&](int j) {
     if (MASK == 0) return;
-    const int c = n0 + j * 32 + fr, cc = F32 ? c : c & ~1;
+    const int c = n0 + j * 32 + fr, cc = ONE ? c : c & ~1;
     const int mt = (int)(cc < g.N ? (uint32_t)(rr * ldm + cc) * MS : GP_FAR);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
         const int at = row_of(i, q) * ldm * MS;
-        if (MASK == 1) m[j & 1][i][q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, mt, at, 0)
+        if (MASK == 1) m[j & 1][i][q] = ONE ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, mt, at, 0)
                                             : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(mr, mt, at, 0);
-        if (MASK == 2) m[j & 1][i][q] = F32 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(mr, mt, at, 0)
+        if (MASK == 2) m[j & 1][i][q] = ONE ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(mr, mt, at, 0)
                                             : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(mr, mt, at, 0);
       }
   };
@@ -516,20 +557,20 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int c = n0 + j * 32 + fr;
-    const int cc = F32 ? c : c & ~1;
+    const int cc = ONE ? c : c & ~1;
     const uint32_t at = cc < g.N ? (uint32_t)(rr * ldo + cc) * ES : GP_FAR;
     if (j < 3) mask_of(j + 1);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const int k = F32 ? q : 2 * q;
+        const int k = ONE ? q : 2 * q;
         float v = __builtin_elementwise_maximum(fmaf(acc[i][j][k], g.scale, bias[j]), lo);
         uint32_t w;
-        if (F32) {
+        if (ONE) {
           if (MASK == 1 && !(__uint_as_float(m[j & 1][i][q] << 16) > 0.f)) v = 0.f;
           if (MASK == 2 && !a8_positive(m[j & 1][i][q])) v = 0.f;
-          w = __float_as_uint(v);
+          w = OUT == 1 ? __float_as_uint(v) : (uint32_t)__builtin_bit_cast(uint16_t, f2bf(v));
         } else {
           typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
           const float u = __builtin_elementwise_maximum(fmaf(acc[i][j][k + 1], g.scale, bias[j]), lo);
@@ -541,7 +582,8 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
                              (__uint_as_float(mv & 0xFFFF0000u) > 0.f ? w & 0xFFFF0000u : 0u);
           if (MASK == 2) w = (a8_positive(mv & 0xFFu) ? w & 0xFFFFu : 0u) | (a8_positive(mv >> 8) ? w & 0xFFFF0000u : 0u);
         }
-        __builtin_amdgcn_raw_buffer_store_b32(w, o, (int)at, row_of(i, q) * ldo * ES, 0);
+        if (OUT == 2) __builtin_amdgcn_raw_buffer_store_b16((uint16_t)w, o, (int)at, row_of(i, q) * ldo * ES, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(w, o, (int)at, row_of(i, q) * ldo * ES, 0);
       }
     }
   }
@@ -560,7 +602,7 @@ constexpr int GN2_K = 64, GN2_PANEL = GP_B * GN2_K * 2, GN2_BUF = 2 * GN2_PANEL;
 
 template <int NI>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
-group_nt_mm_kernel(GroupNtArgs g, int tiles_n) {
+group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
   __shared__ __attribute__((aligned(16))) char smem[2 * GN2_BUF];
   // (the grid has room for one more row tile per group: the tiles that there are go round the XCDs)
   const int tiles_m = group_tiles<64 * NI>(g.offs, g.E, g.S);
@@ -678,46 +720,99 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (nothing in flight into LDS at the end)
   const int row0 = r0 + wr * 32 * NI, n1 = n0 + wc * 128;
+#define HFM_OUT(MASK)                                                                   \
+  if (out == 0) mm_out_nt<NI, MASK, 0>(g, acc, e, row0, r1 - row0, n1, lane);           \
+  else if (out == 1) mm_out_nt<NI, MASK, 1>(g, acc, e, row0, r1 - row0, n1, lane);      \
+  else mm_out_nt<NI, MASK, 2>(g, acc, e, row0, r1 - row0, n1, lane);
   if (!g.mask) {
-    if (g.out_f32) mm_out_nt<NI, 0, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<NI, 0, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    HFM_OUT(0)
   } else if (!g.mask8) {
-    if (g.out_f32) mm_out_nt<NI, 1, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<NI, 1, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    HFM_OUT(1)
   } else {
-    if (g.out_f32) mm_out_nt<NI, 2, true>(g, acc, e, row0, r1 - row0, n1, lane);
-    else mm_out_nt<NI, 2, false>(g, acc, e, row0, r1 - row0, n1, lane);
+    HFM_OUT(2)
   }
+#undef HFM_OUT
+}
+
+// How a call runs: rows a large tile (0: none), and the bytes of the operands' copies for it.
+struct NtPlan {
+  int rows;
+  long pa, pb;
+};
+static NtPlan nt_plan(const GroupNtArgs& g) {
+  NtPlan p{0, 0, 0};
+  if (g.K < 64 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD) return p;
+  // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
+  // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
+  // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 117 at 192).
+  const int tn = (g.N + GP_B - 1) / GP_B;
+  const double step = 0.85 / 256 * ((g.K + GP_K - 1) / GP_K);
+  auto cost = [&](int rows) {
+    const double tiles = (g.E == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * g.E) * tn;
+    return ceil(tiles / 256) * (step * rows + 12.0);
+  };
+  const int rows = cost(192) < cost(256) ? 192 : 256;
+  const long blocks = (long)(g.S / rows + g.E) * tn;
+  if (blocks < GP_MIN_TILES || blocks > 0x7FFFFFFFl) return p;
+  // The LDS-DMA takes 16-byte chunks, and rows through 32-bit offsets (all of x where src says which, else 256 rows):
+  // operands that are otherwise are copied (x with its rows in order), where the copies at 4.5 TB/s and the large
+  // tile take less than the 128 x 128 tile (rounds of 512 tiles, 2.7 us a step and 10 more for such operands,
+  // half as much again with a mask).  Copies against 128 x 128 in us: 25092 rows of 2 experts, 2937 -> 3216 masked:
+  // 555, 1264; 32000 of 16, 255 -> 257 masked: 48, 95; 129 -> 131: 26, 41; 1500 of 16, 1001 -> 1501: 48, 39.
+  const bool whole = g.K % 8 == 0;
+  const bool a = !whole || (uintptr_t)g.a % 16 || g.lda % 8 || (g.src ? (long)g.rows * g.lda : 256l * g.lda) >= 0x7F000000l;
+  const bool b = !whole || (uintptr_t)g.b % 16 || g.ldb % 8 || g.es % 8 || 256l * g.ldb >= 0x7F000000l;
+  const long row = up16(2l * g.K);
+  if (a) p.pa = (long)g.S * row;
+  if (b) p.pb = (long)g.E * g.N * row;
+  if (a || b) {
+    const double t = (a + b) * 3.0 + (p.pa + p.pb) * (2.0 / 4.5e6) + cost(rows);
+    const double tiles = ((double)g.S / GN_B + 0.5 * g.E) * ((g.N + GN_B - 1) / GN_B);
+    const double small = ceil(tiles / 512) * (2.7 * ((g.K + GN_K - 1) / GN_K) + 10.0) * (g.mask ? 1.5 : 1.0);
+    if (t > small || g.S >= GROUP_PAD_MAX || (long)g.E * g.N >= GROUP_PAD_MAX) return NtPlan{0, 0, 0};
+  }
+  p.rows = rows;
+  return p;
+}
+
+HFM_API long hfm_group_nt_ws_bytes(const GroupNtArgs* gp) {
+  if (gp->S <= 0 || gp->K <= 0 || gp->N <= 0 || gp->E < 1) return 0;
+  const NtPlan p = nt_plan(*gp);
+  return p.pa + p.pb;
 }
 
 HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
-  const GroupNtArgs g = *gp;
+  GroupNtArgs g = *gp;
   if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
   if (g.S == 0 || g.N == 0) return 0;
-  const bool vec = ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && g.K % 8 == 0 && g.lda % 8 == 0 && g.ldb % 8 == 0 &&
-                   g.es % 8 == 0;
-  // the large tile stores (and reads the mask) in column pairs of bf16
-  const bool pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && g.ldm % 2 == 0 && (uintptr_t)g.out % 4 == 0 &&
-                     (uintptr_t)g.mask % (g.mask8 ? 2 : 4) == 0 && g.ldo < GP_MAXLD && g.ldm < GP_MAXLD;
-  // ... and takes rows through 32-bit offsets: all of x where src says which, else 256 rows
-  const bool near = (g.src ? (long)g.rows * g.lda : 256l * g.lda) < 0x7F000000l && 256l * g.ldb < 0x7F000000l && g.K < 0x7F00;
-  if (vec && pairs && near && g.K >= 64) {
-    // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
-    // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
-    // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 117 at 192).
-    const int tn = (g.N + GP_B - 1) / GP_B;
-    const double step = 0.85 / 256 * ((g.K + GP_K - 1) / GP_K);
-    auto cost = [&](int rows) {
-      const double tiles = (g.E == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * g.E) * tn;
-      return ceil(tiles / 256) * (step * rows + 12.0);
-    };
-    const int rows = cost(192) < cost(256) ? 192 : 256;
-    const long blocks = (long)(g.S / rows + g.E) * tn;
-    if (blocks >= GP_MIN_TILES && blocks <= 0x7FFFFFFFl) {
-      if (rows == 256) hipLaunchKernelGGL(group_nt_mm_kernel<4>, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
-      else hipLaunchKernelGGL(group_nt_mm_kernel<3>, dim3((unsigned)blocks), dim3(GP_THREADS), 0, st, g, tn);
-      HFM_LAUNCH_CHECK();
+  const NtPlan p = nt_plan(g);
+  if (p.rows) {
+    if (p.pa + p.pb > 0 && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    const long row = up16(2l * g.K);
+    char* ws = reinterpret_cast<char*>(g.ws);
+    if (p.pa) {
+      group_pad(PadArgs{(const char*)g.a, ws, g.src, 0, 2 * g.lda, row, g.S, g.S, 2 * g.K, g.rows, g.top_k}, st);
+      g.a = (const bf16*)ws;
+      g.lda = row / 2;
+      g.src = nullptr;
+      g.rows = g.S;
     }
+    if (p.pb) {
+      group_pad(PadArgs{(const char*)g.b, ws + p.pa, nullptr, 2 * g.es, 2 * g.ldb, row, (long)g.E * g.N, g.N, 2 * g.K, 0, 1}, st);
+      g.b = (const bf16*)(ws + p.pa);
+      g.ldb = row / 2;
+      g.es = (long)g.N * g.ldb;
+    }
+    g.K = (int)(up16(2l * g.K) / 2);
+    const int tn = (g.N + GP_B - 1) / GP_B;
+    const dim3 grid((unsigned)((long)(g.S / p.rows + g.E) * tn)), blk(GP_THREADS);
+    // bf16 outputs in column pairs, with their masks, where the rows are pairs
+    const bool pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && g.ldm % 2 == 0 && (uintptr_t)g.out % 4 == 0 &&
+                       (uintptr_t)g.mask % (g.mask8 ? 2 : 4) == 0;
+    const int out = g.out_f32 ? 1 : pairs ? 0 : 2;
+    if (p.rows == 256) hipLaunchKernelGGL(group_nt_mm_kernel<4>, grid, blk, 0, st, g, tn, out);
+    else hipLaunchKernelGGL(group_nt_mm_kernel<3>, grid, blk, 0, st, g, tn, out);
+    HFM_LAUNCH_CHECK();
   }
   const int tn = (g.N + GN_B - 1) / GN_B;
   const long blocks = (long)(g.S / GN_B + g.E) * tn;      // (each group adds less than one tile)
@@ -1260,12 +1355,9 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
 // 35; 16384: 145, 58; 4 groups, 4096 rows, 512 x 512: 38, 35; 16 groups, 32768 rows, 1024 x 1024: 290, 115.
 constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
 static bool wgrad_big(const GroupWgArgs& g) {
-  const bool x8 = g.xs != nullptr;
-  if ((uintptr_t)g.dz % 16 || (uintptr_t)g.x % 16 || g.N % 8 || g.ldz % 8) return false;
-  if (g.K % (x8 ? 16 : 8) || g.ldx % (x8 ? 16 : 8)) return false;
   if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD || g.E > 65535) return false;      // (32-bit offsets; grid)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
-  return tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS;
+  return g.rows > 0 && tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS;
 }
 // Time in us by l lanes: the rounds of the CUs times a lane's length (its rows, and a group's own cost); then
 // the parts' way through the workspace (0.065 us each, as many as there are cuts through rows) and the
@@ -1289,6 +1381,29 @@ static int wgrad_lanes(const GroupWgArgs& g) {
   }
   return best;
 }
+// The operands' copies that the large tile needs (rows of whole 16-byte chunks), as for the NT product: where they
+// and the large tile take less than the 128 x 128 tile (20 us and 60 TFLOP/s for such operands).  Copies against 128 x
+// 128 in us: 25092 rows of 2 groups, 2937 x 3216: 524, 4125, from 8-bit x 560, 6340; 1500 of 16, 1501 x 1001: 62, 73;
+// 20000 of 8, 201 x 401: 54, 76.
+struct WgPlan {
+  bool big;
+  long pz, px;
+};
+static WgPlan wg_plan(const GroupWgArgs& g) {
+  WgPlan p{wgrad_big(g), 0, 0};
+  if (!p.big) return p;
+  const int per = g.xs ? 16 : 8, xb = g.xs ? 1 : 2;
+  const bool z = (uintptr_t)g.dz % 16 || g.N % 8 || g.ldz % 8, x = (uintptr_t)g.x % 16 || g.K % per || g.ldx % per;
+  if (z) p.pz = (long)g.S * up16(2l * g.N);
+  if (x) p.px = (long)g.rows * up16((long)xb * g.K);
+  if (z || x) {
+    const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
+    const double t = (z + x) * 5.0 + (p.pz + p.px) * (2.0 / 4.5e6) + wgrad_time(g, tiles, wgrad_lanes(g));
+    if (t > 20.0 + 2.0 * g.S * g.N * g.K / 60e6 || g.S >= GROUP_PAD_MAX || g.rows >= GROUP_PAD_MAX) p = WgPlan{false, 0, 0};
+  }
+  return p;
+}
+
 // Two parts a workgroup (a single lane cuts no group), and the sums for db.
 static long wgrad_ws_floats(const GroupWgArgs& g) {
   const long l = wgrad_lanes(g), tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
@@ -1308,7 +1423,8 @@ static int wgrad_splits(int S, int N, int K, int E) {
 }
 
 HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
-  if (wgrad_big(*gp)) return wgrad_ws_floats(*gp);
+  const WgPlan p = wg_plan(*gp);
+  if (p.big) return (p.pz + p.px) / 4 + wgrad_ws_floats(*gp);
   const int ns = wgrad_splits(gp->S, gp->N, gp->K, gp->E);
   return ns > 1 ? (long)ns * gp->E * gp->N * (gp->K + 1) : 0;
 }
@@ -1317,10 +1433,26 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   GroupWgArgs g = *gp;
   if (g.S < 0 || g.K < 0 || g.N < 0 || g.E < 1 || g.top_k < 1) return (int)hipErrorInvalidValue;
   if (g.N == 0) return 0;
-  if (wgrad_big(g)) {
+  const WgPlan p = wg_plan(g);
+  if (p.big) {
     const int tn = (g.N + GP_B - 1) / GP_B, tk = (g.K + GP_B - 1) / GP_B;
     const int lanes = wgrad_lanes(g);
-    if ((lanes > 1 || g.db) && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    if ((lanes > 1 || g.db || p.pz || p.px) && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    char* ws = reinterpret_cast<char*>(g.ws);
+    if (p.pz) {
+      const long row = up16(2l * g.N);
+      group_pad(PadArgs{(const char*)g.dz, ws, nullptr, 0, 2 * g.ldz, row, g.S, g.S, 2 * g.N, 0, 1}, st);
+      g.dz = (const bf16*)ws;
+      g.ldz = row / 2;
+    }
+    if (p.px) {
+      const int xb = g.xs ? 1 : 2;
+      const long row = up16((long)xb * g.K);
+      group_pad(PadArgs{(const char*)g.x, ws + p.pz, nullptr, 0, xb * g.ldx, row, g.rows, g.rows, xb * g.K, 0, 1}, st);
+      g.x = ws + p.pz;
+      g.ldx = row / xb;
+    }
+    g.ws = reinterpret_cast<float*>(ws + p.pz + p.px);
     const int ovec = g.K % 8 == 0 && (uintptr_t)g.dw % 16 == 0;
     const dim3 grid((unsigned)(tn * tk * lanes)), blk(GP_THREADS);
     if (g.xs && g.src) hipLaunchKernelGGL((group_wgrad_mm_kernel<true, true>), grid, blk, 0, st, g, tn, tk, lanes);

@@ -232,7 +232,7 @@ class GroupNtArgs(C.Structure):
                 ("offs", c_void_p), ("src", c_void_p), ("lda", c_long), ("ldb", c_long), ("es", c_long),
                 ("ldm", c_long), ("ldo", c_long), ("S", c_int), ("rows", c_int), ("K", c_int), ("N", c_int),
                 ("E", c_int), ("top_k", c_int), ("relu", c_int), ("mask8", c_int), ("out_f32", c_int),
-                ("scale", c_float)]
+                ("scale", c_float), ("ws", c_void_p)]
 
 
 class GroupWgArgs(C.Structure):
@@ -255,6 +255,7 @@ _SIGS = {
     "hfm_act8_unpack": [C.POINTER(Act8Args), c_void_p],
     "hfm_act8_args_bytes": [],
     "hfm_group_nt": [C.POINTER(GroupNtArgs), c_void_p],
+    "hfm_group_nt_ws_bytes": [C.POINTER(GroupNtArgs)],
     "hfm_group_nt_args_bytes": [],
     "hfm_group_wgrad_ws_floats": [C.POINTER(GroupWgArgs)],
     "hfm_group_wgrad": [C.POINTER(GroupWgArgs), c_void_p],
@@ -400,7 +401,7 @@ def get_lib():
         for name, args in _SIGS.items():
             fn = getattr(lib, name)
             fn.argtypes = args
-            fn.restype = c_long if name == "hfm_group_wgrad_ws_floats" else c_int
+            fn.restype = c_long if name in ("hfm_group_wgrad_ws_floats", "hfm_group_nt_ws_bytes") else c_int
         # ABI checks: ctypes struct layouts must match the C structs
         for cname, pys in (("hfm_epi_args_bytes", EpiArgs), ("hfm_head_args_bytes", HeadArgs),
                            ("hfm_slab_job_bytes", SlabJob), ("hfm_rowsum_job_bytes", RowSumJob),

@@ -27,6 +27,9 @@ that the call allocated holds nothing there).
 
 Results are allocated by the call unless ``out`` is given; workspaces come from torch's allocator on
 the current stream, so calls on several streams and in several graphs share nothing.
+
+Any widths and strides are taken.  Large products are fastest where rows start on 16 bytes and widths are
+multiples of 8 (16 for 8-bit ``x``): operands that are otherwise are copied in the call.
 """
 from __future__ import annotations
 
@@ -220,6 +223,14 @@ def _check_out_type(dtype):
         raise ValueError(f"out must be bf16 or fp32, not {dtype}")
 
 
+def _nt(a: GroupNtArgs, dev, st, what):
+    lib = _lib.get_lib()
+    n = lib.hfm_group_nt_ws_bytes(C.byref(a))          # copies of operands of odd widths
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    a.ws = ptr(ws)
+    check(lib.hfm_group_nt(C.byref(a), st), what)
+
+
 def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], offs: torch.Tensor,
                  relu: bool = False, src: Optional[torch.Tensor] = None, top_k: int = 1,
                  out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -243,7 +254,7 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
                     w.stride(0), 0, row_stride(out), S, x.shape[0], K, N, E, top_k, 1 if relu else 0, 0,
                     0 if _bf(out) else 1, 1.0)
     with launch("group_linear", x, w, bias, offs, src, out) as st:
-        check(_lib.get_lib().hfm_group_nt(C.byref(a), st), "group_linear")
+        _nt(a, x.device, st, "group_linear")
     return out
 
 
@@ -272,7 +283,7 @@ def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
     a = GroupNtArgs(ptr(dz), ptr(wt), 0, ptr(m), ptr(out), ptr(offs), 0, row_stride(dz), wt.stride(1), wt.stride(0),
                     ldm, row_stride(out), S, S, N, K, E, 1, 0, m8, 0 if _bf(out) else 1, float(scale))
     with launch("group_dgrad", dz, wt, offs, m, out) as st:
-        check(_lib.get_lib().hfm_group_nt(C.byref(a), st), "group_dgrad")
+        _nt(a, dz.device, st, "group_dgrad")
     return out
 
 

@@ -379,7 +379,69 @@ def test_group_wgrad(sizes, K, N, x8):
 
 
 LARGE = [([9000, 0, 257, 1, 5000, 256], 200, 1032), ([20000], 64, 777), ([3] * 150, 72, 40), ([700, 4000, 1300], 1248, 2048),
-         ([1, 0, 30000], 136, 264), ([5000, 6000], 512, 1000)]
+         ([1, 0, 30000], 136, 264), ([5000, 6000], 512, 1000), ([6000, 0, 7000], 517, 1003), ([3000, 2500, 1], 1032, 1000),
+         ([9000], 1001, 390)]
+
+
+def test_large_products_of_rows_at_any_alignment():
+    """Operands, masks and results that start at odd places in wider rows give the bits of aligned ones."""
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(9)
+    S, K, N, E = 9000, 320, 600, 3
+    offs, _ = groups([4000, 0, 4900], tail=0)
+    o, live = offs.int().to(DEV), int(offs[-1])
+
+    def shifted(t):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + 11), math.nan, dtype=t.dtype, device=DEV)
+        wide[..., 3:3 + t.shape[-1]] = t
+        return wide[..., 3:3 + t.shape[-1]]
+
+    x, w, dz = (torch.randn(*s, device=DEV, generator=g).bfloat16() for s in ((S, K), (E, N, K), (S, N)))
+    wt = w.transpose(1, 2).contiguous()
+    out = torch.full((S, N + 7), 5.0, dtype=torch.bfloat16, device=DEV)
+    y = EX.group_linear(x, w, None, o)
+    EX.group_linear(shifted(x), shifted(w), None, o, out=out[:, 3:3 + N])
+    assert torch.equal(out[:live, 3:3 + N], y[:live]) and bool((out[:, :3] == 5).all()) and bool((out[:, 3 + N:] == 5).all())
+    assert bool((out[live:] == 5).all())
+    mask = torch.randn(S, K, device=DEV, generator=g).bfloat16()
+    dx = EX.group_dgrad(dz, wt, o, mask=mask, scale=2.0)
+    assert torch.equal(EX.group_dgrad(shifted(dz), shifted(wt), o, mask=shifted(mask), scale=2.0)[:live], dx[:live])
+    dw, db = EX.group_wgrad(dz, x, o)
+    dw2, db2 = EX.group_wgrad(shifted(dz), shifted(x), o)
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+    src = torch.randperm(S, device=DEV, generator=g).int()
+    assert torch.equal(EX.group_linear(shifted(x), w, None, o, src=src)[:live], EX.group_linear(x, w, None, o, src=src)[:live])
+    a = A8.pack(x)
+    # no row of x at all: every place reads zeros
+    none = torch.full((S,), -1, dtype=torch.int32, device=DEV)
+    assert bool((EX.group_linear(x[:0], w, None, o, src=none)[:live] == 0).all())
+    for e in (x[:0], A8.Act8(a.codes[:0], a.scales[:0])):
+        dw0, db0 = EX.group_wgrad(dz, e, o, src=none)
+        assert bool((dw0 == 0).all()) and bool(((db0 - db).abs() <= 2 * (4900 + 4) * 2.0 ** -23 * dz.float().abs().sum(0)).all())
+
+
+def test_odd_large_products_in_a_graph():
+    """The copies of odd operands are made in the call, in every replay."""
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(11)
+    S, K, N = 9000, 333, 601
+    o = torch.tensor([0, 3000, 8990], dtype=torch.int32, device=DEV)
+    x, w, dz = (torch.randn(*s, device=DEV, generator=g).bfloat16() for s in ((S, K), (2, N, K), (S, N)))
+    wt = w.transpose(1, 2).contiguous()
+
+    def run():
+        return (EX.group_linear(x, w, None, o)[:8990], EX.group_dgrad(dz, wt, o, mask=x)[:8990], *EX.group_wgrad(dz, x, o))
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i in range(3):
+        x.copy_(torch.randn(S, K, device=DEV, generator=g))
+        dz.copy_(torch.randn(S, N, device=DEV, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, run())), i
 
 
 @pytest.mark.parametrize("sizes", [[10], [300], [40, 700], [0, 130, 1], [64 * 9 + 1, 64 * 5], [1] * 6, [0, 0]])
