@@ -81,13 +81,13 @@ class _Here:
 
 def launch(what: str, *tensors):
     """Context with the stream to launch on; refuses operands that are not on one GPU."""
-    dev = tensors[0].device
+    at = tensors[0].get_device()          # (-1: the host)
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: operands on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError(f"{what} runs on the GPU: operands are on {dev}")
-    if dev.index == torch.cuda.current_device():
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"{what}: operands on {tensors[0].device} and {t.device}")
+    if at < 0:
+        raise ValueError(f"{what} runs on the GPU: operands are on {tensors[0].device}")
+    if at == torch._C._cuda_getDevice():
         # (the handle itself: torch.cuda.current_stream() takes 5 us to wrap it)
-        return _Here(torch._C._cuda_getCurrentRawStream(dev.index))
-    return _on(dev)
+        return _Here(torch._C._cuda_getCurrentRawStream(at))
+    return _on(tensors[0].device)

@@ -81,17 +81,18 @@ def _check_gate(logits, top_k):
 def _check_routes(r: Routes, T: Optional[int] = None) -> Tuple[int, int]:
     if not isinstance(r, Routes):
         raise ValueError("routes must be a Routes")
-    if r.expert.dim() != 2 or not 1 <= r.expert.shape[1] <= MAX_TOP_K:
+    expert, weight, pos, src, _ = r
+    if expert.dim() != 2 or not 1 <= expert.shape[1] <= MAX_TOP_K:
         raise ValueError(f"routes.expert must be [T, 1 to {MAX_TOP_K}]")
-    n, k = shape = r.expert.shape
+    n, k = shape = expert.shape
     if T is not None and n != T:
         raise ValueError(f"routes are of {n} tokens, the rows of {T}")
     if n * k > _MAX_SLOTS:
         raise ValueError(f"{n} x {k} slots are more than {_MAX_SLOTS}")
-    flat(r.expert, "routes.expert", torch.int32, shape)
-    flat(r.weight, "routes.weight", torch.float32, shape)
-    flat(r.pos, "routes.pos", torch.int32, shape)
-    flat(r.src, "routes.src", torch.int32, (n * k,))
+    flat(expert, "routes.expert", torch.int32, shape)
+    flat(weight, "routes.weight", torch.float32, shape)
+    flat(pos, "routes.pos", torch.int32, shape)
+    flat(src, "routes.src", torch.int32, (n * k,))
     return n, k
 
 
