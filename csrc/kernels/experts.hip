@@ -36,6 +36,12 @@ struct RouteArgs {
   int T, E, k, renorm, bf, nblk, tpb;   // tpb: tokens per block
 };
 
+// Workgroups of 256 threads in x and y: a launch has less than 2^32 threads in x.
+static dim3 wide_grid(long n) {
+  const long row = 1l << 23;
+  return dim3((unsigned)(n < row ? n : row), (unsigned)((n + row - 1) / row));
+}
+
 struct RouteBwdArgs {
   const void* logits;
   const int* expert;
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
   constexpr int V = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   const int gl = threadIdx.x & (G - 1);
-  const int t = blockIdx.x * (256 / G) + threadIdx.x / G;
+  const long t = ((long)blockIdx.y * gridDim.x + blockIdx.x) * (256 / G) + threadIdx.x / G;
   if (t >= a.T) return;
   const size_t o = (size_t)t * a.k + gl;
   const int e = gl < a.k ? a.expert[o] : -1;
@@ -454,10 +460,11 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdArgs a) {
 template <typename T>
 static void route_bwd(const RouteBwdArgs& a, hipStream_t st) {
   const int lanes = (a.E * (int)sizeof(T) + 15) / 16;          // (and one for each choice)
-  const dim3 blk(256);
-  if (lanes <= 16) hipLaunchKernelGGL((route_bwd_kernel<T, 16>), dim3((a.T + 15) / 16), blk, 0, st, a);
-  else if (lanes <= 32) hipLaunchKernelGGL((route_bwd_kernel<T, 32>), dim3((a.T + 7) / 8), blk, 0, st, a);
-  else hipLaunchKernelGGL((route_bwd_kernel<T, 64>), dim3((a.T + 3) / 4), blk, 0, st, a);
+  const int G = lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+  const dim3 grid = wide_grid((a.T + 256l / G - 1) / (256 / G)), blk(256);
+  if (G == 16) hipLaunchKernelGGL((route_bwd_kernel<T, 16>), grid, blk, 0, st, a);
+  else if (G == 32) hipLaunchKernelGGL((route_bwd_kernel<T, 32>), grid, blk, 0, st, a);
+  else hipLaunchKernelGGL((route_bwd_kernel<T, 64>), grid, blk, 0, st, a);
 }
 
 HFM_API int hfm_route_bwd(const RouteBwdArgs* ap, hipStream_t st) {
@@ -497,13 +504,13 @@ struct RowVec {               // (aligned to an element only)
 enum { EX_DISPATCH = 0, EX_DISPATCH_BWD = 1, EX_COMBINE = 2, EX_COMBINE_BWD = 3 };
 
 // Columns c + 64 V u .. + V - 1 of token t's rows, for the U turns u of them that lie before `end`; all rows'
-// loads of the U turns are under way before any is used.
+// loads of the U turns are under way before any is used or written (combine_bwd may write over ys).
 template <typename T, int V, int U, int K, int MODE>
-__device__ __forceinline__ void exchange_cols(const ExchArgs& a, int t, int c, int end, const int (&p)[K], const float (&w)[K],
+__device__ __forceinline__ void exchange_cols(const ExchArgs& a, size_t t, int c, int end, const int (&p)[K], const float (&w)[K],
                                               float (&dot)[K]) {
-  const T* __restrict__ A = reinterpret_cast<const T*>(a.a) + c;
-  const T* __restrict__ B = reinterpret_cast<const T*>(a.b) + c;
-  T* __restrict__ O = reinterpret_cast<T*>(a.out) + c;
+  const T* A = reinterpret_cast<const T*>(a.a) + c;
+  const T* B = reinterpret_cast<const T*>(a.b) + c;
+  T* O = reinterpret_cast<T*>(a.out) + c;
   typedef typename RowVec<T, V>::type vec;
   auto at = [&](const T* x, size_t row, long ld, int u) -> vec { return *reinterpret_cast<const vec*>(x + row * ld + u * 64 * V); };
   auto on = [&](int u) { return u == 0 || c + u * 64 * V < end; };
@@ -555,7 +562,7 @@ template <typename T, int K, int MODE>
 __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long t = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   int p[K];
   float w[K], dot[K];
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(256) exchange_kernel(ExchArgs a) {
 
 template <typename T, int MODE>
 static void exchange_k(const ExchArgs& a, hipStream_t st) {
-  const dim3 grid((a.T + 3) / 4), blk(256);
+  const dim3 grid = wide_grid((a.T + 3l) / 4), blk(256);
   if (a.k <= 1) hipLaunchKernelGGL((exchange_kernel<T, 1, MODE>), grid, blk, 0, st, a);
   else if (a.k <= 2) hipLaunchKernelGGL((exchange_kernel<T, 2, MODE>), grid, blk, 0, st, a);
   else if (a.k <= 4) hipLaunchKernelGGL((exchange_kernel<T, 4, MODE>), grid, blk, 0, st, a);

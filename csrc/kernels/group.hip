@@ -162,7 +162,7 @@ struct PadArgs {
 };
 __global__ void __launch_bounds__(256) group_pad_kernel(PadArgs a) {
   typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
-  const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long r = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (r >= a.rows) return;
   const int row = group_row(a.map, a.map ? (int)r : 0, a.have, a.top_k);
   const char* from = a.map ? a.from + (size_t)max(row, 0) * a.lds : a.from + (size_t)(r / a.per) * a.gs + (size_t)(r % a.per) * a.lds;
@@ -183,9 +183,10 @@ __global__ void __launch_bounds__(256) group_pad_kernel(PadArgs a) {
   }
 }
 static void group_pad(const PadArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(group_pad_kernel, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+  const unsigned n = (unsigned)((a.rows + 3) / 4), row = 1u << 23;       // (a launch has less than 2^32 threads in x)
+  hipLaunchKernelGGL(group_pad_kernel, dim3(n < row ? n : row, (n + row - 1) / row), dim3(256), 0, st, a);
 }
-constexpr long GROUP_PAD_MAX = 1l << 32;                   // (grid)
+constexpr long GROUP_PAD_MAX = 1l << 33;                   // (grid)
 static long up16(long bytes) { return (bytes + 15) / 16 * 16; }
 
 // One output of the NT product: scale, bias, relu (NaN stays), mask, rounding.

@@ -28,6 +28,9 @@ that the call allocated holds nothing there).
 Results are allocated by the call unless ``out`` is given; workspaces come from torch's allocator on
 the current stream, so calls on several streams and in several graphs share nothing.
 
+``out`` shares no memory with the operands, but ``combine_bwd`` may write over ``ys`` and ``group_dgrad`` over a
+bf16 ``mask``.
+
 Any widths and strides are taken.  Large products are fastest where rows start on 16 bytes and widths are
 multiples of 8 (16 for 8-bit ``x``): operands that are otherwise are copied in the call.
 """

@@ -383,6 +383,23 @@ LARGE = [([9000, 0, 257, 1, 5000, 256], 200, 1032), ([20000], 64, 777), ([3] * 1
          ([9000], 1001, 390)]
 
 
+@pytest.mark.parametrize("S,K,N", [(300, 40, 72), (9000, 320, 512)])
+def test_results_over_operands_they_may_replace(S, K, N):
+    """combine_bwd over ys, group_dgrad over its bf16 mask."""
+    EX, _ = ops()
+    g = torch.Generator(device=DEV).manual_seed(S)
+    r = EX.route(torch.randn(S, 6, device=DEV, generator=g), 3)
+    dy, ys = torch.randn(S, N, device=DEV, generator=g), torch.randn(3 * S, N, device=DEV, generator=g)
+    dys, dw = EX.combine_bwd(dy, ys, r)
+    dys2, dw2 = EX.combine_bwd(dy, ys, r, out=ys)
+    assert dys2.data_ptr() == ys.data_ptr() and torch.equal(dys2, dys) and torch.equal(dw2, dw)
+    offs = torch.tensor([0, S // 3, S], dtype=torch.int32, device=DEV)
+    dz, wt = torch.randn(S, K, device=DEV, generator=g).bfloat16(), torch.randn(2, N, K, device=DEV, generator=g).bfloat16()
+    mask = torch.randn(S, N, device=DEV, generator=g).bfloat16()
+    dx = EX.group_dgrad(dz, wt, offs, mask=mask)
+    assert torch.equal(EX.group_dgrad(dz, wt, offs, mask=mask, out=mask), dx)
+
+
 def test_large_products_of_rows_at_any_alignment():
     """Operands, masks and results that start at odd places in wider rows give the bits of aligned ones."""
     EX, A8 = ops()
