@@ -788,7 +788,8 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   if (g.S == 0 || g.N == 0) return 0;
   const NtPlan p = nt_plan(g);
   if (p.rows) {
-    if (p.pa + p.pb > 0 && (!g.ws || (uintptr_t)g.ws % 16)) return (int)hipErrorInvalidValue;
+    if (p.pa + p.pb > 0 && !g.ws) return -1;                 // (nothing launched: the caller brings hfm_group_nt_ws_bytes)
+    if ((uintptr_t)g.ws % 16) return (int)hipErrorInvalidValue;
     const long row = up16(2l * g.K);
     char* ws = reinterpret_cast<char*>(g.ws);
     if (p.pa) {

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import Act8Args, check, ptr
-from .checks import flat, launch, out_or_new, row_stride, rows2d
+from .checks import call, flat, out_or_new, rows2d
 
 BLOCK = 32            # columns per scale
 
@@ -45,19 +45,22 @@ def empty(M: int, N: int, device) -> Act8:
 _U8 = (torch.uint8,)
 
 
-def check_act8(a: Act8, M: int, N: int, what: str) -> None:
+def check_act8(a: Act8, M: int, N: int, what: str) -> int:
+    """``a`` is an [M, N] Act8.  The row stride of its codes."""
     if not isinstance(a, Act8):
         raise ValueError(f"{what} must be an Act8")
-    rows2d(a.codes, what + ".codes", _U8, M, N)
+    ld = rows2d(a.codes, what + ".codes", _U8, M, N)
     flat(a.scales, what + ".scales", torch.uint8, (M, scale_cols(N)))
+    return ld
 
 
-def check_own_act8(a: Act8, what: str) -> None:
-    """``a`` is an Act8 whose parts fit one another."""
+def check_own_act8(a: Act8, what: str) -> int:
+    """``a`` is an Act8 whose parts fit one another.  The row stride of its codes."""
     if not isinstance(a, Act8):
         raise ValueError(f"{what} must be an Act8")
-    rows2d(a.codes, what + ".codes", _U8)
+    ld = rows2d(a.codes, what + ".codes", _U8)
     flat(a.scales, what + ".scales", torch.uint8, (a.codes.shape[0], scale_cols(a.codes.shape[1])))
+    return ld
 
 
 _VALUES = (torch.float32, torch.bfloat16)
@@ -65,29 +68,27 @@ _VALUES = (torch.float32, torch.bfloat16)
 
 def pack(x: torch.Tensor, out: Optional[Act8] = None) -> Act8:
     """x [M, N] (fp32 or bf16, rows may be strided) -> ``Act8``."""
-    rows2d(x, "x", _VALUES)
+    ld = rows2d(x, "x", _VALUES)
     M, N = x.shape
     if out is None:
-        out = empty(M, N, x.device)
+        out, ldc = empty(M, N, x.device), N
     else:
-        check_act8(out, M, N, "out")
-    a = Act8Args(ptr(x), ptr(out.codes), ptr(out.scales), 0, row_stride(x), row_stride(out.codes), M, N,
+        ldc = check_act8(out, M, N, "out")
+    a = Act8Args(ptr(x), ptr(out.codes), ptr(out.scales), 0, ld, ldc, M, N,
                  1 if x.dtype == torch.bfloat16 else 0)
-    with launch("act8.pack", x, *out) as st:
-        check(_lib.get_lib().hfm_act8_pack(C.byref(a), st), "act8_pack")
+    check(call("act8.pack", (x, *out), _lib.get_lib().hfm_act8_pack, C.byref(a)), "act8_pack")
     return out
 
 
 def unpack(a: Act8, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values that ``a`` stands for, in fp32 or bf16 (exact in both, but where a value of a
     block with the smallest scales lies below the type's normal range)."""
-    check_own_act8(a, "a")
+    ldc = check_own_act8(a, "a")
     M, N = a.codes.shape
     if dtype not in _VALUES:
         raise ValueError(f"unpack to fp32 or bf16, not {dtype}")
-    out = out_or_new(out, M, N, dtype, a.codes.device)
-    args = Act8Args(0, ptr(a.codes), ptr(a.scales), ptr(out), row_stride(out), row_stride(a.codes), M, N,
+    out, ld = out_or_new(out, M, N, dtype, a.codes.device)
+    args = Act8Args(0, ptr(a.codes), ptr(a.scales), ptr(out), ld, ldc, M, N,
                     1 if dtype == torch.bfloat16 else 0)
-    with launch("act8.unpack", *a, out) as st:
-        check(_lib.get_lib().hfm_act8_unpack(C.byref(args), st), "act8_unpack")
+    check(call("act8.unpack", (*a, out), _lib.get_lib().hfm_act8_unpack, C.byref(args)), "act8_unpack")
     return out

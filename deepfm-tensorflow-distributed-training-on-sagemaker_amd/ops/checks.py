@@ -8,29 +8,23 @@ the host's: the checks of a good call build no text.
 """
 from __future__ import annotations
 
-import contextlib
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
 LIMIT = 1 << 31          # rows, columns: int32 in the kernels
 
 
-def row_stride(t: torch.Tensor) -> int:
-    """Elements from a row to the next (of a single row: any that hold it)."""
-    s = t.stride(0)
-    return s if t.shape[0] > 1 else max(s, t.shape[1])
-
-
 def rows2d(t: torch.Tensor, what: str, dtypes: Sequence[torch.dtype], M: Optional[int] = None,
-           N: Optional[int] = None) -> None:
-    """``t`` is [M, N] of one of ``dtypes`` with unit column stride and rows that do not overlap."""
+           N: Optional[int] = None) -> int:
+    """``t`` is [M, N] of one of ``dtypes`` with unit column stride and rows that do not overlap.  Elements from a
+    row to the next (of a single row: any that hold it)."""
     if isinstance(t, torch.Tensor) and t.dim() == 2 and t.dtype in dtypes:
         m, n = t.shape
         s0, s1 = t.stride()
         if ((M is None or m == M) and (N is None or n == N) and m < LIMIT and n < LIMIT
                 and (((s1 == 1 or n == 1) and (s0 >= n or m == 1)) or m == 0 or n == 0)):
-            return
+            return s0 if m > 1 or s0 > n else n
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what} must be a tensor")
     if t.dim() != 2:
@@ -52,42 +46,25 @@ def flat(t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple) -> None:
         raise ValueError(f"{what} must be a contiguous {dtype} {tuple(shape)}{got}")
 
 
-def out_or_new(out: Optional[torch.Tensor], M: int, N: int, dtype, device, what: str = "out") -> torch.Tensor:
+def out_or_new(out: Optional[torch.Tensor], M: int, N: int, dtype, device, what: str = "out") -> Tuple[torch.Tensor, int]:
+    """``out`` or a new tensor, and its row stride."""
     if out is None:
-        return torch.empty(M, N, dtype=dtype, device=device)
-    rows2d(out, what, (dtype,), M, N)
-    return out
+        return torch.empty(M, N, dtype=dtype, device=device), N
+    return out, rows2d(out, what, (dtype,), M, N)
 
 
-@contextlib.contextmanager
-def _on(dev):
-    with torch.cuda.device(dev):
-        yield torch.cuda.current_stream(dev).cuda_stream
-
-
-class _Here:
-    """The current device's stream, without switching (the usual case)."""
-    __slots__ = ("st",)
-
-    def __init__(self, st):
-        self.st = st
-
-    def __enter__(self):
-        return self.st
-
-    def __exit__(self, *exc):
-        return False
-
-
-def launch(what: str, *tensors):
-    """Context with the stream to launch on; refuses operands that are not on one GPU."""
-    at = tensors[0].get_device()          # (-1: the host)
+def call(what: str, tensors, fn, *args) -> int:
+    """``fn(*args, stream)`` on the current stream of the operands' device; refuses operands (None: not
+    given) that are not on one GPU.  The result of ``fn``."""
+    first = tensors[0]
+    at = first.get_device()               # (-1: the host)
     for t in tensors:
         if t is not None and t.get_device() != at:
-            raise ValueError(f"{what}: operands on {tensors[0].device} and {t.device}")
+            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
     if at < 0:
-        raise ValueError(f"{what} runs on the GPU: operands are on {tensors[0].device}")
+        raise ValueError(f"{what} runs on the GPU: operands are on {first.device}")
     if at == torch._C._cuda_getDevice():
         # (the handle itself: torch.cuda.current_stream() takes 5 us to wrap it)
-        return _Here(torch._C._cuda_getCurrentRawStream(at))
-    return _on(tensors[0].device)
+        return fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    with torch.cuda.device(at):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(at))

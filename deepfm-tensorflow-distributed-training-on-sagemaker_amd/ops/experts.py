@@ -44,7 +44,7 @@ import torch
 from . import _lib
 from ._lib import ExchArgs, GroupNtArgs, GroupWgArgs, RouteArgs, RouteBwdArgs, check, ptr
 from .act8 import Act8, check_act8, check_own_act8
-from .checks import flat, launch, out_or_new, row_stride, rows2d
+from .checks import call, flat, out_or_new, rows2d
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 16
@@ -70,7 +70,7 @@ def _bf(t) -> int:
 
 
 def _check_gate(logits, top_k):
-    rows2d(logits, "logits", _VALUES)
+    ld = rows2d(logits, "logits", _VALUES)
     T, E = logits.shape
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"1 to {MAX_EXPERTS} experts, got {E}")
@@ -78,7 +78,7 @@ def _check_gate(logits, top_k):
         raise ValueError(f"top_k must be 1 to {min(E, MAX_TOP_K)}, got {top_k}")
     if T * top_k > _MAX_SLOTS:
         raise ValueError(f"{T} x {top_k} slots are more than {_MAX_SLOTS}")
-    return T, E
+    return T, E, ld
 
 
 def _check_routes(r: Routes, T: Optional[int] = None) -> Tuple[int, int]:
@@ -105,7 +105,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, valid: Opt
     lowest index first among equals; weights are the softmax over the chosen (``renormalize``) or
     over all experts.  A logit of -inf or NaN closes its expert, +inf counts as the largest finite
     number; rows where ``valid`` (bool [T]) is False choose nothing."""
-    T, E = _check_gate(logits, top_k)
+    T, E, ld = _check_gate(logits, top_k)
     if valid is not None:
         flat(valid, "valid", torch.bool, (T,))
     dev = logits.device
@@ -117,13 +117,12 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, valid: Opt
         if _check_routes(out, T)[1] != top_k:
             raise ValueError("out has another top_k")
         flat(out.offs, "out.offs", torch.int32, (E + 1,))
-    with launch("route", logits, valid, *out) as st:
-        lib = _lib.get_lib()
-        n = lib.hfm_route_ws_ints(T, E)
-        ws = torch.empty(n, dtype=torch.int32, device=dev) if n else None
-        a = RouteArgs(ptr(logits), ptr(valid), *(ptr(t) for t in out), ptr(ws), 0, row_stride(logits), T, E, top_k,
-                      1 if renormalize else 0, _bf(logits), 0, 0)
-        check(lib.hfm_route(C.byref(a), st), "route")
+    lib = _lib.get_lib()
+    n = lib.hfm_route_ws_ints(T, E)
+    ws = torch.empty(n, dtype=torch.int32, device=dev) if n else None
+    a = RouteArgs(ptr(logits), ptr(valid), *(ptr(t) for t in out), ptr(ws), 0, ld, T, E, top_k,
+                  1 if renormalize else 0, _bf(logits), 0, 0)
+    check(call("route", (logits, valid, *out), lib.hfm_route, C.byref(a)), "route")
     return out
 
 
@@ -133,68 +132,66 @@ def route_bwd(logits: torch.Tensor, routes: Routes, dweight: torch.Tensor, renor
     ``renormalize`` as in ``route``.  Closed experts, empty slots and rows that are not valid get zeros."""
     rows2d(logits, "logits", _VALUES)
     T, k = _check_routes(routes, logits.shape[0])
-    _, E = _check_gate(logits, k)
+    _, E, ld = _check_gate(logits, k)
     flat(dweight, "dweight", torch.float32, (T, k))
-    out = out_or_new(out, T, E, logits.dtype, logits.device)
+    out, ldo = out_or_new(out, T, E, logits.dtype, logits.device)
     a = RouteBwdArgs(ptr(logits), ptr(routes.expert), ptr(routes.weight), ptr(dweight), ptr(out),
-                     row_stride(logits), row_stride(out), T, E, k, 1 if renormalize else 0, _bf(logits))
-    with launch("route_bwd", logits, *routes, dweight, out) as st:
-        check(_lib.get_lib().hfm_route_bwd(C.byref(a), st), "route_bwd")
+                     ld, ldo, T, E, k, 1 if renormalize else 0, _bf(logits))
+    check(call("route_bwd", (logits, *routes, dweight, out), _lib.get_lib().hfm_route_bwd, C.byref(a)), "route_bwd")
     return out
 
 
-def _exchange(mode, what, a, b, out, r: Routes, weight, dweight, T, k, D, S):
-    args = ExchArgs(ptr(a), ptr(b), ptr(out), ptr(r.pos), ptr(weight), ptr(dweight), row_stride(a),
-                    row_stride(b) if b is not None else 0, row_stride(out), T, k, D, S, _bf(a))
-    with launch(what, a, b, out, r.pos, weight, dweight) as st:
-        check(_lib.get_lib().hfm_exchange(mode, C.byref(args), st), what)
+def _exchange(mode, what, a, b, out, pos, weight, dweight, lda, ldb, ldo, T, k, D):
+    args = ExchArgs(a.data_ptr(), ptr(b), out.data_ptr(), pos.data_ptr(), ptr(weight), ptr(dweight), lda, ldb, ldo, T, k, D,
+                    T * k, _bf(a))
+    check(call(what, (a, b, out, pos, weight, dweight), _lib.get_lib().hfm_exchange, mode, C.byref(args)), what)
 
 
 def dispatch(x: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [T, D] (fp32 or bf16) -> its rows in expert order, [T * top_k, D]."""
-    rows2d(x, "x", _VALUES)
-    T, k = _check_routes(routes, x.shape[0])
-    D = x.shape[1]
-    out = out_or_new(out, T * k, D, x.dtype, x.device)
-    _exchange(_EX_DISPATCH, "dispatch", x, None, out, routes, None, None, T, k, D, T * k)
+    ld = rows2d(x, "x", _VALUES)
+    T, D = x.shape
+    _, k = _check_routes(routes, T)
+    out, ldo = out_or_new(out, T * k, D, x.dtype, x.device)
+    _exchange(_EX_DISPATCH, "dispatch", x, None, out, routes.pos, None, None, ld, 0, ldo, T, k, D)
     return out
 
 
 def dispatch_bwd(dxs: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of ``dispatch``: dx[t] = the sum of token t's rows of dxs (fp32 sum, in slot order)."""
-    rows2d(dxs, "dxs", _VALUES)
+    ld = rows2d(dxs, "dxs", _VALUES)
     T, k = _check_routes(routes)
-    D = dxs.shape[1]
-    if dxs.shape[0] != T * k:
-        raise ValueError(f"dxs must have {T * k} rows, got {dxs.shape[0]}")
-    out = out_or_new(out, T, D, dxs.dtype, dxs.device)
-    _exchange(_EX_DISPATCH_BWD, "dispatch_bwd", dxs, None, out, routes, None, None, T, k, D, T * k)
+    n, D = dxs.shape
+    if n != T * k:
+        raise ValueError(f"dxs must have {T * k} rows, got {n}")
+    out, ldo = out_or_new(out, T, D, dxs.dtype, dxs.device)
+    _exchange(_EX_DISPATCH_BWD, "dispatch_bwd", dxs, None, out, routes.pos, None, None, ld, 0, ldo, T, k, D)
     return out
 
 
 def combine(ys: torch.Tensor, routes: Routes, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """ys [T * top_k, D] in expert order -> y[t] = sum_j weight[t, j] ys[pos[t, j]] (fp32 sum, in slot
     order); a token without live slots gets zeros."""
-    rows2d(ys, "ys", _VALUES)
+    ld = rows2d(ys, "ys", _VALUES)
     T, k = _check_routes(routes)
-    D = ys.shape[1]
-    if ys.shape[0] != T * k:
-        raise ValueError(f"ys must have {T * k} rows, got {ys.shape[0]}")
-    out = out_or_new(out, T, D, ys.dtype, ys.device)
-    _exchange(_EX_COMBINE, "combine", ys, None, out, routes, routes.weight, None, T, k, D, T * k)
+    n, D = ys.shape
+    if n != T * k:
+        raise ValueError(f"ys must have {T * k} rows, got {n}")
+    out, ldo = out_or_new(out, T, D, ys.dtype, ys.device)
+    _exchange(_EX_COMBINE, "combine", ys, None, out, routes.pos, routes.weight, None, ld, 0, ldo, T, k, D)
     return out
 
 
 def combine_bwd(dy: torch.Tensor, ys: torch.Tensor, routes: Routes,
                 out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Gradients of ``combine``: (dys [T * top_k, D], dweight fp32 [T, top_k]) from dy [T, D]."""
-    rows2d(dy, "dy", _VALUES)
-    T, k = _check_routes(routes, dy.shape[0])
-    D = dy.shape[1]
-    rows2d(ys, "ys", (dy.dtype,), T * k, D)
-    out = out_or_new(out, T * k, D, dy.dtype, dy.device)
+    ld = rows2d(dy, "dy", _VALUES)
+    T, D = dy.shape
+    _, k = _check_routes(routes, T)
+    ldb = rows2d(ys, "ys", (dy.dtype,), T * k, D)
+    out, ldo = out_or_new(out, T * k, D, dy.dtype, dy.device)
     dweight = torch.empty(T, k, dtype=torch.float32, device=dy.device)
-    _exchange(_EX_COMBINE_BWD, "combine_bwd", dy, ys, out, routes, routes.weight, dweight, T, k, D, T * k)
+    _exchange(_EX_COMBINE_BWD, "combine_bwd", dy, ys, out, routes.pos, routes.weight, dweight, ld, ldb, ldo, T, k, D)
     return out, dweight
 
 
@@ -227,12 +224,17 @@ def _check_out_type(dtype):
         raise ValueError(f"out must be bf16 or fp32, not {dtype}")
 
 
-def _nt(a: GroupNtArgs, dev, st, what):
-    lib = _lib.get_lib()
-    n = lib.hfm_group_nt_ws_bytes(C.byref(a))          # copies of operands of odd widths
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    a.ws = ptr(ws)
-    check(lib.hfm_group_nt(C.byref(a), st), what)
+_NEEDS_WS = -1
+
+
+def _nt(what, a: GroupNtArgs, tensors):
+    lib, r = _lib.get_lib(), C.byref(a)
+    rc = call(what, tensors, lib.hfm_group_nt, r)
+    if rc == _NEEDS_WS:                    # copies of operands of odd widths
+        ws = torch.empty(lib.hfm_group_nt_ws_bytes(r), dtype=torch.uint8, device=tensors[0].device)
+        a.ws = ptr(ws)
+        rc = call(what, tensors, lib.hfm_group_nt, r)
+    check(rc, what)
 
 
 def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], offs: torch.Tensor,
@@ -242,7 +244,7 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     w bf16 [E, N, K], bias fp32 [E, N] or None, out bf16 or fp32 [S, N].  row(p) = p, or with ``src`` (int32
     [S]) row(p) = src[p] // top_k, the token of the slot; an entry of ``src`` that is no slot of a row
     of x reads as a row of zeros.  Without ``src``, S is x's rows."""
-    rows2d(x, "x", _BF)
+    ld = rows2d(x, "x", _BF)
     _check_weight(w, "w", x.shape[1])
     E, N, K = w.shape
     _check_groups(offs, E)
@@ -253,12 +255,11 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     if out is not None:
         out_dtype = out.dtype
     _check_out_type(out_dtype)
-    out = out_or_new(out, S, N, out_dtype, x.device)
-    a = GroupNtArgs(ptr(x), ptr(w), ptr(bias), 0, ptr(out), ptr(offs), ptr(src), row_stride(x), w.stride(1),
-                    w.stride(0), 0, row_stride(out), S, x.shape[0], K, N, E, top_k, 1 if relu else 0, 0,
+    out, ldo = out_or_new(out, S, N, out_dtype, x.device)
+    a = GroupNtArgs(ptr(x), ptr(w), ptr(bias), 0, ptr(out), ptr(offs), ptr(src), ld, w.stride(1),
+                    w.stride(0), 0, ldo, S, x.shape[0], K, N, E, top_k, 1 if relu else 0, 0,
                     0 if _bf(out) else 1, 1.0)
-    with launch("group_linear", x, w, bias, offs, src, out) as st:
-        _nt(a, x.device, st, "group_linear")
+    _nt("group_linear", a, (x, w, bias, offs, src, out))
     return out
 
 
@@ -268,26 +269,23 @@ def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
     """Gradient towards the layer's input in expert order: out[p] = scale * dz[p] w[e(p)], zero where
     ``mask`` [S, K] (the input itself, bf16 or ``Act8``: what its relu and dropout left) is not above
     zero.  dz bf16 [S, N]; ``wt`` bf16 [E, K, N] is the transposed copy of w."""
-    rows2d(dz, "dz", _BF)
+    ld = rows2d(dz, "dz", _BF)
     S = dz.shape[0]
     _check_weight(wt, "wt", dz.shape[1])
     E, K, N = wt.shape
     _check_groups(offs, E)
     m, ldm, m8 = None, 0, 0
     if isinstance(mask, Act8):
-        check_act8(mask, S, K, "mask")
-        m, ldm, m8 = mask.codes, row_stride(mask.codes), 1
+        m, ldm, m8 = mask.codes, check_act8(mask, S, K, "mask"), 1
     elif mask is not None:
-        rows2d(mask, "mask", _BF, S, K)
-        m, ldm = mask, row_stride(mask)
+        m, ldm = mask, rows2d(mask, "mask", _BF, S, K)
     if out is not None:
         out_dtype = out.dtype
     _check_out_type(out_dtype)
-    out = out_or_new(out, S, K, out_dtype, dz.device)
-    a = GroupNtArgs(ptr(dz), ptr(wt), 0, ptr(m), ptr(out), ptr(offs), 0, row_stride(dz), wt.stride(1), wt.stride(0),
-                    ldm, row_stride(out), S, S, N, K, E, 1, 0, m8, 0 if _bf(out) else 1, float(scale))
-    with launch("group_dgrad", dz, wt, offs, m, out) as st:
-        _nt(a, dz.device, st, "group_dgrad")
+    out, ldo = out_or_new(out, S, K, out_dtype, dz.device)
+    a = GroupNtArgs(ptr(dz), ptr(wt), 0, ptr(m), ptr(out), ptr(offs), 0, ld, wt.stride(1), wt.stride(0),
+                    ldm, ldo, S, S, N, K, E, 1, 0, m8, 0 if _bf(out) else 1, float(scale))
+    _nt("group_dgrad", a, (dz, wt, offs, m, out))
     return out
 
 
@@ -299,13 +297,13 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
     ([E, N, K]) and db[e] = sum dz[p] ([E, N], None without ``bias``); an expert without rows gets zeros.
     dz bf16 [S, N]; x bf16 [rows, K] or ``Act8``; ``src`` and ``top_k`` as in ``group_linear``.
     ``out``: the pair to write into, contiguous."""
-    rows2d(dz, "dz", _BF)
+    ld = rows2d(dz, "dz", _BF)
     S, N = dz.shape
     x8 = isinstance(x, Act8)
     if x8:
-        check_own_act8(x, "x")
+        ldx = check_own_act8(x, "x")
     else:
-        rows2d(x, "x", _BF)
+        ldx = rows2d(x, "x", _BF)
     xv = x.codes if x8 else x
     K = xv.shape[1]
     if not (isinstance(offs, torch.Tensor) and offs.dim() == 1 and offs.shape[0] >= 2):
@@ -323,12 +321,12 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
         flat(dw, "dw", torch.float32, (E, N, K))
         if db is not None:
             flat(db, "db", torch.float32, (E, N))
-    with launch("group_wgrad", dz, xv, x.scales if x8 else None, offs, src, dw, db) as st:
-        lib = _lib.get_lib()
-        a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), 0,
-                        row_stride(dz), row_stride(xv), S, xv.shape[0], K, N, E, top_k, 1)
-        n = lib.hfm_group_wgrad_ws_floats(C.byref(a))      # split products and column sums
-        ws = torch.empty(n, dtype=torch.float32, device=dz.device) if n else None
-        a.ws = ptr(ws)
-        check(lib.hfm_group_wgrad(C.byref(a), st), "group_wgrad")
+    lib = _lib.get_lib()
+    a = GroupWgArgs(ptr(dz), ptr(xv), ptr(x.scales) if x8 else 0, ptr(offs), ptr(src), ptr(dw), ptr(db), 0,
+                    ld, ldx, S, xv.shape[0], K, N, E, top_k, 1)
+    r = C.byref(a)
+    n = lib.hfm_group_wgrad_ws_floats(r)      # split products, column sums, copies of operands of odd widths
+    ws = torch.empty(n, dtype=torch.float32, device=dz.device) if n else None
+    a.ws = ptr(ws)
+    check(call("group_wgrad", (dz, xv, x.scales if x8 else None, offs, src, dw, db), lib.hfm_group_wgrad, r), "group_wgrad")
     return dw, db
