@@ -2,13 +2,6 @@
 // e has rows offs[e] .. offs[e + 1) (device memory: no host synchronization, ragged and empty groups
 // allowed); rows behind offs[E] are not touched.
 //
-//   group_nt     out[p, n] = epi(sum_k A[row(p), k] B[e, n, k])      A, B bf16, K-contiguous
-//                forward:  A = x (row(p) = p, or src[p] / top_k: the sorted slot's token), B = w,
-//                          epi = + bias[e, n], relu
-//                gradient: A = dz, B = w^T, epi = * scale, masked where the layer input is not > 0
-//                          (the input in bf16 or as 8-bit codes)
-//   group_wgrad  dw[e, n, k] = sum_p dz[p, n] x[row(p), k],  db[e, n] = sum_p dz[p, n]    (fp32)
-//                x in bf16, or 8-bit codes with one scale per 32 columns (act8.h)
 //
 // A workgroup finds its expert by a scan over the group sizes in its own registers.  Accumulation is
 // fp32 on MFMA; nothing is summed by atomics.
@@ -122,7 +115,9 @@ template <bool WHOLE>
 __device__ __forceinline__ bf16x8 begin8_bf(const bf16* row, int c, int n) {
   bf16x8 v = {};
   if (!row || c >= n) return v;
-  if (WHOLE || n >= 8) return __builtin_bit_cast(bf16x8, *reinterpret_cast<const any_bf16x8*>(row + (WHOLE ? c : min(c, n - 8))));
+  if (WHOLE || n >= 8) {
+    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const any_bf16x8*>(row + (WHOLE ? c : min(c, n - 8))));
+  }
   return load8_bf(row, c, n);
 }
 __device__ __forceinline__ void end8_bf(bf16x8& v, int c, int n) {
@@ -165,7 +160,8 @@ __global__ void __launch_bounds__(256) group_pad_kernel(PadArgs a) {
   const long r = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (r >= a.rows) return;
   const int row = group_row(a.map, a.map ? (int)r : 0, a.have, a.top_k);
-  const char* from = a.map ? a.from + (size_t)max(row, 0) * a.lds : a.from + (size_t)(r / a.per) * a.gs + (size_t)(r % a.per) * a.lds;
+  const char* from = a.map ? a.from + (size_t)max(row, 0) * a.lds
+                           : a.from + (size_t)(r / a.per) * a.gs + (size_t)(r % a.per) * a.lds;
   char* to = a.to + (size_t)r * a.ldd;
   for (int c = (threadIdx.x & 63) * 16; c < a.ldd; c += 1024) {
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -335,14 +331,14 @@ __global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs
 }
 
 // ------------------------------------------------------------------ 256 x 256 products
-// 256 threads = 4 waves, one per SIMD, of 128 x 128 outputs (4 x 4 MFMA 32x32x16 tiles: 256
-// accumulators; 32 cycles an MFMA leave room for the other instructions of the one wave).  The reduction runs in 32-deep steps through a ring of 4 LDS buffers (A 16 KB + B 16 KB
-// each).  In step s a wave multiplies fragments that it read during step s - 1, reads those of step s + 1
-// and starts the LDS-DMA of step s + 3, spread between the MFMAs, so that no load is waited for:
-// a fragment has 4 rounds of 128 cycles of MFMA or more to arrive, DMA two steps.  Row fragment i
-// is replaced after its round; the 8 column fragments serve all rounds and are held twice.
+// 256 threads = 4 waves, one per SIMD, of 128 x 128 outputs (4 x 4 MFMA 32x32x16 tiles: 256 accumulators; 32
+// cycles an MFMA leave room for the other instructions of the one wave).  The reduction runs in 32-deep steps
+// through a ring of 4 LDS buffers (A 16 KB + B 16 KB each).  In step s a wave multiplies fragments that it read
+// during step s - 1, reads those of step s + 1 and starts the LDS-DMA of step s + 3, spread between the MFMAs,
+// so that no load is waited for: a fragment has 4 rounds of 128 cycles of MFMA or more to arrive, DMA two
+// steps.  Row fragment i is replaced after its round; the 8 column fragments serve all rounds and are held
+// twice.
 //   Top of step s: the wave's own DMA of step s + 1 has landed; the barrier makes that true for all waves,
-//   and buffer (s + 3) % 4 = (s - 1) % 4 free: its fragments were multiplied in step s - 1.
 // A 128 x 128 block per wave reads 64 KB of fragments a step and CU and writes 32 KB: 768 cycles of LDS
 // against 1024 of MFMA; 128 x 64 blocks (8 waves) need 1024 + 256.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -393,7 +389,10 @@ __device__ __forceinline__ void col_sums(float (&c)[4], const bf16x8 (&fa)[8], i
       "v_dot2c_f32_bf16 %2, 0x3f803f80, %31\n\t" "v_dot2c_f32_bf16 %3, 0x3f803f80, %35\n\t"
       "s_nop 3\n.Lskip%=:"
       : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3])
-      : "v"(u[0].x), "v"(u[0].y), "v"(u[0].z), "v"(u[0].w), "v"(u[1].x), "v"(u[1].y), "v"(u[1].z), "v"(u[1].w), "v"(u[2].x), "v"(u[2].y), "v"(u[2].z), "v"(u[2].w), "v"(u[3].x), "v"(u[3].y), "v"(u[3].z), "v"(u[3].w), "v"(u[4].x), "v"(u[4].y), "v"(u[4].z), "v"(u[4].w), "v"(u[5].x), "v"(u[5].y), "v"(u[5].z), "v"(u[5].w), "v"(u[6].x), "v"(u[6].y), "v"(u[6].z), "v"(u[6].w), "v"(u[7].x), "v"(u[7].y), "v"(u[7].z), "v"(u[7].w), "s"(take)
+      : "v"(u[0].x), "v"(u[0].y), "v"(u[0].z), "v"(u[0].w), "v"(u[1].x), "v"(u[1].y), "v"(u[1].z), "v"(u[1].w),
+        "v"(u[2].x), "v"(u[2].y), "v"(u[2].z), "v"(u[2].w), "v"(u[3].x), "v"(u[3].y), "v"(u[3].z), "v"(u[3].w),
+        "v"(u[4].x), "v"(u[4].y), "v"(u[4].z), "v"(u[4].w), "v"(u[5].x), "v"(u[5].y), "v"(u[5].z), "v"(u[5].w),
+        "v"(u[6].x), "v"(u[6].y), "v"(u[6].z), "v"(u[6].w), "v"(u[7].x), "v"(u[7].y), "v"(u[7].z), "v"(u[7].w), "s"(take)
       : "scc");
 }
 // extra(k): what else the step does, after MFMA k (-1: before all); WAIT: the loads that may be in flight at its
@@ -445,7 +444,8 @@ __device__ __forceinline__ void mm_begin(bf16x8 (&fa)[2 * NI], bf16x8 (&fb)[2][8
 // A whole reduction of ns steps.  stage(i, step): zeros from the step `ns` on (the loop runs on a pair of steps
 // at a time and three steps ahead, without a branch: its registers do not survive one).
 template <int NI, int D, int WAIT, typename ST, typename LA, typename LB, typename EX>
-__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], float (&cs)[NI], int turn, int period, ST stage, LA load_a, LB load_b, EX extra) {
+__device__ __forceinline__ void mm_loop(char* smem, int ns, f32x16 (&acc)[NI][4], float (&cs)[NI], int turn, int period, ST stage,
+                                        LA load_a, LB load_b, EX extra) {
   bf16x8 fa[2 * NI], fb[2][8];
   mm_begin<NI, D, WAIT>(fa, fb, stage, [&](int i) { return load_a(i, smem); }, [&](int j) { return load_b(j, smem); });
   auto step = [&](auto PAR, int s) {
@@ -591,12 +591,12 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
 }
 
 // ---- NT: rows of A and B are K-contiguous, and 32-deep steps would ask the L2 for half lines (57 % of its
-// channels' cycles were requests, 28 % now): so two buffers of 64-deep steps (rows of 128 B, 16-byte chunk c
-// of row r at c ^ ((r >> 1) & 7)).  A step is two halves of 32: in half 0 the fragments of half 1 are read, and in half 1, after its second round, comes
-// the step's one barrier: the wave has read all of its buffer, and its DMA of the next step has landed.
-// Then the next step's first fragments are read, and the DMA of the step after it goes into this
-// step's buffer (12 pieces here, the rest at the start of the next half 0): 8 to 14 rounds of 128
-// cycles to arrive.  A piece is three instructions: the buffers do the bounds (with addresses of 64 bits
+// channels' cycles were requests, 28 % now): so two buffers of 64-deep steps (rows of 128 B, 16-byte chunk c of
+// row r at c ^ ((r >> 1) & 7)).  A step is two halves of 32: in half 0 the fragments of half 1 are read, and in
+// half 1, after its second round, comes the step's one barrier: the wave has read all of its buffer, and its
+// DMA of the next step has landed. Then the next step's first fragments are read, and the DMA of the step after
+// it goes into this step's buffer (12 pieces here, the rest at the start of the next half 0): 8 to 14 rounds of
+// 128 cycles to arrive.  A piece is three instructions: the buffers do the bounds (with addresses of 64 bits
 // and a selected source of zeros it was eight, and the loop 8 % slower).  K a multiple of 8.
 constexpr uint32_t GP_NONE = 0xFFFF0000u;                // an offset past every buffer here, with a step's added too
 constexpr int GN2_K = 64, GN2_PANEL = GP_B * GN2_K * 2, GN2_BUF = 2 * GN2_PANEL;
@@ -1097,7 +1097,9 @@ __device__ __forceinline__ void lds_put(char* __restrict__ p, uint32_t a, uint32
 // (2 tiles_k) == 2 tk + wc), and leave 256 sums for each group and lane, behind the tiles of the workspace:
 // [group + lane][row of tiles][tile column, wave][256].  (group + lane tells the parts of the line
 // apart: from one to the next, one of the two grows.)
-__host__ __device__ __forceinline__ size_t wg_slabs(int tiles, int lanes) { return lanes > 1 ? (size_t)2 * lanes * tiles * GW_SLAB : 0; }
+__host__ __device__ __forceinline__ size_t wg_slabs(int tiles, int lanes) {
+  return lanes > 1 ? (size_t)2 * lanes * tiles * GW_SLAB : 0;
+}
 __device__ __forceinline__ float* wg_sums(const GroupWgArgs& g, int tiles_n, int tiles_k, int lanes, int part, int tn) {
   return g.ws + wg_slabs(tiles_n * tiles_k, lanes) + ((size_t)part * tiles_n + tn) * 2 * tiles_k * GP_B;
 }
@@ -1129,10 +1131,12 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   const int hi = lane >> 5, c16 = lane & 31;
   const int ce = (((c16 >> 1) ^ ((hi << 1) | (wave & 1))) * 2 + (c16 & 1)) * 8;
   const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
-  // 8-bit x: 32 codes (granules 2 q, 2 q + 1) of row xr
-  const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32;
+  // 8-bit x: 32 codes (granules 2 xq, 2 xq + 1) of row xr, in four pieces of 8 (16 bytes as bf16).  A lane's piece in
+  // turn q is q ^ xp: eight neighbouring lanes then write to eight different 16-byte places of 128 bytes (all in
+  // the same order: four in one place, half of the LDS cycles were conflicts, 16384 x 4096 x 4096 took 466 us, 434 so).
+  const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32, xp = xq >> 1;
   const int xf = ((xr & 3) << 1) | ((xr >> 3) & 1);
-  const int xo = GP_PANEL + xr * 512 + (((2 * xq) ^ xf) << 5);        // (granule 2 q + 1: ^ 32)
+  const int xo = GP_PANEL + xr * 512 + ((((2 * xq) ^ xf) << 5) ^ (xp << 4));           // (piece of turn q: ^ q << 4)
   for (; e < g.E && first < u1; ++e) {
     const int steps = wg_steps(g.offs, e, g.S), rows0 = first + GW_SEG;      // (the group's rows begin here)
     first = rows0 + steps;
@@ -1191,29 +1195,42 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
                   2u * i * rb, to);
       }
     };
-    // X8: a step's codes and scale into registers (set), and from there into the image
-    // (as loaded: a row that is none is cleared on the way to the image, where the loads have arrived)
-    uint4 cd[2][2];
+    // X8: a step's codes and scale into registers (set), and from there into the image.  Rows past p1 are zeros: by
+    // the buffer's end; where src says the rows, cleared on the way to the image, where the loads have arrived.
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 cd[2][4];
     uint32_t cs[2], con[2];
-    const bool x0 = k0 + xc < g.K, x1 = k0 + xc + 16 < g.K;     // (columns past K: any values)
+    const int xv = xr * (int)g.ldx + k0 + xc, xsv = xr * sblk + (k0 + xc) / A8_BLOCK;        // (columns past K: any values)
     auto codes_of = [&](int set, int s) {
-      const int p = p0 + s * GP_K + xr;
-      const int row = GATHER ? xrow[set][0] : (p < p1 ? p : -1);
-      con[set] = row >= 0 ? 0xFFFFFFFFu : 0u;
-      const size_t at = row >= 0 ? (size_t)row : 0;     // (row 0 is there: the part has rows)
-      const uint8_t* q = reinterpret_cast<const uint8_t*>(g.x) + at * g.ldx + (x0 ? k0 + xc : 0);
-      cd[set][0] = *reinterpret_cast<const uint4*>(q);
-      cd[set][1] = *reinterpret_cast<const uint4*>(x1 ? q + 16 : q);
-      cs[set] = g.xs[at * sblk + (x0 ? (k0 + xc) / A8_BLOCK : 0)];
+      const int r0 = p0 + s * GP_K;
+      if constexpr (GATHER) {
+        const int row = xrow[set][0];
+        con[set] = row >= 0 ? 0xFFFFFFFFu : 0u;
+        const size_t at = row >= 0 ? (size_t)row : 0;     // (row 0 is there: x has rows)
+        const bool in = k0 + xc < g.K;                    // (columns past K: any values)
+        const uint8_t* c = reinterpret_cast<const uint8_t*>(g.x) + at * g.ldx + (in ? k0 + xc : 0);
+        const int last = in ? (min(32, g.K - k0 - xc) - 1) >> 3 : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) cd[set][q] = *reinterpret_cast<const u32x2*>(c + min(q ^ xp, last) * 8);
+        cs[set] = g.xs[at * sblk + (in ? (k0 + xc) / A8_BLOCK : 0)];
+      } else {
+        const int n = __builtin_amdgcn_readfirstlane(min(max(p1 - r0, 0), GP_K));
+        const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(g.x)) + (size_t)r0 * g.ldx, 0, n * (int)g.ldx, 0x00020000);
+        const __amdgpu_buffer_rsrc_t sc =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.xs) + (size_t)r0 * sblk, 0, n * sblk, 0x00020000);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          cd[set][q] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(c, xv + ((q ^ xp) << 3), 0, 0));
+        cs[set] = __builtin_amdgcn_raw_buffer_load_b8(sc, xsv, 0, 0);
+        con[set] = 0xFFFFFFFFu;
+      }
     };
-    // (in four pieces of 16 bytes)
     auto codes_put = [&](int set, int s, int q) {
       const float f = a8_scale(cs[set]);
-      const uint32_t m = con[set];
-      const uint4 v = cd[set][q >> 1];
-      const uint32_t a = ((q & 1) ? v.z : v.x) & m, b = ((q & 1) ? v.w : v.y) & m;
-      lds_put(smem + (s & (GP_RING - 1)) * GP_BUF + (xo ^ ((q >> 1) << 5)) + (q & 1) * 16, a8_pair_bf16<false>(a, f),
-              a8_pair_bf16<true>(a, f), a8_pair_bf16<false>(b, f), a8_pair_bf16<true>(b, f));
+      const uint32_t a = GATHER ? cd[set][q][0] & con[set] : cd[set][q][0], b = GATHER ? cd[set][q][1] & con[set] : cd[set][q][1];
+      lds_put(smem + (s & (GP_RING - 1)) * GP_BUF + (xo ^ (q << 4)), a8_pair_bf16<false>(a, f), a8_pair_bf16<true>(a, f),
+              a8_pair_bf16<false>(b, f), a8_pair_bf16<true>(b, f));
     };
     auto codes_to = [&](int set, int s) {
 #pragma unroll
@@ -1233,9 +1250,10 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       rows_of(0, 0);
       rows_of(1, 1);
       if constexpr (X8) {
-        // the codes of step s + 3 (read in step s - 2) go to the image in step s, in pieces between the MFMAs, and then those of s + 5 are read; they are in LDS before
-        // the last fragment of step s is read, so before step s + 2 reads them.  At a step's top 3 + 4 + 3 loads
-        // follow the DMA that it waits for: two steps' codes and one's DMA.
+        // the codes of step s + 3 (read in step s - 2) go to the image in step s, in pieces between the MFMAs,
+        // and then those of s + 5 are read; they are in LDS before the last fragment of step s is read, so
+        // before step s + 2 reads them.  At a step's top 5 + 4 + 5 loads (or more) follow the DMA that it waits
+        // for: two steps' codes and one's DMA.
         codes_of(0, 0);
         codes_of(1, 1);
         codes_to(0, 0);
@@ -1249,7 +1267,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         codes_of(0, 4);
         rows_of(1, 5);
         rows_of(0, 6);
-        mm_loop<4, 4, 10>(smem, ns, acc, sum, 2 * tk + wc, 2 * tiles_k, piece_a, load_a, load_b, [&](auto PAR, int s, int k) {
+        mm_loop<4, 4, 14>(smem, ns, acc, sum, 2 * tk + wc, 2 * tiles_k, piece_a, load_a, load_b, [&](auto PAR, int s, int k) {
           constexpr int set = decltype(PAR)::value ^ 1;
           if (k == -1) hide();
           if (k >= 0 && k % 6 == 5 && k / 6 < 4) codes_put(set, s + 3, k / 6);
