@@ -2,6 +2,13 @@
 // e has rows offs[e] .. offs[e + 1) (device memory: no host synchronization, ragged and empty groups
 // allowed); rows behind offs[E] are not touched.
 //
+//   group_nt     out[p, n] = epi(sum_k A[row(p), k] B[e, n, k])      A, B bf16, K-contiguous
+//                forward:  A = x (row(p) = p, or src[p] / top_k: the sorted slot's token), B = w,
+//                          epi = + bias[e, n], relu
+//                gradient: A = dz, B = w^T, epi = * scale, masked where the layer input is not > 0
+//                          (the input in bf16 or as 8-bit codes)
+//   group_wgrad  dw[e, n, k] = sum_p dz[p, n] x[row(p), k],  db[e, n] = sum_p dz[p, n]    (fp32)
+//                x in bf16, or 8-bit codes with one scale per 32 columns (act8.h)
 //
 // A workgroup finds its expert by a scan over the group sizes in its own registers.  Accumulation is
 // fp32 on MFMA; nothing is summed by atomics.
@@ -339,6 +346,7 @@ __global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs
 // steps.  Row fragment i is replaced after its round; the 8 column fragments serve all rounds and are held
 // twice.
 //   Top of step s: the wave's own DMA of step s + 1 has landed; the barrier makes that true for all waves,
+//   and buffer (s + 3) % 4 = (s - 1) % 4 free: its fragments were multiplied in step s - 1.
 // A 128 x 128 block per wave reads 64 KB of fragments a step and CU and writes 32 KB: 768 cycles of LDS
 // against 1024 of MFMA; 128 x 64 blocks (8 waves) need 1024 + 256.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -594,7 +602,7 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
 // channels' cycles were requests, 28 % now): so two buffers of 64-deep steps (rows of 128 B, 16-byte chunk c of
 // row r at c ^ ((r >> 1) & 7)).  A step is two halves of 32: in half 0 the fragments of half 1 are read, and in
 // half 1, after its second round, comes the step's one barrier: the wave has read all of its buffer, and its
-// DMA of the next step has landed. Then the next step's first fragments are read, and the DMA of the step after
+// DMA of the next step has landed.  Then the next step's first fragments are read, and the DMA of the step after
 // it goes into this step's buffer (12 pieces here, the rest at the start of the next half 0): 8 to 14 rounds of
 // 128 cycles to arrive.  A piece is three instructions: the buffers do the bounds (with addresses of 64 bits
 // and a selected source of zeros it was eight, and the loop 8 % slower).  K a multiple of 8.
