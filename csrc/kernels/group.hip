@@ -750,7 +750,8 @@ struct NtPlan {
 };
 static NtPlan nt_plan(const GroupNtArgs& g) {
   NtPlan p{0, 0, 0};
-  if (g.K < 64 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD) return p;
+  // (short reductions too: 31639 rows of 33 experts, 32 -> 3368 masked: 151 to 186 us, 128 x 128 633 to 676)
+  if (g.K < 8 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD) return p;
   // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
   // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
   // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 117 at 192).
@@ -1013,6 +1014,7 @@ __global__ void __launch_bounds__(256) group_wgrad_sum_kernel(GroupWgArgs g) {
   const float* s = i < nw ? g.ws + i : g.ws + (size_t)g.ns * nw + (i - nw);
   const size_t step = i < nw ? nw : (size_t)g.E * g.N;
   float v = s[0];
+#pragma unroll 8
   for (int q = 1; q < g.ns; ++q) v += s[q * step];
   (i < nw ? g.dw[i] : g.db[i - nw]) = v;
 }
@@ -1410,7 +1412,7 @@ static int wgrad_lanes(const GroupWgArgs& g) {
   return best;
 }
 // The operands' copies that the large tile needs (rows of whole 16-byte chunks), as for the NT product: where they
-// and the large tile take less than the 128 x 128 tile (20 us and 60 TFLOP/s for such operands).  Copies against 128 x
+// and the large tile take less than the 128 x 128 tile (20 us and 60 TFLOP/s for such operands, 25 from 8 bits).  Copies against 128 x
 // 128 in us: 25092 rows of 2 groups, 2937 x 3216: 524, 4125, from 8-bit x 560, 6340; 1500 of 16, 1501 x 1001: 62, 73;
 // 20000 of 8, 201 x 401: 54, 76.
 struct WgPlan {
@@ -1427,7 +1429,7 @@ static WgPlan wg_plan(const GroupWgArgs& g) {
   if (z || x) {
     const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
     const double t = (z + x) * 5.0 + (p.pz + p.px) * (2.0 / 4.5e6) + wgrad_time(g, tiles, wgrad_lanes(g));
-    if (t > 20.0 + 2.0 * g.S * g.N * g.K / 60e6 || g.S >= GROUP_PAD_MAX || g.rows >= GROUP_PAD_MAX) p = WgPlan{false, 0, 0};
+    if (t > 20.0 + 2.0 * g.S * g.N * g.K / (g.xs ? 25e6 : 60e6) || g.S >= GROUP_PAD_MAX || g.rows >= GROUP_PAD_MAX) p = WgPlan{false, 0, 0};
   }
   return p;
 }
@@ -1438,16 +1440,25 @@ static long wgrad_ws_floats(const GroupWgArgs& g) {
   return (long)wg_slabs((int)(tn * tk), (int)l) + (g.db ? (g.E + l) * tn * 2 * tk * GP_B : 0);
 }
 
-// Splits of the rows: enough workgroups for two rounds of the 256 CUs while a split keeps 4 steps of 64 rows on
-// average (770 rows, 55 x 40: 21 us; with 8 steps: 42; 4096 rows of 4 groups, 512 x 512: 31, 40).
+// Splits of the rows, within a workgroup for every CU: the least of the steps of 64 rows that follow one another
+// (2.2 us each) and the partial products' way (6 us and their bytes at 4.5 TB/s).  762 rows of 2 groups, 64 x 59: 14
+// us, with 2 steps a split 19, with 4 25; 4096 rows of 4 groups, 512 x 512: 27, with two workgroups for every
+// CU 34; 512 rows of them: 12 unsplit, 17 in two.
 static int wgrad_splits(int S, int N, int K, int E) {
   const long tiles = (long)E * ((N + GN_B - 1) / GN_B) * ((K + GN_B - 1) / GN_B);
   if (tiles <= 0) return 1;
-  long ns = 512 / tiles;
-  const long most = (long)S / E / 256;
-  if (ns > most) ns = most;
-  if (ns > 32) ns = 32;
-  return ns < 1 ? 1 : (int)ns;
+  const int steps = (int)((long)S / E / 64) + 1;
+  const double bytes = 4.0 * E * N * K;
+  int best = 1;
+  double least = 2.2 * steps;
+  for (int ns = 2; ns <= 32 && ns <= steps && ns * tiles <= GW_CUS; ++ns) {
+    const double t = 2.2 * ((steps + ns - 1) / ns) + 6.0 + (2 * ns + 1) * bytes / 4.5e6;
+    if (t < least) {
+      least = t;
+      best = ns;
+    }
+  }
+  return best;
 }
 
 HFM_API long hfm_group_wgrad_ws_floats(const GroupWgArgs* gp) {
