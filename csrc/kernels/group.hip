@@ -352,7 +352,6 @@ __global__ void __launch_bounds__(GS_WAVES * 64) group_nt_few_kernel(GroupNtArgs
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int GP_B = 256, GP_K = 32, GP_THREADS = 256;
 constexpr int GP_PANEL = GP_B * GP_K * 2, GP_BUF = 2 * GP_PANEL, GP_RING = 4;
-constexpr int GP_MIN_TILES = 128;
 
 __device__ __attribute__((aligned(16))) uint32_t g_zero16[4];      // the source of padding chunks
 
@@ -743,46 +742,52 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
 #undef HFM_OUT
 }
 
-// How a call runs: rows a large tile (0: none), and the bytes of the operands' copies for it.
+// How a call runs: rows a large tile (0: one of the small ones, 32 x 32 where `few`), and the bytes of the operands'
+// copies for it.
 struct NtPlan {
   int rows;
   long pa, pb;
+  bool few;
 };
+// The least of three times in us, each as measured:
+//   32 x 32: 3.5, 3 for 1024 tiles, and the operands from the L2s (twice the time for rows that end within 16 bytes);
+//   128 x 128: rounds of 512 tiles, 1.2 a step of 64 with one tile a CU or 1.4 with two, and 10 more (rows at odd
+//   places: 1.5 and 2.7 a step; a mask: 1.4 times);
+//   the large tile, 256 or 192 rows: rounds of 256 tiles, 0.5 a step of 32 and 8 more (12 with a mask) while there
+//   is one round, 0.85 and 12 with more (32768 x 1248 -> 1024, 16 experts: 135 us at 256 rows = 3 rounds, the last one
+//   seventh full; 117 at 192).  It takes 16-byte chunks by LDS-DMA, and rows through 32-bit offsets (all of
+//   x where src says which, else 256 rows): operands that are otherwise are copied first (x with its rows in order).
+// 32 x 32, 128 x 128, large in us: 192 rows of 8 experts, 1248 -> 400: 6, 25, 31; 256 rows, 4096 -> 4096: 66, 66, 59; 4096
+// rows of 4 experts, 512 -> 512: 25, 24, 15; 2048 of 8, 1024 -> 1024 masked: 42, 44, 26; 8192 of 8, 128 -> 64: 7, 17, 9.
+// Copies and large against 128 x 128: 25092 rows of 2 experts, 2937 -> 3216 masked: 555, 1264; 32000 of 16, 255 -> 257
+// masked: 48, 95; short reductions: 31639 of 33, 32 -> 3368 masked: 151 to 186 against 633 to 676.
 static NtPlan nt_plan(const GroupNtArgs& g) {
-  NtPlan p{0, 0, 0};
-  // (short reductions too: 31639 rows of 33 experts, 32 -> 3368 masked: 151 to 186 us, 128 x 128 633 to 676)
+  const bool whole = g.K % 8 == 0, mask = g.mask != nullptr;
+  const long groups = g.E < g.S ? g.E : g.S;                // (those with rows)
+  const bool odd_a = !whole || (uintptr_t)g.a % 16 || g.lda % 8, odd_b = !whole || (uintptr_t)g.b % 16 || g.ldb % 8 || g.es % 8;
+  const double ft = ((double)g.S / GS_B + 0.5 * groups) * ((g.N + GS_B - 1) / GS_B);
+  const double few = (3.5 + ft * (3.0 / 1024) + ft * g.K * 1.2e-5) * (whole ? 1.0 : 2.0);
+  const double st = ((double)g.S / GN_B + 0.5 * groups) * ((g.N + GN_B - 1) / GN_B), steps = (g.K + GN_K - 1) / GN_K;
+  const double step = odd_a || odd_b ? (st <= 256 ? 1.5 : 2.7) : (st <= 256 ? 1.2 : 1.4);
+  const double small = ceil(st / 512) * (step * steps + 10.0) * (mask ? 1.4 : 1.0);
+  NtPlan p{0, 0, 0, few < small && (long)(g.S / GS_B + groups) * ((g.N + GS_B - 1) / GS_B) <= 1l << 20};
   if (g.K < 8 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD) return p;
-  // Rows a tile: 256 or 192, whichever makes less of the last round of the 256 CUs.  A round costs its
-  // steps (0.85 us at 256 rows, in proportion) and 12 us of start and outputs (32768 x 1248 -> 1024, 16
-  // experts: 135 us at 256 rows = 3 rounds, the last one seventh full; 117 at 192).
   const int tn = (g.N + GP_B - 1) / GP_B;
-  const double step = 0.85 / 256 * ((g.K + GP_K - 1) / GP_K);
-  auto cost = [&](int rows) {
-    const double tiles = (g.E == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * g.E) * tn;
-    return ceil(tiles / 256) * (step * rows + 12.0);
+  auto time = [&](int rows) {
+    const double tiles = (groups == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * groups) * tn;
+    const double deep = (g.K + GP_K - 1) / GP_K * (rows / 256.0);
+    const double t = tiles <= 256 ? 0.5 * deep + 8.0 + (mask ? 4.0 : 0.0) : ceil(tiles / 256) * (0.85 * deep + 12.0);
+    return t + groups * tn / 256.0;                          // (workgroups without a tile: the grid is made for the most)
   };
-  const int rows = cost(192) < cost(256) ? 192 : 256;
-  const long blocks = (long)(g.S / rows + g.E) * tn;
-  if (blocks < GP_MIN_TILES || blocks > 0x7FFFFFFFl) return p;
-  // The LDS-DMA takes 16-byte chunks, and rows through 32-bit offsets (all of x where src says which, else 256 rows):
-  // operands that are otherwise are copied (x with its rows in order), where the copies at 4.5 TB/s and the large
-  // tile take less than the 128 x 128 tile (rounds of 512 tiles, 2.7 us a step and 10 more for such operands,
-  // half as much again with a mask).  Copies against 128 x 128 in us: 25092 rows of 2 experts, 2937 -> 3216 masked:
-  // 555, 1264; 32000 of 16, 255 -> 257 masked: 48, 95; 129 -> 131: 26, 41; 1500 of 16, 1001 -> 1501: 48, 39.
-  const bool whole = g.K % 8 == 0;
-  const bool a = !whole || (uintptr_t)g.a % 16 || g.lda % 8 || (g.src ? (long)g.rows * g.lda : 256l * g.lda) >= 0x7F000000l;
-  const bool b = !whole || (uintptr_t)g.b % 16 || g.ldb % 8 || g.es % 8 || 256l * g.ldb >= 0x7F000000l;
-  const long row = up16(2l * g.K);
-  if (a) p.pa = (long)g.S * row;
-  if (b) p.pb = (long)g.E * g.N * row;
-  if (a || b) {
-    const double t = (a + b) * 3.0 + (p.pa + p.pb) * (2.0 / 4.5e6) + cost(rows);
-    const double tiles = ((double)g.S / GN_B + 0.5 * g.E) * ((g.N + GN_B - 1) / GN_B);
-    const double small = ceil(tiles / 512) * (2.7 * ((g.K + GN_K - 1) / GN_K) + 10.0) * (g.mask ? 1.5 : 1.0);
-    if (t > small || g.S >= GROUP_PAD_MAX || (long)g.E * g.N >= GROUP_PAD_MAX) return NtPlan{0, 0, 0};
-  }
-  p.rows = rows;
-  return p;
+  const int rows = time(192) < time(256) ? 192 : 256;
+  const bool a = odd_a || (g.src ? (long)g.rows * g.lda : 256l * g.lda) >= 0x7F000000l;
+  const bool b = odd_b || 256l * g.ldb >= 0x7F000000l;
+  const long row = up16(2l * g.K), pa = a ? (long)g.S * row : 0, pb = b ? (long)g.E * g.N * row : 0;
+  const double big = time(rows) + (a + b) * 5.0 + (pa + pb) * (2.0 / 4e6);
+  if (big >= (p.few ? few : small) || (g.S / rows + groups) * tn > 0xFFFFFFl || (a && g.S >= GROUP_PAD_MAX) ||
+      (b && (long)g.E * g.N >= GROUP_PAD_MAX))
+    return p;
+  return NtPlan{rows, pa, pb, false};
 }
 
 HFM_API long hfm_group_nt_ws_bytes(const GroupNtArgs* gp) {
@@ -816,7 +821,8 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
     }
     g.K = (int)(up16(2l * g.K) / 2);
     const int tn = (g.N + GP_B - 1) / GP_B;
-    const dim3 grid((unsigned)((long)(g.S / p.rows + g.E) * tn)), blk(GP_THREADS);
+    const long groups = g.E < g.S ? g.E : g.S;
+    const dim3 grid((unsigned)((g.S / p.rows + groups) * tn)), blk(GP_THREADS);
     // bf16 outputs in column pairs, with their masks, where the rows are pairs
     const bool pairs = g.N % 2 == 0 && g.ldo % 2 == 0 && g.ldm % 2 == 0 && (uintptr_t)g.out % 4 == 0 &&
                        (uintptr_t)g.mask % (g.mask8 ? 2 : 4) == 0;
@@ -825,19 +831,14 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
     else hipLaunchKernelGGL(group_nt_mm_kernel<3>, grid, blk, 0, st, g, tn, out);
     HFM_LAUNCH_CHECK();
   }
-  const int tn = (g.N + GN_B - 1) / GN_B;
-  const long blocks = (long)(g.S / GN_B + g.E) * tn;      // (each group adds less than one tile)
-  // Few rows: a 128 x 128 tile's workgroup takes 1.4 us for each of its 64-deep steps, two at a time on a CU;
-  // the 32 x 32 tiles' operands come from the L2s at 8 TB/s or so.  32 x 32 against 128 x 128 in us: 32 rows,
-  // 4096 -> 4096: 19, 60; 128 rows: 34, 66; 256 rows: 66, 66; 1024 rows: 262, 67; 1024 rows of 8 experts, 1024
-  // -> 1024: 20, 28; 2048: 35, 29; 5000 rows, 256 -> 1024: 35, 21; 8192 rows of 8 experts, 128 -> 64: 4.8, 17.
-  const int fn = (g.N + GS_B - 1) / GS_B;
-  const long few = (long)(g.S / GS_B + g.E) * fn;
-  if (few <= 1l << 20 &&
-      few * g.K * (4.0 * GS_B / 8e6) < ceil(blocks / 512.0) * ((g.K + GN_K - 1) / GN_K) * 1.4) {
-    hipLaunchKernelGGL(group_nt_few_kernel, dim3((unsigned)few), dim3(GS_WAVES * 64), 0, st, g, fn);
+  const long groups = g.E < g.S ? g.E : g.S;               // (each adds less than one tile)
+  if (p.few) {
+    const int fn = (g.N + GS_B - 1) / GS_B;
+    hipLaunchKernelGGL(group_nt_few_kernel, dim3((unsigned)((g.S / GS_B + groups) * fn)), dim3(GS_WAVES * 64), 0, st, g, fn);
     HFM_LAUNCH_CHECK();
   }
+  const int tn = (g.N + GN_B - 1) / GN_B;
+  const long blocks = (g.S / GN_B + groups) * tn;
   if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL(group_nt_kernel, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
   HFM_LAUNCH_CHECK();
