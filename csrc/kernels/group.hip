@@ -1380,15 +1380,16 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
   }
 }
 
-// Where the large tile is taken: operands with 16-byte rows, and enough work for every CU (GP_MIN_UNITS
-// steps of 64 rows each; below that the 128 x 128 tile's smaller pieces fill the chip better).  128 x 128 against
-// 256 x 256 in us, one group: 16384 rows, 256 x 256: 32, 44; 32768: 48, 56; 1024 rows, 1024 x 1024: 28, 26; 4096: 52,
-// 35; 16384: 145, 58; 4 groups, 4096 rows, 512 x 512: 38, 35; 16 groups, 32768 rows, 1024 x 1024: 290, 115.
+// Where the large tile is taken: enough work for every CU (GP_MIN_UNITS steps of 64 rows each, from 8 bits half as
+// many; below that the 128 x 128 tile's smaller pieces fill the chip better).  128 x 128 against 256 x 256 in us, one
+// group: 16384 rows, 256 x 256: 32, 44 (8 bits: 52, 46); 32768: 48, 56; 1024 rows, 1024 x 1024: 28, 26; 4096: 52, 35;
+// 16384: 145, 58; 4 groups, 4096 rows, 512 x 512: 27, 35 (8 bits: 44, 34); 16 groups, 32768 rows, 1024 x
+// 1024: 290, 115.
 constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
 static bool wgrad_big(const GroupWgArgs& g) {
   if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD || g.E > 65535) return false;      // (32-bit offsets; grid)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
-  return g.rows > 0 && tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS;
+  return g.rows > 0 && tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS / (g.xs ? 2 : 1);
 }
 // Time in us by l lanes: the rounds of the CUs times a lane's length (its rows, and a group's own cost); then
 // the parts' way through the workspace (0.065 us each, as many as there are cuts through rows) and the
@@ -1413,9 +1414,9 @@ static int wgrad_lanes(const GroupWgArgs& g) {
   return best;
 }
 // The operands' copies that the large tile needs (rows of whole 16-byte chunks), as for the NT product: where they
-// and the large tile take less than the 128 x 128 tile (20 us and 60 TFLOP/s for such operands, 25 from 8 bits).  Copies against 128 x
-// 128 in us: 25092 rows of 2 groups, 2937 x 3216: 524, 4125, from 8-bit x 560, 6340; 1500 of 16, 1501 x 1001: 62, 73;
-// 20000 of 8, 201 x 401: 54, 76.
+// and the large tile take less than the 128 x 128 tile (20 us and 60 TFLOP/s of whole tiles for such operands,
+// 25 from 8 bits).  Copies against 128 x 128 in us: 25092 rows of 2 groups, 2937 x 3216: 524, 4125, from 8-bit x
+// 560, 6340; 1500 of 16, 1501 x 1001: 62, 73; 20000 of 8, 201 x 401: 54, 76; 26966 of 10, 42 x 2191: 114, 223.
 struct WgPlan {
   bool big;
   long pz, px;
@@ -1430,7 +1431,8 @@ static WgPlan wg_plan(const GroupWgArgs& g) {
   if (z || x) {
     const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
     const double t = (z + x) * 5.0 + (p.pz + p.px) * (2.0 / 4.5e6) + wgrad_time(g, tiles, wgrad_lanes(g));
-    if (t > 20.0 + 2.0 * g.S * g.N * g.K / (g.xs ? 25e6 : 60e6) || g.S >= GROUP_PAD_MAX || g.rows >= GROUP_PAD_MAX) p = WgPlan{false, 0, 0};
+    const double wide = 2.0 * g.S * ((g.N + GN_B - 1) / GN_B * GN_B) * ((g.K + GN_B - 1) / GN_B * GN_B);
+    if (t > 20.0 + wide / (g.xs ? 25e6 : 60e6) || g.S >= GROUP_PAD_MAX || g.rows >= GROUP_PAD_MAX) p = WgPlan{false, 0, 0};
   }
   return p;
 }
