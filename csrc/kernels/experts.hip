@@ -344,12 +344,32 @@ __global__ void __launch_bounds__(256) route_scan_kernel(RouteArgs a) {
   if (q == 0) a.bh[(size_t)a.nblk * a.E + e] = all;
 }
 
-template <int W>
+// SCAN: after route_scan_kernel; without it (up to 64 experts) a block sums what it needs by itself.
+template <int W, bool SCAN>
 __global__ void __launch_bounds__(64 * W) route_place_kernel(RouteArgs a) {
-  __shared__ int base[2 * RT_MAXE + 1];
+  __shared__ int base[2 * RT_MAXE + 1], sums[128];
   const int b = blockIdx.x;
-  route_place<W>(a, b, base, base + 2 * RT_MAXE, a.bh + (size_t)b * a.E, a.bh + (size_t)a.nblk * a.E,
-                 a.wpre + (size_t)b * W * a.E);
+  const int *before = a.bh + (size_t)b * a.E, *all = a.bh + (size_t)a.nblk * a.E;
+  if (!SCAN) {
+    const int e = threadIdx.x & 63;
+    if (threadIdx.x < 128) sums[threadIdx.x] = 0;
+    __syncthreads();
+    if (e < a.E) {
+      int n = 0, m = 0;
+#pragma unroll 16
+      for (int r = threadIdx.x >> 6; r < a.nblk; r += W) {
+        const int c = a.bh[(size_t)r * a.E + e];
+        m += c;
+        n += r < b ? c : 0;
+      }
+      atomicAdd(&sums[e], n);                // (integers: the order does not matter)
+      atomicAdd(&sums[64 + e], m);
+    }
+    __syncthreads();
+    before = sums;
+    all = sums + 64;
+  }
+  route_place<W>(a, b, base, base + 2 * RT_MAXE, before, all, a.wpre + (size_t)b * W * a.E);
 }
 
 static int route_group(int E) {
@@ -413,9 +433,12 @@ HFM_API int hfm_route(const RouteArgs* ap, hipStream_t st) {
   }
 #undef HFM_ROUTE
   if (a.nblk > 1) {
-    hipLaunchKernelGGL(route_scan_kernel, dim3((a.E + 15) / 16), dim3(256), 0, st, a);
-    if (W == 8) hipLaunchKernelGGL(route_place_kernel<8>, grid, blk, 0, st, a);
-    else hipLaunchKernelGGL(route_place_kernel<16>, grid, blk, 0, st, a);
+    // (16384 x 64 with its gradient, from Python: 32 us with the scan's launch, 29 so)
+    if (a.E > 64) hipLaunchKernelGGL(route_scan_kernel, dim3((a.E + 15) / 16), dim3(256), 0, st, a);
+    if (a.E > 64 && W == 8) hipLaunchKernelGGL((route_place_kernel<8, true>), grid, blk, 0, st, a);
+    else if (a.E > 64) hipLaunchKernelGGL((route_place_kernel<16, true>), grid, blk, 0, st, a);
+    else if (W == 8) hipLaunchKernelGGL((route_place_kernel<8, false>), grid, blk, 0, st, a);
+    else hipLaunchKernelGGL((route_place_kernel<16, false>), grid, blk, 0, st, a);
   }
   HFM_LAUNCH_CHECK();
 }
