@@ -380,7 +380,8 @@ def test_group_wgrad(sizes, K, N, x8):
 
 LARGE = [([9000, 0, 257, 1, 5000, 256], 200, 1032), ([20000], 64, 777), ([3] * 150, 72, 40), ([700, 4000, 1300], 1248, 2048),
          ([1, 0, 30000], 136, 264), ([5000, 6000], 512, 1000), ([6000, 0, 7000], 517, 1003), ([3000, 2500, 1], 1032, 1000),
-         ([9000], 1001, 390)]
+         ([9000], 1001, 390), ([9000, 0, 700], 40, 1000), ([9000, 700], 1000, 40), ([5000, 4000], 33, 1001),
+         ([5000, 4000], 1001, 33), ([700, 300], 512, 512), ([1500, 0, 500], 1024, 328), ([2100], 8, 2048), ([2100], 2048, 16)]
 
 
 @pytest.mark.parametrize("S,K,N", [(300, 40, 72), (9000, 320, 512)])
