@@ -598,20 +598,23 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
 }
 
 // ---- NT: rows of A and B are K-contiguous, and 32-deep steps would ask the L2 for half lines (57 % of its
-// channels' cycles were requests, 28 % now): so two buffers of 64-deep steps (rows of 128 B, 16-byte chunk c of
-// row r at c ^ ((r >> 1) & 7)).  A step is two halves of 32: in half 0 the fragments of half 1 are read, and in
-// half 1, after its second round, comes the step's one barrier: the wave has read all of its buffer, and its
-// DMA of the next step has landed.  Then the next step's first fragments are read, and the DMA of the step after
-// it goes into this step's buffer (12 pieces here, the rest at the start of the next half 0): 8 to 14 rounds of
-// 128 cycles to arrive.  A piece is three instructions: the buffers do the bounds (with addresses of 64 bits
-// and a selected source of zeros it was eight, and the loop 8 % slower).  K a multiple of 8.
+// channels' cycles were requests, 28 % now): so steps of 64 (rows of 128 B, 16-byte chunk c of row r at
+// c ^ ((r >> 1) & 7)), A's in a ring of three panels and w's in two, which is all of the LDS.  A step is two halves
+// of 32: in half 0 the fragments of half 1 are read, and in half 1, after its second round, comes the step's one
+// barrier: the wave has read all of its panels, and its DMA of the next step has landed.  Then the next step's
+// first fragments are read, and the DMA of w's step after it goes into this step's panel; A's is a step further
+// ahead, and at the barrier its last panel may still be on its way (two panels each: 32768 x 1248 -> 1024 of 16 experts 107
+// to 112 us, now 101 to 106; 8192 x 1024 -> 2048 of 8 masked 57.2, now 56.1; the others 0 to 2 %).
+// A piece is three instructions: the buffers do the bounds (with addresses of 64 bits and a selected source of
+// zeros it was eight, and the loop 8 % slower).  K a multiple of 8.
 constexpr uint32_t GP_NONE = 0xFFFF0000u;                // an offset past every buffer here, with a step's added too
-constexpr int GN2_K = 64, GN2_PANEL = GP_B * GN2_K * 2, GN2_BUF = 2 * GN2_PANEL;
+constexpr int GN2_K = 64, GN2_PANEL = GP_B * GN2_K * 2;
 
 template <int NI>
 __global__ void __launch_bounds__(GP_THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
 group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * GN2_BUF];
+  constexpr int PANEL_A = 64 * NI * GN2_K * 2, RING_B = 3 * PANEL_A;
+  __shared__ __attribute__((aligned(16))) char smem[RING_B + 2 * GN2_PANEL];
   // (the grid has room for one more row tile per group: the tiles that there are go round the XCDs)
   const int tiles_m = group_tiles<64 * NI>(g.offs, g.E, g.S);
   if ((int)blockIdx.x >= tiles_m * tiles_n) return;
@@ -628,7 +631,7 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
   int fo[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) fo[q] = fr * 128 + (((2 * q + fq) ^ sw) << 4);
-  const int la = wr * 32 * NI * 128, lb = GN2_PANEL + wc * 128 * 128;
+  const int la = wr * 32 * NI * 128, lb = wc * 128 * 128;
   // staging pieces of 8 rows x 128 B: 2 NI of A and 8 of B per wave, from buffers that end with the group's
   // rows (with x, where rows are taken through src) and with w's: what lies past them reads as zeros.
   constexpr int PA = 2 * NI, PN = PA + 8;
@@ -652,12 +655,17 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
                                              2u * (uint32_t)((g.src ? g.rows : min(r1 - r0, 64 * NI)) * (uint32_t)g.lda));
   const __amdgpu_buffer_rsrc_t bb = out_rows(g.b + (size_t)e * g.es + (size_t)n0 * g.ldb,
                                              2u * (uint32_t)min(g.N - n0, GP_B) * (uint32_t)g.ldb);
-  auto stage = [&](int p, int t) {
-    // (a chunk past K: zeros too)
-    const uint32_t v = t * GN2_K + (odd_piece(p) ? ck0 ^ 32 : ck0) < g.K ? off[p] : GP_NONE;
-    char* to = smem + (t & 1) * GN2_BUF + (p < PA ? (wave * PA + p) * 1024 : GN2_PANEL + (wave * 8 + p - PA) * 1024);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(p < PA ? ab : bb, (__attribute__((address_space(3))) void*)to, 16, (int)v,
-                                             t * GN2_K * 2, 0, 0);
+  // piece i of step t, w's and A's, the latter into the panel at `to` (a chunk past K: zeros too)
+  auto stage_b = [&](int i, int t) {
+    const uint32_t v = t * GN2_K + (odd_piece(PA + i) ? ck0 ^ 32 : ck0) < g.K ? off[PA + i] : GP_NONE;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        bb, (__attribute__((address_space(3))) void*)(smem + RING_B + (t & 1) * GN2_PANEL + (wave * 8 + i) * 1024), 16, (int)v,
+        t * GN2_K * 2, 0, 0);
+  };
+  auto stage_a = [&](int i, int t, int to) {
+    const uint32_t v = t * GN2_K + (odd_piece(i) ? ck0 ^ 32 : ck0) < g.K ? off[i] : GP_NONE;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ab, (__attribute__((address_space(3))) void*)(smem + to + (wave * PA + i) * 1024), 16,
+                                             (int)v, t * GN2_K * 2, 0, 0);
   };
   // fragments r = 0 .. 2 NI - 1 of a half: quarter 2 h + r / NI, rows 32 (r % NI) ..
   auto load_a = [&](int r, int h, const char* b) {
@@ -666,24 +674,30 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
   auto load_b = [&](int j, int h, const char* b) {
     return *reinterpret_cast<const bf16x8*>(b + lb + fo[2 * h + (j >> 2)] + (j & 3) * 32 * 128);
   };
-  constexpr int NA = 2 * NI, EARLY = 2 * (NA - 2);           // pieces that follow the barrier (two a round)
+  constexpr int NA = 2 * NI, EARLY = 2 * (NA - 2);           // pieces that follow the barrier (two a round): w's, then A's
   const int nt = (g.K + GN2_K - 1) / GN2_K;
+  static_assert(EARLY >= 8 && EARLY - 8 <= PA, "w's pieces all follow the barrier");
+  // (as the steps issue them: all but those of step 0 may be on their way)
 #pragma unroll
-  for (int p = 0; p < PN; ++p) stage(p, 0);
+  for (int s = 0; s < 3; ++s) {
 #pragma unroll
-  for (int p = 0; p < EARLY; ++p) stage(p, 1);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(EARLY) : "memory");
+    for (int i = 0; i < (s < 2 ? PA : EARLY - 8); ++i) stage_a(i, s, s * PANEL_A);
+#pragma unroll
+    for (int i = 0; i < (s < 2 ? 8 : 0); ++i) stage_b(i, s);
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PA + EARLY) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   bf16x8 fa[NA], fb[2][8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) fb[0][j] = load_b(j, 0, smem);
+  for (int j = 0; j < 8; ++j) fb[0][j] = load_b(j, 0, smem + RING_B);
 #pragma unroll
   for (int r = 0; r < NA - 1; ++r) fa[r] = load_a(r, 0, smem);
   f32x16 acc[NI][4] = {};
+  int pa = 0, qa = PANEL_A, ra = 2 * PANEL_A;                // A's panels of the steps t, t + 1, t + 2
   for (int t = 0; t < nt; ++t) {
-    const char* cur = smem + (t & 1) * GN2_BUF;
-    const char* nxt = smem + ((t + 1) & 1) * GN2_BUF;
+    const char *cur = smem + pa, *nxt = smem + qa;
+    const char *bcur = smem + RING_B + (t & 1) * GN2_PANEL, *bnxt = smem + RING_B + ((t + 1) & 1) * GN2_PANEL;
     // (a row fragment is read after its round, the last one after the next half's first MFMA: nothing is
     // read just before a half begins, where the compiler waits for all reads)
     constexpr int FB0 = 2, FB1 = NI == 4 ? 2 : 3;            // column fragments a round, in halves 0 and 1
@@ -696,9 +710,9 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
       if (j == 0 && r > 0) fa[r - 1] = load_a(r - 1, 1, cur);
       if (j == 2) {
 #pragma unroll
-        for (int i = FB0 * r; i < FB0 * r + FB0 && i < 8; ++i) fb[1][i] = load_b(i, 1, cur);
+        for (int i = FB0 * r; i < FB0 * r + FB0 && i < 8; ++i) fb[1][i] = load_b(i, 1, bcur);
       }
-      if ((j & 1) && EARLY + 2 * r + (j >> 1) < PN) stage(EARLY + 2 * r + (j >> 1), t + 1);
+      if ((j & 1) && EARLY + 2 * r + (j >> 1) < PN) stage_a(EARLY - 8 + 2 * r + (j >> 1), t + 2, ra);
       __builtin_amdgcn_sched_barrier(0);
     }
     // half 1
@@ -708,7 +722,7 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
       acc[r % NI][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[r], fb[1][(r / NI) * 4 + j], acc[r % NI][j], 0, 0, 0);
       if (k == 0) fa[NA - 1] = load_a(NA - 1, 1, cur);
       if (k == 7) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PA) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");      // (no access moves over the barrier)
       }
@@ -719,12 +733,20 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
         }
         if (j == 2) {
 #pragma unroll
-          for (int i = FB1 * (r - 2); i < FB1 * (r - 2) + FB1 && i < 8; ++i) fb[0][i] = load_b(i, 0, nxt);
+          for (int i = FB1 * (r - 2); i < FB1 * (r - 2) + FB1 && i < 8; ++i) fb[0][i] = load_b(i, 0, bnxt);
         }
-        if (j & 1) stage(2 * (r - 2) + (j >> 1), t + 2);
+        if (j & 1) {
+          const int i = 2 * (r - 2) + (j >> 1);
+          if (i < 8) stage_b(i, t + 2);
+          else stage_a(i - 8, t + 3, pa);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    const int x = pa;
+    pa = qa;
+    qa = ra;
+    ra = x;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (nothing in flight into LDS at the end)
   const int row0 = r0 + wr * 32 * NI, n1 = n0 + wc * 128;
@@ -754,13 +776,13 @@ struct NtPlan {
 //   128 x 128: rounds of 512 tiles, 1.2 a step of 64 with one tile a CU or 1.4 with two, and 10 more (rows at odd
 //   places: 1.5 and 2.7 a step; a mask: 1.4 times);
 //   the large tile, 256 or 192 rows: rounds of 256 tiles, 0.5 a step of 32 and 8 more (12 with a mask) while there
-//   is one round, 0.85 and 12 with more (32768 x 1248 -> 1024, 16 experts: 135 us at 256 rows = 3 rounds, the last one
-//   seventh full; 117 at 192).  It takes 16-byte chunks by LDS-DMA, and rows through 32-bit offsets (all of
+//   is one round, 0.85 and 12 with more (32768 x 1248 -> 1024, 16 experts: 114 us at 256 rows = 3 rounds, the last one
+//   seventh full; 102 to 105 at 192).  It takes 16-byte chunks by LDS-DMA, and rows through 32-bit offsets (all of
 //   x where src says which, else 256 rows): operands that are otherwise are copied first (x with its rows in order).
-// 32 x 32, 128 x 128, large in us: 192 rows of 8 experts, 1248 -> 400: 6, 25, 31; 256 rows, 4096 -> 4096: 66, 66, 59; 4096
-// rows of 4 experts, 512 -> 512: 25, 24, 15; 2048 of 8, 1024 -> 1024 masked: 42, 44, 26; 8192 of 8, 128 -> 64: 7, 17, 9.
-// Copies and large against 128 x 128: 25092 rows of 2 experts, 2937 -> 3216 masked: 555, 1264; 32000 of 16, 255 -> 257
-// masked: 48, 95; short reductions: 31639 of 33, 32 -> 3368 masked: 151 to 186 against 633 to 676.
+// 32 x 32, 128 x 128, large in us: 192 rows of 8 experts, 1248 -> 400: 7, 25, 22; 256 rows, 4096 -> 4096: 66, 66, 56; 4096
+// rows of 4 experts, 512 -> 512: 25, 24, 14; 2048 of 8, 1024 -> 1024 masked: 42, 44, 25; 8192 of 8, 128 -> 64: 7, 17, 9.
+// Copies and large against 128 x 128: 25092 rows of 2 experts, 2937 -> 3216 masked: 530, 1264; 32000 of 16, 255 -> 257
+// masked: 49, 95; short reductions: 31639 of 33, 32 -> 3368 masked: 174 to 183 against 633 to 676.
 static NtPlan nt_plan(const GroupNtArgs& g) {
   const bool whole = g.K % 8 == 0, mask = g.mask != nullptr;
   const long groups = g.E < g.S ? g.E : g.S;                // (those with rows)
