@@ -653,8 +653,9 @@ group_nt_mm_kernel(GroupNtArgs g, int tiles_n, int out) {
   }
   const __amdgpu_buffer_rsrc_t ab = out_rows(g.src ? g.a : g.a + (size_t)r0 * g.lda,
                                              2u * (uint32_t)((g.src ? g.rows : min(r1 - r0, 64 * NI)) * (uint32_t)g.lda));
+  // (w's rows may share memory, by a stride from 0 on: the last one ends K elements after its start)
   const __amdgpu_buffer_rsrc_t bb = out_rows(g.b + (size_t)e * g.es + (size_t)n0 * g.ldb,
-                                             2u * (uint32_t)min(g.N - n0, GP_B) * (uint32_t)g.ldb);
+                                             2u * ((uint32_t)(min(g.N - n0, GP_B) - 1) * (uint32_t)g.ldb + (uint32_t)g.K));
   // piece i of step t, w's and A's, the latter into the panel at `to` (a chunk past K: zeros too)
   auto stage_b = [&](int i, int t) {
     const uint32_t v = t * GN2_K + (odd_piece(PA + i) ? ck0 ^ 32 : ck0) < g.K ? off[PA + i] : GP_NONE;

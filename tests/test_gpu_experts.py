@@ -737,3 +737,38 @@ def test_layer_again_other_stream_and_graph():
             graph.replay()
             layer(EX, A8, *b, 2, True)              # eager work between the replays
             same(out, want)
+
+
+SHARED = [(9000, 1024, 512), (9000, 320, 600), (9000, 333, 601), (700, 256, 256), (150, 40, 72)]
+
+
+@pytest.mark.parametrize("S,K,N", SHARED)
+@pytest.mark.parametrize("stride", [0, 3, 8, 64])
+def test_weights_whose_rows_share_memory(S, K, N, stride):
+    """Rows a stride apart that is less than their length, in a weight of its own for every expert and in one for all,
+    whichever tile the sizes take."""
+    EX, _ = ops()
+    g = torch.Generator(device=DEV).manual_seed(S + K + stride)
+    offs = [0, S // 3, S - 7]
+    o = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    x = torch.randn(S, K, device=DEV, generator=g).bfloat16()
+    mask = torch.randn(S, N, device=DEV, generator=g).bfloat16()
+    b = torch.randn(2, N, device=DEV, generator=g)
+    src = torch.randperm(S, device=DEV, generator=g).int()
+    es = -(-((N - 1) * stride + K) // 8) * 8
+    buf = torch.randn(2 * es, device=DEV, generator=g).bfloat16()
+    for step in (es, 0):
+        w = buf.as_strided((2, N, K), (step, stride, 1))
+        results = (("linear", EX.group_linear(x, w, b, o), x), ("through src", EX.group_linear(x, w, b, o, src=src), x[src.long()]),
+                   ("gradient", EX.group_dgrad(x, w, o), x), ("masked", EX.group_dgrad(x, w, o, mask=mask), x))
+        for what, y, a in results:
+            for e in range(2):
+                rows = slice(offs[e], offs[e + 1])
+                ad, wd = a[rows].double(), w[e].double().contiguous()
+                want, mag = ad @ wd.T, ad.abs() @ wd.abs().T
+                if what in ("linear", "through src"):
+                    want = want + b[e].double()
+                if what == "masked":
+                    want = torch.where(mask[rows] > 0, want, 0.0)
+                bound = HALF[torch.bfloat16] * want.abs() + 1.01 * 2.0 ** -23 * ((K + 4) * mag + want.abs())
+                assert bool(((y[rows].double() - want).abs() <= bound).all()), (what, step, e)
