@@ -1234,7 +1234,8 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     u32x2 cd[2][4];
     uint32_t cs[2], con[2];
-    const int xv = xr * (int)g.ldx + k0 + xc, xsv = xr * sblk + (k0 + xc) / A8_BLOCK;        // (columns past K: any values)
+    // (columns past K: any values of the next row, zeros behind the last)
+    const int xv = xr * (int)g.ldx + k0 + xc, xsv = xr * sblk + (k0 + xc) / A8_BLOCK;
     auto codes_of = [&](int set, int s) {
       const int r0 = p0 + s * GP_K;
       if constexpr (GATHER) {
@@ -1249,8 +1250,11 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         cs[set] = g.xs[at * sblk + (in ? (k0 + xc) / A8_BLOCK : 0)];
       } else {
         const int n = __builtin_amdgcn_readfirstlane(min(max(p1 - r0, 0), GP_K));
+        // (the codes end with the last row's K: what lies behind it may be nobody's, where they are columns of wider rows.
+        // A K that is no multiple of 8 has its copies' rows, which go on in zeros)
         const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(g.x)) + (size_t)r0 * g.ldx, 0, n * (int)g.ldx, 0x00020000);
+            const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(g.x)) + (size_t)r0 * g.ldx, 0,
+            n > 0 ? (n - 1) * (int)g.ldx + (g.K + 7) / 8 * 8 : 0, 0x00020000);
         const __amdgpu_buffer_rsrc_t sc =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.xs) + (size_t)r0 * sblk, 0, n * sblk, 0x00020000);
 #pragma unroll

@@ -772,3 +772,27 @@ def test_weights_whose_rows_share_memory(S, K, N, stride):
                     want = torch.where(mask[rows] > 0, want, 0.0)
                 bound = HALF[torch.bfloat16] * want.abs() + 1.01 * 2.0 ** -23 * ((K + 4) * mag + want.abs())
                 assert bool(((y[rows].double() - want).abs() <= bound).all()), (what, step, e)
+
+
+@pytest.mark.parametrize("K,off", [(384, 128), (1040, 64), (528, 48), (4000, 96), (1001, 40)])
+def test_weight_gradient_from_columns_of_wider_codes(K, off):
+    """Codes that are columns of wider rows, up to the last element of their storage: nothing beside them is taken."""
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(K)
+    S, N = 16384, 520
+    offs = [0, 9001, S]
+    dz, x = (torch.randn(*s, device=DEV, generator=g).bfloat16() for s in ((S, N), (S, K)))
+    a = A8.pack(x)
+    wide = torch.full((S, off + K), 127, dtype=torch.uint8, device=DEV)         # (127: NaN)
+    wide[:, off:] = a.codes
+    o = torch.tensor(offs, dtype=torch.int32, device=DEV)
+    src = torch.arange(S, dtype=torch.int32, device=DEV)
+    v = A8.unpack(a, torch.float32).double()
+    for kw in (dict(), dict(src=src)):
+        dw, db = EX.group_wgrad(dz, A8.Act8(wide[:, off:], a.scales), o, **kw)
+        for e in range(2):
+            lo, hi = offs[e], offs[e + 1]
+            z = dz[lo:hi].double()
+            c = 1.01 * (hi - lo + 4) * 2.0 ** -23
+            assert bool(((dw[e].double() - z.T @ v[lo:hi]).abs() <= c * (z.abs().T @ v[lo:hi].abs())).all()), (len(kw), e)
+            assert bool(((db[e].double() - z.sum(0)).abs() <= c * z.abs().sum(0)).all()), (len(kw), e)
