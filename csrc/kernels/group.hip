@@ -1235,6 +1235,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     u32x2 cd[2][4];
     uint32_t cs[2], con[2];
     // (columns past K: any values of the next row, zeros behind the last)
+    const int behind = (int)g.ldx - (g.K + 7) / 8 * 8;
     const int xv = xr * (int)g.ldx + k0 + xc, xsv = xr * sblk + (k0 + xc) / A8_BLOCK;
     auto codes_of = [&](int set, int s) {
       const int r0 = p0 + s * GP_K;
@@ -1254,7 +1255,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
         // A K that is no multiple of 8 has its copies' rows, which go on in zeros)
         const __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(g.x)) + (size_t)r0 * g.ldx, 0,
-            n > 0 ? (n - 1) * (int)g.ldx + (g.K + 7) / 8 * 8 : 0, 0x00020000);
+            max(n * (int)g.ldx - behind, 0), 0x00020000);
         const __amdgpu_buffer_rsrc_t sc =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.xs) + (size_t)r0 * sblk, 0, n * sblk, 0x00020000);
 #pragma unroll
