@@ -1,5 +1,8 @@
 // Activations in 8 bits: OCP e4m3 codes [M, N] and one power-of-two scale per row and 32 columns
 // [M, ceil(N / 32)], stored as the biased exponent e + 127 (the scale's fp32 exponent byte).
+//
+// At the largest scale 2^120 magnitudes from 248 * 2^120 on have the code of 256, and 2^128 is past fp32 and
+// bf16: that code reads as 240 there, the largest finite value of the format (at most 2^-4 off, half an e4m3 step).
 #pragma once
 #include "common.h"
 
@@ -36,16 +39,44 @@ __device__ __forceinline__ uint32_t a8_pack4(float a, float b, float c, float d,
   return r;
 }
 
-// 8 codes (two words) -> 8 fp32 values times the scale (exact: 4 significant bits)
-__device__ __forceinline__ void a8_unpack8(uint2 w, float s, float (&f)[8]) {
+// 4 codes with those of +-256 made 240 where their scale's byte is the largest: a byte of m is 0 for the code
+// 0x78 of either sign, and only then (m + 0x7F) has no bit 7, without a carry to the next byte.
+__device__ __forceinline__ uint32_t a8_finite(uint32_t w, uint32_t scale) {
+  const uint32_t m = (w & 0x7F7F7F7Fu) ^ 0x78787878u;
+  return w - ((~(m + 0x7F7F7F7Fu) >> 7) & (scale == A8_EMAX + 127 ? 0x01010101u : 0u));
+}
+
+// The same for 8 words of one scale (the scale itself, not its byte), with a wave's branch over it (no lane has that scale but for values next to the
+// type's largest) that the compiler does not see, for loops whose registers do not survive a block.
+__device__ __forceinline__ void a8_finite_rare(uint32_t (&w)[8], float scale) {
+  uint32_t t, one;
+#define HFM_A8_WORD(i)                                                                                   \
+  "v_and_b32 %8, 0x7f7f7f7f, %" #i "\n\tv_xor_b32 %8, 0x78787878, %8\n\tv_add_u32 %8, 0x7f7f7f7f, %8\n\t" \
+  "v_not_b32 %8, %8\n\tv_lshrrev_b32 %8, 7, %8\n\tv_and_b32 %8, %9, %8\n\tv_sub_u32 %" #i ", %" #i ", %8\n\t"
+  asm volatile(
+      "v_cmp_eq_u32 vcc, %11, %10\n\ts_nop 4\n\ts_cmp_lg_u64 vcc, 0\n\ts_cbranch_scc0 .Lskip%=\n\t"
+      "v_mov_b32 %9, 0x01010101\n\tv_cndmask_b32 %9, 0, %9, vcc\n\t"
+      HFM_A8_WORD(0) HFM_A8_WORD(1) HFM_A8_WORD(2) HFM_A8_WORD(3)
+      HFM_A8_WORD(4) HFM_A8_WORD(5) HFM_A8_WORD(6) HFM_A8_WORD(7)
+      "s_nop 1\n.Lskip%=:"
+      : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]), "=&v"(t), "=&v"(one)
+      : "v"(scale), "s"((A8_EMAX + 127) << 23)
+      : "vcc", "scc");
+#undef HFM_A8_WORD
+}
+
+// 8 codes (two words) -> 8 fp32 values times their scale (its byte; exact: 4 significant bits)
+__device__ __forceinline__ void a8_unpack8(uint2 w, uint32_t scale, float (&f)[8]) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const float s = a8_scale(scale);
+  w = make_uint2(a8_finite(w.x, scale), a8_finite(w.y, scale));
   const f32x2 p0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), p1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true);
   const f32x2 p2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false), p3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true);
   f[0] = p0[0] * s; f[1] = p0[1] * s; f[2] = p1[0] * s; f[3] = p1[1] * s;
   f[4] = p2[0] * s; f[5] = p2[1] * s; f[6] = p3[0] * s; f[7] = p3[1] * s;
 }
 
-// 2 codes (the low or high half of a word) -> 2 bf16 values times the scale, exact: one conversion
+// 2 codes (the low or high half of a word, after a8_finite) -> 2 bf16 values times the scale, exact: one conversion
 template <bool HI>
 __device__ __forceinline__ uint32_t a8_pair_bf16(uint32_t w, float s) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

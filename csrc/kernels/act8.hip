@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(Act8Args a) {
       if (j < n) (j < 4 ? w.x : w.y) |= (uint32_t)s[j] << (8 * (j & 3));
   }
   float f[8];
-  a8_unpack8(w, a8_scale(a.scales[row * nb + c / A8_BLOCK]), f);
+  a8_unpack8(w, a.scales[row * nb + c / A8_BLOCK], f);
   if (n < 8) {
 #pragma unroll
     for (int j = 0; j < 7; ++j)

@@ -946,7 +946,7 @@ __global__ void __launch_bounds__(256) group_wgrad_kernel(GroupWgArgs g, int til
       for (int m = 0; m < 8; ++m) {
         if (!WHOLE) end8_code(w[m], col, g.K);
         float f[8];
-        a8_unpack8(make_uint2((uint32_t)w[m], (uint32_t)(w[m] >> 32)), a8_scale(sc[m]), f);
+        a8_unpack8(make_uint2((uint32_t)w[m], (uint32_t)(w[m] >> 32)), sc[m], f);
         bf16x8 v;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = f2bf(f[j]);
@@ -1267,6 +1267,14 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
     };
     auto codes_put = [&](int set, int s, int q) {
       const float f = a8_scale(cs[set]);
+      if (q == 0) {
+        uint32_t u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = cd[set][i >> 1][i & 1];
+        a8_finite_rare(u, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cd[set][i >> 1][i & 1] = u[i];
+      }
       const uint32_t a = GATHER ? cd[set][q][0] & con[set] : cd[set][q][0], b = GATHER ? cd[set][q][1] & con[set] : cd[set][q][1];
       lds_put(smem + (s & (GP_RING - 1)) * GP_BUF + (xo ^ (q << 4)), a8_pair_bf16<false>(a, f), a8_pair_bf16<true>(a, f),
               a8_pair_bf16<false>(b, f), a8_pair_bf16<true>(b, f));

@@ -6,7 +6,8 @@ columns: 1.03 bytes a value instead of 2 or 4.  A block's scale is the smallest 
 x / 2^e (ties to even).  Two rules serve the backward pass: a value that is not zero never becomes
 a zero (it takes the smallest code of its sign instead), so a relu or dropout mask read from the
 codes is the mask of the activations themselves; and infinities and NaN become NaN, in their own
-place only.
+place only.  A finite value stays finite: the code of 256 at the scale 2^120, of magnitudes from 248 *
+2^120 on, stands for 240 * 2^120, because 2^128 is past fp32 and bf16.
 
 The codes go into the gradient products as they are: ``experts.group_wgrad`` takes an ``Act8`` for
 its input, ``experts.group_dgrad`` for its mask.
@@ -81,8 +82,8 @@ def pack(x: torch.Tensor, out: Optional[Act8] = None) -> Act8:
 
 
 def unpack(a: Act8, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The values that ``a`` stands for, in fp32 or bf16 (exact in both, but where a value of a
-    block with the smallest scales lies below the type's normal range)."""
+    """The values that ``a`` stands for, in fp32 or bf16 (exact in both: four significant bits, and magnitudes from
+    2^-119 to 240 * 2^120)."""
     ldc = check_own_act8(a, "a")
     M, N = a.codes.shape
     if dtype not in _VALUES:

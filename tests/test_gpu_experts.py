@@ -796,3 +796,46 @@ def test_weight_gradient_from_columns_of_wider_codes(K, off):
             c = 1.01 * (hi - lo + 4) * 2.0 ** -23
             assert bool(((dw[e].double() - z.T @ v[lo:hi]).abs() <= c * (z.abs().T @ v[lo:hi].abs())).all()), (len(kw), e)
             assert bool(((db[e].double() - z.sum(0)).abs() <= c * z.abs().sum(0)).all()), (len(kw), e)
+
+
+def next_to_the_largest(g, S, K, dtype):
+    """Rows of ordinary values, some with one of the largest magnitudes in blocks here and there."""
+    x = torch.randn(S, K, device=DEV, generator=g)
+    big = torch.tensor([3.4028234e38, -3.4028234e38, 248 * 2.0 ** 120, -247.9 * 2.0 ** 120, 255.0 * 2.0 ** 120, 3.3895314e38], device=DEV)
+    for i in range(0, S, 97):
+        x[i, (7 * i) % K] = big[i % 6]
+    x[5 % S, 3 % K] = math.nan
+    return x.clamp(-3.3895314e38, 3.3895314e38).to(dtype) if dtype == torch.bfloat16 else x
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N", [(300, 36), (1000, 401), (64, 4096)])
+def test_finite_values_stay_finite_in_8_bits(M, N, dtype):
+    """Up to the type's largest: half an e4m3 step, 2^-4 of a value in the format's normal range."""
+    _, A8 = ops()
+    x = next_to_the_largest(torch.Generator(device=DEV).manual_seed(N), M, N, dtype)
+    a = A8.pack(x)
+    u, v = A8.unpack(a, torch.float32), A8.unpack(a, torch.bfloat16)
+    assert torch.equal(torch.isnan(u), torch.isnan(x)) and not torch.isinf(u).any()
+    assert torch.equal(u.nan_to_num(nan=7.0), v.float().nan_to_num(nan=7.0))
+    large = x.abs() >= 2.0 ** 115
+    assert large.any() and bool(((u.double() - x.double()).abs() <= 2.0 ** -4 * x.double().abs())[large].all())
+
+
+@pytest.mark.parametrize("S,N,K", [(600, 64, 96), (600, 33, 100), (16384, 512, 256), (16384, 512, 600)])
+def test_weight_gradient_from_8_bits_next_to_the_largest(S, N, K):
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(S + K)
+    x = next_to_the_largest(g, S, K, torch.float32).nan_to_num(nan=0.0)
+    dz = (torch.randn(S, N, device=DEV, generator=g) * 2.0 ** -12).bfloat16()
+    dz[::3] = 0
+    a = A8.pack(x)
+    v = A8.unpack(a, torch.float32).double()
+    assert bool((v.abs() >= 240 * 2.0 ** 120).any())
+    o = torch.tensor([0, S // 2, S], dtype=torch.int32, device=DEV)
+    src = torch.arange(S, dtype=torch.int32, device=DEV)
+    for kw in (dict(), dict(src=src)):
+        dw, _ = EX.group_wgrad(dz, a, o, **kw)
+        for e, (lo, hi) in enumerate(((0, S // 2), (S // 2, S))):
+            z = dz[lo:hi].double()
+            assert bool(((dw[e].double() - z.T @ v[lo:hi]).abs() <= 1.01 * (hi - lo + 4) * 2.0 ** -23 * (z.abs().T @ v[lo:hi].abs())).all())
