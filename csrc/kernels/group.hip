@@ -1230,7 +1230,8 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       }
     };
     // X8: a step's codes and scale into registers (set), and from there into the image.  Rows past p1 are zeros: by
-    // the buffer's end; where src says the rows, cleared on the way to the image, where the loads have arrived.
+    // the buffer's end; where src says the rows, cleared on the way to the image, where the loads have arrived (the
+    // scale too: what row 0 has there may be no scale at all, and zero times it no zero).
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     u32x2 cd[2][4];
     uint32_t cs[2], con[2];
@@ -1266,7 +1267,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
       }
     };
     auto codes_put = [&](int set, int s, int q) {
-      const float f = a8_scale(cs[set]);
+      const float f = a8_scale(GATHER ? cs[set] & con[set] : cs[set]);
       if (q == 0) {
         uint32_t u[8];
 #pragma unroll

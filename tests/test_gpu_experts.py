@@ -839,3 +839,22 @@ def test_weight_gradient_from_8_bits_next_to_the_largest(S, N, K):
         for e, (lo, hi) in enumerate(((0, S // 2), (S // 2, S))):
             z = dz[lo:hi].double()
             assert bool(((dw[e].double() - z.T @ v[lo:hi]).abs() <= 1.01 * (hi - lo + 4) * 2.0 ** -23 * (z.abs().T @ v[lo:hi].abs())).all())
+
+
+@pytest.mark.parametrize("S,N,K", [(600, 64, 96), (16384, 512, 256), (16384, 512, 600)])
+def test_places_without_a_row_read_zeros_whatever_row_0_holds(S, N, K):
+    """Sources that are no slot of a row, beside a row 0 of x that nobody packed: codes and scales of any bits."""
+    EX, A8 = ops()
+    g = torch.Generator(device=DEV).manual_seed(S + K)
+    dz, x = (torch.randn(*s, device=DEV, generator=g).bfloat16() for s in ((S, N), (S, K)))
+    a = A8.pack(x)
+    o = torch.tensor([0, S // 2, S], dtype=torch.int32, device=DEV)
+    src = torch.randint(1, S, (S,), device=DEV, generator=g).int()
+    src[::3] = -1
+    src[1::5] = S
+    want = EX.group_wgrad(dz, a, o, src=src)
+    assert bool(torch.isfinite(want[0]).all())
+    for code, scale in ((0x33, 255), (0x7F, 0), (0xFF, 255)):
+        a.codes[0], a.scales[0] = code, scale
+        got = EX.group_wgrad(dz, a, o, src=src)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (code, scale)
