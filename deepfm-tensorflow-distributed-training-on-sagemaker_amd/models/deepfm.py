@@ -532,7 +532,7 @@ class NativeDeepFM(GraphRunnerMixin, NativeStateMixin, LayerPathMixin):
         self.y_fm = torch.zeros(M, **f32)
         self.S = torch.zeros(M, K, **f32)
         self.E = torch.zeros(M, K0p, **bf)
-        self.Et = torch.zeros(K0p, M, **bf)
+        self.Et = None if self.act8 else torch.zeros(K0p, M, **bf)      # (act8: the gradient takes rows of E)
         if self.fp8:
             self.E8 = torch.zeros(M, K0p, dtype=torch.uint8, device=dev)
             self.sE = torch.ones(M, **f32)

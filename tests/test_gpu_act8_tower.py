@@ -93,3 +93,14 @@ def test_a_larger_batch_and_evaluation():
         m.train_step(*data[1])
     torch.cuda.synchronize()
     assert torch.equal(a.p, b.p) and a.H8[0].codes.shape[0] == 512
+
+
+def test_no_transposed_copies():
+    """Neither kept nor written: the gradient products take rows."""
+    layers, B = [1024, 256], 300
+    synth, params, data = setup(layers, B)
+    m = make(synth, layers, [1.0, 1.0], B, "fp8", params)
+    m.train_step(*data[0])
+    torch.cuda.synchronize()
+    m.check_errors()
+    assert m.Et is None and m.Ht is None and m.dZt is None
