@@ -104,3 +104,50 @@ def test_no_transposed_copies():
     torch.cuda.synchronize()
     m.check_errors()
     assert m.Et is None and m.Ht is None and m.dZt is None
+
+
+@pytest.mark.parametrize("layers,keep", [([96, 160, 64], [0.5, 1.0, 0.8]), ([1024, 256, 512], [0.9, 0.5, 1.0]),
+                                         ([64, 160, 96, 32], [1.0, 0.5, 0.5, 1.0]), ([256, 1024, 128, 512], [0.5, 0.9, 1.0, 0.5])])
+def test_layers_that_share_buffers(layers, keep):
+    """H and dZ of layers two apart lie in one buffer, at other widths.  Every layer's dZ, as its weight gradient takes it,
+    against the product of the layer above's in 64 bits, and its gradients against those of this dZ and the default tower's
+    activations; in a second step too, whose batch leaves rows of the first one's behind it."""
+    from hipfm.ops import act8 as A8
+    synth, params, (first, second) = setup(layers, 601, steps=2)
+    m, d = (make(synth, layers, keep, 601, t, params) for t in ("fp8", "bf16"))
+    taken, wgrad = {}, m._wgrad_act8
+
+    def keep_dz(i):
+        taken[i] = m.dZ[i].clone()
+        wgrad(i)
+
+    m._wgrad_act8 = keep_dz
+    for batch in (first, [t[:333].contiguous() for t in second]):
+        wts = [w.clone() for w in m.WT16]                      # (the optimizer refreshes them)
+        for t in (m, d):
+            t.train_step(*batch)
+        torch.cuda.synchronize()
+        m.check_errors()
+        g = {n: m.g[s.off:s.off + int(torch.Size(s.shape).numel())].view(s.shape).double().cpu()
+             for n, s in m.dense_segs.items()}
+        assert torch.equal(m.prob, d.prob) and torch.equal(m.E, d.E)
+        top = len(layers) - 1
+        assert torch.equal(taken[top], d.dZ[top])
+        for i in reversed(range(top + 1)):
+            x = A8.unpack(A8.pack(d.H[i - 1]), torch.float32) if i else m.E
+            for what, right in (("weights", x), ("biases", torch.ones(m.M, 1, device=DEV))):
+                w, bound = dsum(taken[i], right)
+                got = g[f"Deep-part/mlp{i}/{what}"]
+                assert ((got - w.view(got.shape)).abs() <= bound.view(got.shape)).all(), (i, what)
+            if i:
+                s = 1.0 / keep[i - 1]
+                prod, bound = dsum(taken[i].t(), wts[i].view(m.Np[i - 1], m.Np[i]).t())
+                prod, bound = s * prod, s * bound + 2.0 ** -23 * s * prod.abs()      # (the scale's own rounding and its product's)
+                on = x.double().cpu() > 0
+                want = torch.where(on, prod, torch.zeros(()).double())
+                assert ((taken[i - 1].double().cpu() - want).abs() <= bound + 2.0 ** -8 * (prod.abs() + bound)).all(), i
+                assert (taken[i - 1].cpu()[~on] == 0).all() and on.any(), i
+        # the second step starts from the same parameters
+        d.p.copy_(m.p)
+        d.rec.copy_(m.rec)
+        d.refresh_shadows()
