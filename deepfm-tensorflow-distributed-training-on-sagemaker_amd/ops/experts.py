@@ -31,7 +31,7 @@ the current stream, so calls on several streams and in several graphs share noth
 ``out`` shares no memory with the operands, but ``combine_bwd`` may write over ``ys`` and ``group_dgrad`` over a
 bf16 ``mask``.
 
-Any widths and strides are taken.  Large products are fastest where rows start on 16 bytes and widths are
+Any widths and strides are taken, sizes up to 2^31 - 1024.  Large products are fastest where rows start on 16 bytes and widths are
 multiples of 8 (16 for 8-bit ``x``): operands that are otherwise are copied in the call.
 """
 from __future__ import annotations
@@ -49,6 +49,7 @@ from .checks import call, flat, out_or_new, rows2d
 MAX_EXPERTS = 1024
 MAX_TOP_K = 16
 _MAX_SLOTS = 1 << 30
+_MAX_SIZE = (1 << 31) - 1024          # grouped products: int32 that counts on to the next whole tiles
 _VALUES = (torch.float32, torch.bfloat16)
 _BF = (torch.bfloat16,)
 _EX_DISPATCH, _EX_DISPATCH_BWD, _EX_COMBINE, _EX_COMBINE_BWD = 0, 1, 2, 3
@@ -200,9 +201,14 @@ def _check_groups(offs, E):
     flat(offs, "offs", torch.int32, (E + 1,))
 
 
+def _check_sizes(*sizes):
+    if max(sizes) > _MAX_SIZE:
+        raise ValueError(f"rows, widths and experts up to {_MAX_SIZE}, got {sizes}")
+
+
 def _check_gather(src, top_k, S):
-    if not (isinstance(top_k, int) and top_k >= 1):
-        raise ValueError(f"top_k must be a positive int, got {top_k}")
+    if not (isinstance(top_k, int) and 1 <= top_k <= _MAX_SIZE):
+        raise ValueError(f"top_k must be an int from 1 to {_MAX_SIZE}, got {top_k}")
     if src is not None:
         flat(src, "src", torch.int32, (S,))
     elif top_k != 1:
@@ -250,6 +256,7 @@ def group_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     _check_groups(offs, E)
     S = x.shape[0] if src is None else src.shape[0]
     _check_gather(src, top_k, S)
+    _check_sizes(S, x.shape[0], E, N, K)
     if bias is not None:
         flat(bias, "bias", torch.float32, (E, N))
     if out is not None:
@@ -274,6 +281,7 @@ def group_dgrad(dz: torch.Tensor, wt: torch.Tensor, offs: torch.Tensor,
     _check_weight(wt, "wt", dz.shape[1])
     E, K, N = wt.shape
     _check_groups(offs, E)
+    _check_sizes(S, E, N, K)
     m, ldm, m8 = None, 0, 0
     if isinstance(mask, Act8):
         m, ldm, m8 = mask.codes, check_act8(mask, S, K, "mask"), 1
@@ -311,6 +319,7 @@ def group_wgrad(dz: torch.Tensor, x: Union[torch.Tensor, Act8], offs: torch.Tens
     E = offs.shape[0] - 1
     _check_groups(offs, E)
     _check_gather(src, top_k, S)
+    _check_sizes(S, xv.shape[0], E, N, K)
     if src is None and xv.shape[0] != S:
         raise ValueError(f"x must have {S} rows, got {xv.shape[0]}")
     if out is None:

@@ -108,3 +108,29 @@ GOOD = {
 def test_host_tensors_refused(name):
     with pytest.raises(ValueError, match=f"{name} runs on the GPU"):
         GOOD[name]()
+
+
+def meta(*s, dtype=BF):
+    return torch.empty(*s, dtype=dtype, device="meta")
+
+
+PAST = 2 ** 32 + 4             # (4 in 32 bits)
+WIDE = {
+    "linear slots": lambda: EX.group_linear(meta(4, 8), meta(1, 8, 8), None, meta(2, dtype=I32), src=meta(PAST, dtype=I32)),
+    "linear columns": lambda: EX.group_linear(meta(4, 8), meta(1, 1, 8).expand(1, PAST, 8), None, meta(2, dtype=I32)),
+    "linear experts": lambda: EX.group_linear(meta(4, 8), meta(1, 8, 8).expand(PAST, 8, 8), None, meta(PAST + 1, dtype=I32)),
+    "linear rows of the last tile": lambda: EX.group_linear(meta(2 ** 31 - 1, 1), meta(1, 8, 1), None, meta(2, dtype=I32)),
+    "linear top_k": lambda: EX.group_linear(meta(4, 8), meta(1, 8, 8), None, meta(2, dtype=I32), src=meta(5, dtype=I32), top_k=PAST),
+    "dgrad rows of the last tile": lambda: EX.group_dgrad(meta(2 ** 31 - 1, 1), meta(1, 8, 1), meta(2, dtype=I32)),
+    "dgrad columns": lambda: EX.group_dgrad(meta(4, 8), meta(1, 1, 8).expand(1, PAST, 8), meta(2, dtype=I32)),
+    "wgrad experts": lambda: EX.group_wgrad(meta(4, 8), meta(4, 8), meta(PAST + 1, dtype=I32)),
+    "wgrad rows of the last tile": lambda: EX.group_wgrad(meta(2 ** 31 - 1, 1), meta(2 ** 31 - 1, 1), meta(2, dtype=I32)),
+    "wgrad top_k": lambda: EX.group_wgrad(meta(4, 8), meta(4, 8), meta(2, dtype=I32), src=meta(4, dtype=I32), top_k=PAST),
+}
+
+
+@pytest.mark.parametrize("name", sorted(WIDE))
+def test_sizes_past_32_bits_refused(name):
+    with pytest.raises(ValueError) as e:
+        WIDE[name]()
+    assert "runs on the GPU" not in str(e.value), "its size would reach the kernel in 32 bits"
