@@ -81,6 +81,10 @@ __device__ __forceinline__ bool group_find(const int* offs, int E, int S, int tm
   return false;
 }
 
+// The kernels that count the rows of all groups in one line do so in 32 bits.  Offsets that are not in order may give every
+// second group all rows (a group ends where the next one begins), in units of 64 rows and 7 more a group, at most.
+static bool groups_count(int E, int S) { return (E / 2 + 1l) * (S / 64 + 1l) + 7l * E < 1l << 31; }
+
 // row tiles of all groups
 template <int BM>
 __device__ __forceinline__ int group_tiles(const int* offs, int E, int S) {
@@ -794,7 +798,7 @@ static NtPlan nt_plan(const GroupNtArgs& g) {
   const double step = odd_a || odd_b ? (st <= 256 ? 1.5 : 2.7) : (st <= 256 ? 1.2 : 1.4);
   const double small = ceil(st / 512) * (step * steps + 10.0) * (mask ? 1.4 : 1.0);
   NtPlan p{0, 0, 0, few < small && (long)(g.S / GS_B + groups) * ((g.N + GS_B - 1) / GS_B) <= 1l << 20};
-  if (g.K < 8 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD) return p;
+  if (g.K < 8 || g.K >= 0x7F00 || g.ldo >= GP_MAXLD || g.ldm >= GP_MAXLD || !groups_count(g.E, g.S)) return p;
   const int tn = (g.N + GP_B - 1) / GP_B;
   auto time = [&](int rows) {
     const double tiles = (groups == 1 ? (double)((g.S + rows - 1) / rows) : (double)g.S / rows + 0.5 * groups) * tn;
@@ -1424,7 +1428,8 @@ __global__ void __launch_bounds__(256) group_wgrad_join_kernel(GroupWgArgs g, in
 // 1024: 290, 115.
 constexpr int GW_CUS = 256, GP_MIN_UNITS = 2;
 static bool wgrad_big(const GroupWgArgs& g) {
-  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD || g.E > 65535) return false;      // (32-bit offsets; grid)
+  if (g.ldz >= 1l << 25 || g.ldx >= 1l << 25 || g.K >= GP_MAXLD || g.E > 65535 || !groups_count(g.E, g.S))
+    return false;                                          // (32-bit offsets; grid; the line's units)
   const long tiles = (long)((g.N + GP_B - 1) / GP_B) * ((g.K + GP_B - 1) / GP_B);
   return g.rows > 0 && tiles <= 1l << 20 && tiles * (g.S / GW_UNIT) >= (long)GW_CUS * GP_MIN_UNITS / (g.xs ? 2 : 1);
 }

@@ -1,8 +1,11 @@
 """Refusals of the expert and 8-bit operators: the same with and without a GPU, before anything is
 launched."""
+import ctypes as C
+
 import pytest
 import torch
 
+from hipfm.ops import _lib
 from hipfm.ops import act8 as A8
 from hipfm.ops import experts as EX
 
@@ -134,3 +137,20 @@ def test_sizes_past_32_bits_refused(name):
     with pytest.raises(ValueError) as e:
         WIDE[name]()
     assert "runs on the GPU" not in str(e.value), "its size would reach the kernel in 32 bits"
+
+
+def nt_args(**kw):
+    d = dict(lda=kw["K"], ldb=kw["K"], es=0, ldo=kw["N"], rows=kw["S"], top_k=1, scale=1.0)
+    return _lib.GroupNtArgs(**{**d, **kw})
+
+
+def test_lines_of_rows_are_counted_in_32_bits():
+    """Where offsets that are not in order could make the count of all groups' rows overflow, the kernels that count them
+    are not taken (seen by their workspace: copies of the odd rows, slabs for the bias)."""
+    lib = _lib.get_lib()
+    for E, large in ((1, True), (1024, True), (1 << 14, False), (1 << 16, False), (1 << 17, False)):
+        a = nt_args(S=1 << 24, E=E, K=1024, N=256, lda=1025)
+        assert (lib.hfm_group_nt_ws_bytes(C.byref(a)) > 0) == large, E
+    for E, S, large in ((1, 1 << 24, True), (1024, 1 << 24, True), (65535, 1 << 22, False), (65535, 1 << 21, True)):
+        b = _lib.GroupWgArgs(S=S, rows=S, E=E, K=8, N=8, ldz=8, ldx=8, top_k=1, ns=1, db=16)
+        assert (lib.hfm_group_wgrad_ws_floats(C.byref(b)) > 0) == large, E
