@@ -866,7 +866,7 @@ HFM_API int hfm_group_nt(const GroupNtArgs* gp, hipStream_t st) {
   }
   const int tn = (g.N + GN_B - 1) / GN_B;
   const long blocks = (g.S / GN_B + groups) * tn;
-  if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
+  if (blocks > 0xFFFFFFl) return (int)hipErrorInvalidValue;       // (a launch has less than 2^32 threads in x)
   hipLaunchKernelGGL(group_nt_kernel, dim3((unsigned)blocks), dim3(256), 0, st, g, tn);
   HFM_LAUNCH_CHECK();
 }
@@ -1556,7 +1556,7 @@ HFM_API int hfm_group_wgrad(const GroupWgArgs* gp, hipStream_t st) {
   if (g.ns > 1 && !g.ws) return (int)hipErrorInvalidValue;
   const int tn = (g.N + GN_B - 1) / GN_B, tk = g.K > 0 ? (g.K + GN_B - 1) / GN_B : 1;
   const long blocks = (long)tn * tk * g.E * g.ns;
-  if (blocks > 0x7FFFFFFFl) return (int)hipErrorInvalidValue;
+  if (blocks > 0xFFFFFFl) return (int)hipErrorInvalidValue;       // (a launch has less than 2^32 threads in x)
   const dim3 grid((unsigned)blocks), blk(256);
   if (g.N % 8 == 0 && g.K % 8 == 0) {
     if (g.xs) hipLaunchKernelGGL((group_wgrad_kernel<true, true>), grid, blk, 0, st, g, tn, tk);

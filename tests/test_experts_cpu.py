@@ -154,3 +154,11 @@ def test_lines_of_rows_are_counted_in_32_bits():
     for E, S, large in ((1, 1 << 24, True), (1024, 1 << 24, True), (65535, 1 << 22, False), (65535, 1 << 21, True)):
         b = _lib.GroupWgArgs(S=S, rows=S, E=E, K=8, N=8, ldz=8, ldx=8, top_k=1, ns=1, db=16)
         assert (lib.hfm_group_wgrad_ws_floats(C.byref(b)) > 0) == large, E
+
+
+def test_launches_past_the_grid_refused():
+    """Before anything is launched (1: an invalid value; a launch without a GPU gives another error)."""
+    lib = _lib.get_lib()
+    a = nt_args(S=1 << 25, E=1 << 25, K=4, N=128)
+    b = _lib.GroupWgArgs(S=8, rows=8, E=1 << 25, K=1, N=1, ldz=1, ldx=1, top_k=1, ns=1)
+    assert lib.hfm_group_nt(C.byref(a), None) == 1 and lib.hfm_group_wgrad(C.byref(b), None) == 1
