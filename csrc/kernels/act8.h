@@ -47,7 +47,8 @@ __device__ __forceinline__ uint32_t a8_finite(uint32_t w, uint32_t scale) {
 }
 
 // The same for 8 words of one scale (the scale itself, not its byte), with a wave's branch over it (no lane has that scale but for values next to the
-// type's largest) that the compiler does not see, for loops whose registers do not survive a block.
+// type's largest) that the compiler does not see, for loops whose registers do not survive a block (16384 x 4096 x 4096: 4 us
+// of 450; by a8_finite it would be 56 instructions more in every step).
 __device__ __forceinline__ void a8_finite_rare(uint32_t (&w)[8], float scale) {
   uint32_t t, one;
 #define HFM_A8_WORD(i)                                                                                   \

@@ -601,8 +601,8 @@ __device__ __forceinline__ void mm_out_nt(const GroupNtArgs& g, const f32x16 (&a
   }
 }
 
-// ---- NT: rows of A and B are K-contiguous, and 32-deep steps would ask the L2 for half lines (57 % of its
-// channels' cycles were requests, 28 % now): so steps of 64 (rows of 128 B, 16-byte chunk c of row r at
+// ---- NT: rows of A and B are K-contiguous, and 32-deep steps would ask the L2 for half lines (with whole ones 24 to 41 %
+// of its channels' cycles are requests already): so steps of 64 (rows of 128 B, 16-byte chunk c of row r at
 // c ^ ((r >> 1) & 7)), A's in a ring of three panels and w's in two, which is all of the LDS.  A step is two halves
 // of 32: in half 0 the fragments of half 1 are read, and in half 1, after its second round, comes the step's one
 // barrier: the wave has read all of its panels, and its DMA of the next step has landed.  Then the next step's
@@ -1171,7 +1171,7 @@ group_wgrad_mm_kernel(GroupWgArgs g, int tiles_n, int tiles_k, int lanes) {
   const int sblk = (g.K + A8_BLOCK - 1) / A8_BLOCK;
   // 8-bit x: 32 codes (granules 2 xq, 2 xq + 1) of row xr, in four pieces of 8 (16 bytes as bf16).  A lane's piece in
   // turn q is q ^ xp: eight neighbouring lanes then write to eight different 16-byte places of 128 bytes (all in
-  // the same order: four in one place, half of the LDS cycles were conflicts, 16384 x 4096 x 4096 took 466 us, 434 so).
+  // the same order: four in one place, half of the LDS cycles were conflicts, a product of 466 us took 434 so).
   const int xr = threadIdx.x >> 3, xq = threadIdx.x & 7, xc = xq * 32, xp = xq >> 1;
   const int xf = ((xr & 3) << 1) | ((xr >> 3) & 1);
   const int xo = GP_PANEL + xr * 512 + ((((2 * xq) ^ xf) << 5) ^ (xp << 4));           // (piece of turn q: ^ q << 4)

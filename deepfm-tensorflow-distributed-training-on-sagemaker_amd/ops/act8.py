@@ -5,8 +5,8 @@ columns: 1.03 bytes a value instead of 2 or 4.  A block's scale is the smallest 
 120]) that keeps its largest finite magnitude within 448; a code is the e4m3 value nearest to
 x / 2^e (ties to even).  Two rules serve the backward pass: a value that is not zero never becomes
 a zero (it takes the smallest code of its sign instead), so a relu or dropout mask read from the
-codes is the mask of the activations themselves; and infinities and NaN become NaN, in their own
-place only.  A finite value stays finite: the code of 256 at the scale 2^120, of magnitudes from 248 *
+codes is the mask of the finite activations themselves; and infinities and NaN become NaN, in their own
+place only (a mask is zero there).  A finite value stays finite: the code of 256 at the scale 2^120, of magnitudes from 248 *
 2^120 on, stands for 240 * 2^120, because 2^128 is past fp32 and bf16.
 
 The codes go into the gradient products as they are: ``experts.group_wgrad`` takes an ``Act8`` for
